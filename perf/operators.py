@@ -377,7 +377,8 @@ def _run_own(state):
         return {"table": state["table"], "pool": _values(state)}
     rows = state.get("rows")
     if rows is None:
-        rows = state["rows"] = cache.rows(state["slot"], state["pos0"], state["row0"], state["max_rows"])
+        rows = state["rows"] = cache.rows(state["slot"], state["pos0"],
+                                          state["row0"] if state["max_rows"] > 1 else None, state["max_rows"])
     if case["op"] == "attend":
         return cache.attend(0, rows, state["q"], window=case["window"], sinks=case["sinks"], out=state["out"])
     if case["rot"]:
