@@ -1,4 +1,4 @@
-"""ctypes binding of `include/fmd_decoder.h` (libfmd_decoder.so).
+"""ctypes binding of the headers in `include/` (libfmd_decoder.so).
 
 The library is built in-tree (`csrc/build.py`) and loaded from the package
 directory; there is no CPU fallback -- if the library or a GPU is missing,
@@ -33,6 +33,9 @@ DT_F32, DT_F16, DT_BF16, DT_Q8_0 = 0, 1, 2, 3
 
 FINISH_STOP, FINISH_LENGTH, FINISH_ERROR = 0, 1, 2
 
+# cache formats (fmd_cache.h)
+CACHE_F16, CACHE_BF16, CACHE_Q4 = 1, 2, 4
+
 # every symbol the header declares
 EXPORTS = [
     "fmd_create", "fmd_destroy", "fmd_last_error", "fmd_status_string", "fmd_version", "fmd_load_weights",
@@ -45,6 +48,10 @@ EXPORTS = [
     "fmd_audio_create", "fmd_audio_destroy", "fmd_audio_last_error", "fmd_audio_memory_bytes", "fmd_audio_encode",
     "fmd_audio_encode_audio", "fmd_audio_token_offsets", "fmd_audio_last_timing", "fmd_mel_create", "fmd_mel_destroy", "fmd_mel_last_error",
     "fmd_mel_log_mel", "fmd_mel_filters",
+    # include/fmd_cache.h
+    "fmd_cache_block_bytes", "fmd_cache_pool_bytes", "fmd_cache_append", "fmd_cache_read",
+    "fmd_cache_attend_workspace", "fmd_cache_attend", "fmd_cache_copy_pages", "fmd_cache_fork",
+    "fmd_cache_compact_workspace", "fmd_cache_compact",
 ]
 
 
@@ -125,6 +132,29 @@ class FeatureConfig(C.Structure):
         "feature_size", "sampling_rate", "hop_length", "n_fft", "n_samples", "nb_max_frames")]
 
 
+class Cache(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("page_table", C.c_void_p)] + [(n, C.c_int32) for n in (
+        "format", "layers", "n_pages", "kv_heads", "head_dim", "max_slots", "max_pages_per_slot", "reserved")]
+
+
+class CacheRows(C.Structure):
+    _fields_ = [("slot", C.c_void_p), ("pos0", C.c_void_p), ("row0", C.c_void_p)] + [(n, C.c_int32) for n in (
+        "n_seqs", "n_rows", "max_rows", "reserved")]
+
+
+class CacheAppendArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "q", "q_out")] + [(n, C.c_int64) for n in (
+        "k_row", "k_head", "v_row", "v_head", "q_row", "q_head", "q_out_row", "q_out_head")] + [
+        (n, C.c_void_p) for n in ("q_norm", "k_norm", "cos_table", "sin_table")] + [("eps", C.c_float)] + [
+        (n, C.c_int32) for n in ("dtype", "n_heads", "rot_dim", "table_rows", "interleaved")]
+
+
+class CacheAttendArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p)] + [(n, C.c_int64) for n in (
+        "q_row", "q_head", "out_row", "out_head")] + [("scale", C.c_float)] + [
+        (n, C.c_int32) for n in ("dtype", "n_heads", "window", "sinks")]
+
+
 _lib = None
 
 
@@ -184,6 +214,17 @@ def load() -> C.CDLL:
         "fmd_mel_last_error": (C.c_char_p, [P]),
         "fmd_mel_log_mel": (C.c_int, [P, P, I32, P]),
         "fmd_mel_filters": (C.c_int, [C.POINTER(FeatureConfig), C.POINTER(C.c_float)]),
+        "fmd_cache_block_bytes": (I64, [I32, I32]),
+        "fmd_cache_pool_bytes": (I64, [C.POINTER(Cache)]),
+        "fmd_cache_append": (C.c_int, [C.POINTER(Cache), I32, C.POINTER(CacheRows), C.POINTER(CacheAppendArgs), P, P]),
+        "fmd_cache_read": (C.c_int, [C.POINTER(Cache), I32, C.POINTER(CacheRows), P, P, P, P]),
+        "fmd_cache_attend_workspace": (I64, [C.POINTER(Cache), I32, I32, I32]),
+        "fmd_cache_attend": (C.c_int, [C.POINTER(Cache), I32, C.POINTER(CacheRows), C.POINTER(CacheAttendArgs), P, I64,
+                                       P, P]),
+        "fmd_cache_copy_pages": (C.c_int, [C.POINTER(Cache), I32, IP, IP, P]),
+        "fmd_cache_fork": (C.c_int, [C.POINTER(Cache), I32, IP, IP, IP, IP, P, P]),
+        "fmd_cache_compact_workspace": (I64, [C.POINTER(Cache)]),
+        "fmd_cache_compact": (C.c_int, [C.POINTER(Cache), P, P, I64, P, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

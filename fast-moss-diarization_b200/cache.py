@@ -1,0 +1,533 @@
+"""A paged key/value cache and its operators (`include/fmd_cache.h`).
+
+`PagedCache` holds the keys and values of many sequences ("slots") in pages of
+64 positions, in the activations' 16 bits or in 4 bits, and offers what a
+decoder does with them: `append` rows (query / key norms and the rotation in
+the same pass), `attend` over them with a sliding window and sinks, `fork` a
+sequence, `evict` what a window no longer sees, `release` and `compact`. The
+pages' bookkeeping is on the host; the operators run on the current CUDA
+stream of the cache's device and never synchronise. Tensors are torch tensors
+(torch is only the allocator here). No counterpart in the reference, whose
+cache is one dense 16-bit tensor per layer (qwen3.rs:33-108).
+
+A decode loop:
+
+    rows = cache.step([0, 1], [1, 1])        # one new position each
+    for layer in range(layers):
+        q = cache.append(layer, rows, k, v, q=q, q_norm=..., cos=..., sin=...)
+        out = cache.attend(layer, rows, q, window=4096, sinks=4)
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import heapq
+from dataclasses import dataclass
+
+from . import _lib
+
+PAGE = 64
+_FORMATS = {"f16": _lib.CACHE_F16, "bf16": _lib.CACHE_BF16, "q4": _lib.CACHE_Q4}
+
+
+def _fail(message: str, status: int = _lib.FMD_EINVAL):
+    raise _lib.FmdError(status, message)
+
+
+@dataclass
+class CacheRows:
+    """The rows of a call (`fmd_cache_rows`): sequence i owns rows
+    `row0[i]:row0[i + 1]` (row i when `row0` is None) at positions `pos0[i]`,
+    `pos0[i] + 1`, ... of `slot[i]`; slot -1 is padding. All int32 device
+    tensors, so a captured graph reads what they hold when it is replayed."""
+
+    slot: object
+    pos0: object
+    row0: object
+    n_rows: int
+    max_rows: int
+
+    def advance(self, n: int = 1) -> None:
+        """Move every sequence on by `n` positions, on the device (the pages
+        must be there: `PagedCache.reserve`)."""
+        self.pos0.add_(n)
+
+    def to_c(self) -> _lib.CacheRows:
+        return _lib.CacheRows(self.slot.data_ptr(), self.pos0.data_ptr(),
+                              None if self.row0 is None else self.row0.data_ptr(), self.slot.shape[0], self.n_rows,
+                              self.max_rows, 0)
+
+
+class PagedCache:
+    """A cache of `n_pages` pages for up to `max_slots` sequences of up to
+    `64 * max_pages_per_slot` positions. `kind`: "f16" or "bf16" (rows of that
+    dtype) or "q4" (rows of either). `pool` and `page_table` may be the caller's
+    (uint8 of `pool_bytes`, int32 `[max_slots, max_pages_per_slot]`), with
+    `slots` as `(slot, its pages, its length)` for what they hold already."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, n_pages: int, max_slots: int,
+                 max_pages_per_slot: int, kind: str = "bf16", device="cuda", pool=None, page_table=None, slots=()):
+        import torch
+
+        self.lib = _lib.load()
+        if kind not in _FORMATS:
+            _fail(f"kind must be one of {sorted(_FORMATS)}, not {kind!r}")
+        if min(layers, kv_heads, n_pages, max_slots, max_pages_per_slot) < 1:
+            _fail("layers, kv_heads, n_pages, max_slots and max_pages_per_slot must be at least 1")
+        if head_dim not in (64, 128):
+            _fail(f"head_dim must be 64 or 128, not {head_dim}", _lib.FMD_ENOTSUP)
+        if max_pages_per_slot * PAGE > 2**31 - 1:
+            _fail("positions are 32-bit", _lib.FMD_ENOTSUP)
+        self.layers, self.kv_heads, self.head_dim, self.kind = layers, kv_heads, head_dim, kind
+        self.n_pages, self.max_slots, self.max_pages_per_slot = n_pages, max_slots, max_pages_per_slot
+        self.format = _FORMATS[kind]
+        self.pool_bytes = (layers * n_pages * 2 * kv_heads *
+                           int(self.lib.fmd_cache_block_bytes(self.format, head_dim)))
+        self.device = torch.device(device if pool is None else pool.device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        if pool is None:
+            pool = torch.zeros(self.pool_bytes, dtype=torch.uint8, device=self.device)
+        if page_table is None:
+            page_table = torch.full((max_slots, max_pages_per_slot), -1, dtype=torch.int32, device=self.device)
+        if pool.dtype != torch.uint8 or pool.numel() != self.pool_bytes or not pool.is_contiguous():
+            _fail(f"pool must be a contiguous uint8 tensor of {self.pool_bytes} bytes")
+        if (page_table.dtype != torch.int32 or tuple(page_table.shape) != (max_slots, max_pages_per_slot)
+                or not page_table.is_contiguous()):
+            _fail("page_table must be a contiguous int32 tensor [max_slots, max_pages_per_slot]")
+        if page_table.device != self.device:
+            _fail("pool and page_table must be on the same device")
+        self.pool, self.page_table = pool, page_table
+        self._c = _lib.Cache(pool.data_ptr(), page_table.data_ptr(), self.format, layers, n_pages, kv_heads, head_dim,
+                             max_slots, max_pages_per_slot, 0)
+        self._status = torch.zeros(2, dtype=torch.int32, device=self.device)
+        self._workspaces: dict = {}
+        # bookkeeping: pages of each open slot (-1: evicted), its length, names of each page
+        self._pages: list = [None] * max_slots
+        self._length = [0] * max_slots
+        self._names = [0] * n_pages
+        for slot, pages, length in slots:
+            if not 0 <= slot < max_slots or self._pages[slot] is not None:
+                _fail(f"bad slot {slot}")
+            if len(pages) > max_pages_per_slot or not 0 <= length <= PAGE * len(pages):
+                _fail(f"slot {slot}: {length} positions do not fit its pages")
+            if any(not -1 <= p < n_pages for p in pages):
+                _fail(f"slot {slot}: page out of range")
+            self._pages[slot], self._length[slot] = list(pages), length
+            for p in pages:
+                if p >= 0:
+                    self._names[p] += 1
+        self._free = [p for p in range(n_pages) if self._names[p] == 0]  # a heap: the lowest page goes first
+
+    # -- bookkeeping ---------------------------------------------------------------------
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, slot: int) -> int:
+        self._open(slot)
+        return self._length[slot]
+
+    def pages(self, slot: int) -> list:
+        """The slot's pages in order; -1 where `evict` freed one."""
+        return list(self._open(slot))
+
+    def _open(self, slot: int) -> list:
+        if not 0 <= slot < self.max_slots or self._pages[slot] is None:
+            _fail(f"slot {slot} is not open")
+        return self._pages[slot]
+
+    def open(self, slot: int, positions: int = 0) -> None:
+        """Open an empty sequence, with pages for its first `positions`."""
+        if not 0 <= slot < self.max_slots:
+            _fail(f"slot {slot} is out of range")
+        if self._pages[slot] is not None:
+            _fail(f"slot {slot} is already open", _lib.FMD_EBUSY)
+        self._pages[slot], self._length[slot] = [], 0
+        try:
+            self.reserve(slot, positions)
+        except _lib.FmdError:
+            self._pages[slot] = None
+            raise
+
+    def release(self, *slots: int) -> None:
+        """Close sequences; pages that no other slot names are free again."""
+        if len(set(slots)) != len(slots):
+            _fail("a slot is listed twice")
+        for s in slots:
+            self._open(s)
+        for s in slots:
+            for p in self._pages[s]:
+                self._drop(p)
+            self._pages[s], self._length[s] = None, 0
+
+    def _drop(self, page: int) -> None:
+        if page >= 0:
+            self._names[page] -= 1
+            if self._names[page] == 0:
+                heapq.heappush(self._free, page)
+
+    def _take(self) -> int:
+        p = heapq.heappop(self._free)
+        self._names[p] = 1
+        return p
+
+    def _upload(self, slot: int, first: int) -> None:
+        import torch
+
+        row = self._pages[slot][first:]
+        if row:
+            self.page_table[slot, first:first + len(row)].copy_(torch.tensor(row, dtype=torch.int32))
+
+    def reserve(self, slot: int, positions: int) -> None:
+        """Give the slot pages for its first `positions` positions."""
+        pages = self._open(slot)
+        need = -(-positions // PAGE)
+        if need > self.max_pages_per_slot:
+            _fail(f"slot {slot}: {positions} positions exceed {self.max_pages_per_slot} pages", _lib.FMD_EOVERFLOW)
+        have = len(pages)
+        if need - have > len(self._free):
+            _fail("the cache has too few free pages", _lib.FMD_ENOMEM)
+        if need > have:
+            pages += [self._take() for _ in range(need - have)]
+            self._upload(slot, have)
+
+    def step(self, slots, counts) -> CacheRows:
+        """Rows for `counts[i]` new positions of each slot, which become part of
+        its length: pass them to every layer's `append`, then `attend`. A page
+        that is shared with another slot and about to be written is copied
+        first."""
+        import torch
+
+        slots, counts = list(slots), list(counts)
+        if len(slots) != len(counts) or any(n < 0 for n in counts):
+            _fail("one count >= 0 per slot")
+        if len(set(slots)) != len(slots):
+            _fail("a slot is listed twice")
+        fresh = 0
+        for s, n in zip(slots, counts):
+            pages, at = self._open(s), self._length[s]
+            need = -(-(at + n) // PAGE)
+            if need > self.max_pages_per_slot:
+                _fail(f"slot {s}: {at + n} positions exceed {self.max_pages_per_slot} pages", _lib.FMD_EOVERFLOW)
+            fresh += max(0, need - len(pages))
+            fresh += sum(p < 0 or self._names[p] > 1 for p in pages[at // PAGE:need])
+        if fresh > len(self._free):
+            _fail("the cache has too few free pages", _lib.FMD_ENOMEM)
+        moves = []
+        for s, n in zip(slots, counts):
+            at = self._length[s]
+            need = -(-(at + n) // PAGE)
+            for k in range(at // PAGE, min(need, len(self._pages[s]))):
+                p = self._pages[s][k]
+                if p < 0 or self._names[p] > 1:
+                    self._pages[s][k] = self._take()
+                    if p >= 0:
+                        moves.append((p, self._pages[s][k]))
+                        self._drop(p)
+                    self._upload(s, k)
+            self.reserve(s, at + n)
+        if moves:
+            self.copy_pages([a for a, _ in moves], [b for _, b in moves])
+        pos0 = [self._length[s] for s in slots]
+        for s, n in zip(slots, counts):
+            self._length[s] += n
+        row0 = None
+        if any(n != 1 for n in counts):
+            row0 = [0]
+            for n in counts:
+                row0.append(row0[-1] + n)
+        dev = self.device
+        return CacheRows(torch.tensor(slots, dtype=torch.int32).to(dev), torch.tensor(pos0, dtype=torch.int32).to(dev),
+                         None if row0 is None else torch.tensor(row0, dtype=torch.int32).to(dev), sum(counts),
+                         max(counts, default=0))
+
+    def rows(self, slot, pos0, row0=None, max_rows: int = 1, n_rows: int | None = None) -> CacheRows:
+        """Rows from device tensors of the caller (a device-side scheduler, a
+        graph); `n_rows` defaults to the rows that `append` or `attend` is given."""
+        import torch
+
+        for name, t, n in (("slot", slot, None), ("pos0", pos0, 0), ("row0", row0, 1)):
+            if t is None and name == "row0":
+                continue
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+                _fail(f"{name} must be a contiguous 1-D int32 tensor")
+            if t.device != self.device:
+                _fail(f"{name} must be on {self.device}")
+            if n is not None and t.shape[0] != slot.shape[0] + n:
+                _fail(f"{name} must have {slot.shape[0] + n} entries")
+        if max_rows < 0 or (row0 is None and max_rows != 1):
+            _fail("max_rows must be the rows of the longest sequence")
+        return CacheRows(slot, pos0, row0, -1 if n_rows is None else n_rows, max_rows)
+
+    # -- operators -------------------------------------------------------------------------
+    def _call(self, fn, *args) -> None:
+        import torch
+
+        with torch.cuda.device(self.device):
+            st = fn(C.byref(self._c), *args, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        if st != _lib.FMD_OK:
+            raise _lib.FmdError(st, f"{fn.__name__}: {self.lib.fmd_status_string(st).decode()}")
+
+    def check(self) -> None:
+        """Wait for the operators and raise if a row or page was out of range."""
+        st = int(self._status[0].item())
+        if st != 0:
+            self._status.zero_()
+            raise _lib.FmdError(st, "a slot, position or page was out of range")
+
+    def _dtype(self, t, name: str) -> int:
+        import torch
+
+        codes = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
+        if t.dtype not in codes or (self.kind != "q4" and codes[t.dtype] != self.format):
+            _fail(f"{name} must be {'float16 or bfloat16' if self.kind == 'q4' else self.kind}, not {t.dtype}")
+        return codes[t.dtype]
+
+    def _heads(self, t, name: str, heads: int, like=None) -> tuple:
+        """(row stride, head stride) of a [rows, heads, head_dim] tensor."""
+        if t.dim() != 3 or t.shape[2] != self.head_dim or (heads and t.shape[1] != heads):
+            _fail(f"{name} must be [rows, {heads or 'heads'}, {self.head_dim}], not {tuple(t.shape)}")
+        if t.device != self.device:
+            _fail(f"{name} must be on {self.device}")
+        if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0]):
+            _fail(f"{name} must have the rows and dtype of the others")
+        row, head, dim = t.stride()
+        row, head = (0 if t.shape[0] <= 1 else row), (0 if t.shape[1] <= 1 else head)
+        if t.numel() and (dim != 1 or row % 8 or head % 8 or row < 0 or head < 0 or t.data_ptr() % 16):
+            _fail(f"{name}: heads must be contiguous, 16-byte aligned, with strides of multiples of 8 elements")
+        return row, head
+
+    def _rows_c(self, rows: CacheRows, n: int) -> _lib.CacheRows:
+        c = rows.to_c()
+        if rows.n_rows > n:
+            _fail(f"the rows need {rows.n_rows} rows of the tensors, not {n}")
+        if rows.row0 is None and n < rows.slot.shape[0]:
+            _fail(f"{rows.slot.shape[0]} sequences need a row each, not {n}")
+        c.n_rows = n
+        return c
+
+    def append(self, layer: int, rows: CacheRows, k, v, q=None, q_norm=None, k_norm=None, eps: float = 1e-6, cos=None,
+               sin=None, interleaved: bool = False, q_out=None):
+        """Store the rows' keys and values `[rows, kv_heads, head_dim]` at their
+        positions, with `q_norm` / `k_norm` (RMS norm weights of a head) and the
+        rotation of the first `2 * cos.shape[1]` dims by `cos[position]`,
+        `sin[position]` (f32 tables; pairs i and i + half, or neighbours if
+        `interleaved`) applied to queries and keys in the same pass. Returns the
+        normed and rotated queries (`q_out`, which may be `q`), or None without
+        `q`. f32 arithmetic, one rounding per value."""
+        import torch
+
+        if not 0 <= layer < self.layers:
+            _fail(f"layer {layer} is out of range")
+        a = _lib.CacheAppendArgs(k=k.data_ptr(), v=v.data_ptr(), eps=eps, dtype=self._dtype(k, "k"),
+                                 interleaved=bool(interleaved))
+        a.k_row, a.k_head = self._heads(k, "k", self.kv_heads)
+        a.v_row, a.v_head = self._heads(v, "v", self.kv_heads, k)
+        if q is not None:
+            a.q_row, a.q_head = self._heads(q, "q", 0, k)
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            a.q_out_row, a.q_out_head = self._heads(q_out, "q_out", q.shape[1], q)
+            a.q, a.q_out, a.n_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+        elif q_out is not None or q_norm is not None:
+            _fail("q_out and q_norm need q")
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None:
+                if (w.dtype != k.dtype or tuple(w.shape) != (self.head_dim,) or not w.is_contiguous()
+                        or w.device != self.device or w.data_ptr() % 16):
+                    _fail(f"{name} must be an aligned contiguous [{self.head_dim}] tensor of the rows' dtype")
+                setattr(a, name, w.data_ptr())
+        if (cos is None) != (sin is None):
+            _fail("cos and sin go together")
+        if cos is not None:
+            for t in (cos, sin):
+                if (t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or not t.is_contiguous()
+                        or t.device != self.device or t.data_ptr() % 16):
+                    _fail("cos and sin must be aligned contiguous f32 tables [positions, pairs]")
+            if cos.shape[0] < 1 or cos.shape[1] % 4 or not 0 < cos.shape[1] <= self.head_dim // 2:
+                _fail("the rotated dims must be a multiple of 8, at most head_dim")
+            a.cos_table, a.sin_table = cos.data_ptr(), sin.data_ptr()
+            a.rot_dim, a.table_rows = 2 * cos.shape[1], cos.shape[0]
+        self._call(self.lib.fmd_cache_append, layer, C.byref(self._rows_c(rows, k.shape[0])), C.byref(a),
+                   C.c_void_p(self._status.data_ptr()))
+        return q_out
+
+    def read(self, layer: int, rows: CacheRows, k_out=None, v_out=None, n_rows: int | None = None):
+        """The cached keys and values of the rows' positions, f32
+        `[rows, kv_heads, head_dim]`."""
+        import torch
+
+        if not 0 <= layer < self.layers:
+            _fail(f"layer {layer} is out of range")
+        if n_rows is None:
+            n_rows = k_out.shape[0] if k_out is not None else rows.n_rows
+        shape = (n_rows, self.kv_heads, self.head_dim)
+        if n_rows < 0:
+            _fail("n_rows is needed")
+        k_out = torch.zeros(shape, dtype=torch.float32, device=self.device) if k_out is None else k_out
+        v_out = torch.zeros(shape, dtype=torch.float32, device=self.device) if v_out is None else v_out
+        for t in (k_out, v_out):
+            if (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != self.device
+                    or t.data_ptr() % 16):
+                _fail(f"outputs must be aligned contiguous f32 tensors {shape}")
+        self._call(self.lib.fmd_cache_read, layer, C.byref(self._rows_c(rows, n_rows)), C.c_void_p(k_out.data_ptr()),
+                   C.c_void_p(v_out.data_ptr()), C.c_void_p(self._status.data_ptr()))
+        return k_out, v_out
+
+    def workspace(self, n_heads: int, n_seqs: int, max_rows: int = 1):
+        """A zeroed workspace for `attend` calls of up to `n_seqs` sequences of
+        up to `max_rows` rows, for callers that keep their own (one for each graph
+        or stream whose calls may run at the same time)."""
+        import torch
+
+        n = int(self.lib.fmd_cache_attend_workspace(C.byref(self._c), n_heads, n_seqs, max_rows))
+        return torch.zeros(max(n, 16), dtype=torch.uint8, device=self.device)
+
+    def _workspace(self, n_heads: int, rows: CacheRows):
+        import torch
+
+        n = int(self.lib.fmd_cache_attend_workspace(C.byref(self._c), n_heads, rows.slot.shape[0], rows.max_rows))
+        if n == 0:
+            return None
+        if torch.cuda.is_current_stream_capturing():
+            # a graph's own: graphs replayed at the same time must not share one
+            return torch.zeros(n, dtype=torch.uint8, device=self.device)
+        key = torch.cuda.current_stream(self.device).cuda_stream
+        w = self._workspaces.get(key)
+        if w is None or w.numel() < n:
+            w = self._workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        return w
+
+    def attend(self, layer: int, rows: CacheRows, q, window: int = 0, sinks: int = 0, scale: float | None = None,
+               out=None, workspace=None):
+        """Attention of queries `[rows, heads, head_dim]` over their slots' cached
+        positions j <= p (p: the row's own, already appended): all of them, or
+        with `window` > 0 those with j > p - window or j < sinks. `scale` defaults
+        to head_dim ** -0.5. Returns `out` (rows of padding and behind the last
+        sequence are left as they were)."""
+        import torch
+
+        if not 0 <= layer < self.layers:
+            _fail(f"layer {layer} is out of range")
+        if window < 0 or sinks < 0 or window > 2**31 - 1 or sinks > 2**31 - 1:
+            _fail("window and sinks must be >= 0")
+        a = _lib.CacheAttendArgs(q=q.data_ptr(), dtype=self._dtype(q, "q"), window=window, sinks=sinks,
+                                 scale=self.head_dim ** -0.5 if scale is None else scale)
+        a.q_row, a.q_head = self._heads(q, "q", 0)
+        a.n_heads = q.shape[1]
+        if a.n_heads % self.kv_heads or a.n_heads // self.kv_heads not in (1, 2, 4, 8, 16):
+            _fail(f"heads must be {self.kv_heads} x 1, 2, 4, 8 or 16, not {a.n_heads}", _lib.FMD_ENOTSUP)
+        if out is None:
+            out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        a.out_row, a.out_head = self._heads(out, "out", q.shape[1], q)
+        a.out = out.data_ptr()
+        if workspace is None:
+            workspace = self._workspace(a.n_heads, rows)
+        elif workspace.dtype != torch.uint8 or workspace.device != self.device or not workspace.is_contiguous():
+            _fail("workspace must be a contiguous uint8 tensor of this device (PagedCache.workspace)")
+        ws, nb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+        self._call(self.lib.fmd_cache_attend, layer, C.byref(self._rows_c(rows, q.shape[0])), C.byref(a),
+                   C.c_void_p(ws), nb, C.c_void_p(self._status.data_ptr()))
+        return out
+
+    # -- pages ----------------------------------------------------------------------------
+    def copy_pages(self, src, dst) -> None:
+        """Copy pages `src[i]` to `dst[i]` in every layer (contents only)."""
+        src, dst = list(src), list(dst)
+        if len(src) != len(dst):
+            _fail("src and dst must be as long")
+        if any(not 0 <= p < self.n_pages for p in src + dst):
+            _fail("page out of range")
+        if len(set(dst)) != len(dst) or set(dst) & set(src):
+            _fail("a page is written twice, or read and written")
+        ia = C.c_int32 * len(src)
+        self._call(self.lib.fmd_cache_copy_pages, len(src), ia(*src), ia(*dst))
+
+    def fork(self, src: int, dsts) -> None:
+        """Give each closed slot of `dsts` the sequence of `src`: full pages are
+        shared, the rows behind them are copied to a page of its own."""
+        dsts = list(dsts)
+        pages, n = self._open(src), self._length[src]
+        full, part = divmod(n, PAGE)
+        for d in dsts:
+            if not 0 <= d < self.max_slots:
+                _fail(f"slot {d} is out of range")
+            if self._pages[d] is not None:
+                _fail(f"slot {d} is already open", _lib.FMD_EBUSY)
+        if len(set(dsts)) != len(dsts):
+            _fail("a slot is listed twice")
+        if part and pages[full] < 0:
+            _fail(f"slot {src}: its last page was evicted")
+        if part and len(dsts) > len(self._free):
+            _fail("the cache has too few free pages", _lib.FMD_ENOMEM)
+        fresh = [self._take() if part else -1 for _ in dsts]
+        for d, p in zip(dsts, fresh):
+            self._pages[d] = pages[:full] + ([p] if part else [])
+            self._length[d] = n
+            for s in pages[:full]:
+                if s >= 0:
+                    self._names[s] += 1
+        m = len(dsts)
+        ia = C.c_int32 * m
+        self._call(self.lib.fmd_cache_fork, m, ia(*[src] * m), ia(*dsts), ia(*[n] * m), ia(*fresh),
+                   C.c_void_p(self._status.data_ptr()))
+
+    def evict(self, slot: int, window: int, sinks: int = 0) -> int:
+        """Free the slot's pages that no later row sees with this window and
+        sinks; returns how many. `attend` must not be given more afterwards."""
+        if window < 1 or sinks < 0:
+            _fail("window must be >= 1 and sinks >= 0")
+        pages, n = self._open(slot), self._length[slot]
+        first, last = -(-sinks // PAGE), (n - window + 1) // PAGE  # pages [first, last) lie between them
+        gone = [k for k in range(first, min(last, len(pages))) if pages[k] >= 0]
+        for k in gone:
+            self._drop(pages[k])
+            pages[k] = -1
+        if gone:
+            self._upload(slot, gone[0])
+        return len(gone)
+
+    def compact_tables(self, page_table, n_entries):
+        """Make the pages named by the first `n_entries[slot]` entries of each row
+        of `page_table` dense, in every layer (`fmd_cache_compact`), for callers
+        whose tables live on the device: the i-th used page at or above the number
+        in use moves into the i-th free page below it, and the entries follow.
+        Returns the number in use as a device tensor."""
+        import torch
+
+        if (page_table.dtype != torch.int32 or tuple(page_table.shape) != (self.max_slots, self.max_pages_per_slot)
+                or not page_table.is_contiguous() or page_table.device != self.device):
+            _fail("page_table must be a contiguous int32 tensor [max_slots, max_pages_per_slot] of this device")
+        if (n_entries.dtype != torch.int32 or tuple(n_entries.shape) != (self.max_slots,)
+                or not n_entries.is_contiguous() or n_entries.device != self.device):
+            _fail("n_entries must be a contiguous int32 tensor [max_slots] of this device")
+        c = _lib.Cache.from_buffer_copy(self._c)
+        c.page_table = page_table.data_ptr()
+        nb = int(self.lib.fmd_cache_compact_workspace(C.byref(c)))
+        ws = torch.empty(nb, dtype=torch.uint8, device=self.device)
+        used = torch.empty((), dtype=torch.int32, device=self.device)
+        with torch.cuda.device(self.device):
+            st = self.lib.fmd_cache_compact(C.byref(c), C.c_void_p(n_entries.data_ptr()), C.c_void_p(ws.data_ptr()), nb,
+                                            C.c_void_p(used.data_ptr()), C.c_void_p(self._status.data_ptr()),
+                                            C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        if st != _lib.FMD_OK:
+            raise _lib.FmdError(st, f"fmd_cache_compact: {self.lib.fmd_status_string(st).decode()}")
+        return used
+
+    def compact(self) -> int:
+        """Move the pages in use to the front of the pool; returns how many are
+        in use."""
+        import torch
+
+        counts = torch.tensor([len(p or ()) for p in self._pages], dtype=torch.int32).to(self.device)
+        self.compact_tables(self.page_table, counts)
+        used = [p for p in range(self.n_pages) if self._names[p]]
+        n = len(used)
+        holes = [p for p in range(n) if not self._names[p]]
+        to = dict(zip([p for p in used if p >= n], holes))
+        self._pages = [None if r is None else [to.get(p, p) for p in r] for r in self._pages]
+        for a, b in to.items():
+            self._names[b], self._names[a] = self._names[a], 0
+        self._free = list(range(n, self.n_pages))
+        return n
