@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(256) k_cache_attend(CacheView c, int layer, Ca
 
 cudaError_t launch_cache_attend(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAttend& a,
                                 void* workspace, int* status, cudaStream_t s) {
-  (void)workspace;
+  if (cache_decode_fits(c, a.n_heads, a.max_rows)) return launch_cache_decode(bf16, c, layer, r, a, workspace, status, s);
   const int gx = (int)std::min<long long>(((long long)a.max_rows * a.n_heads + 7) / 8, 4096);
   const dim3 grid(gx, r.n_seqs);
   if (bf16) {

@@ -180,8 +180,11 @@ enum TimeoutSite {
   kSiteLayerTail = 6,
   kSiteWaitProbe = 7,
   kSiteProjTc = 8,
+  kSiteCacheDecode = 9,
+  kSiteCacheChunk = 10,
 };
 FMD_DEV void report_timeout(int* status, int site) {
+  if (status == nullptr) return;
   atomicExch(status, -110);  // FMD_ETIMEDOUT
   atomicCAS(status + 1, 0, site);
 }

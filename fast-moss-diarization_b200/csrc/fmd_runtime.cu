@@ -882,7 +882,7 @@ int sync_check(fmd_handle* h) {
     if (st[0] != 0) {
       cudaMemset(h->d_status, 0, 2 * sizeof(int));
       static const char* const kSites[] = {"?", "k_gemv", "k_lm_head", "k_attn_decode_tma", "k_attn_prefill_tc",
-                                           "k_gemm_tc", "k_layer_tail", "k_wait_probe", "k_proj_tc"};
+                                           "k_gemm_tc", "k_layer_tail", "k_wait_probe", "k_proj_tc", "k_cache_decode", "k_cache_chunk"};
       constexpr int kNumSites = (int)(sizeof(kSites) / sizeof(kSites[0]));
       const char* site = st[1] >= 1 && st[1] < kNumSites ? kSites[st[1]] : "?";
       return fail(h, st[0], st[0] == FMD_EIO ? std::string("a greedy pick found no finite logit (non-finite activations)")

@@ -65,9 +65,10 @@ def append_tolerance(want, rows_max, eps):
 
 def attend_tolerance(want, mag, eps, q4):
     """The output's rounding (eps / 2 of the value), each probability's (eps / 2
-    of its term; 2^-12 in 4 bits, where products run in f16), in 4 bits also
-    each value's product with its scale (2^-12), and f32 arithmetic: scores of
-    magnitude up to 2^5 with 2^-20 of it wrong move p by 2^-15, sums and the
+    of its term; in 4 bits, where products run in f16, half a step of f16,
+    2^-11: a step is 2^-10 of a value just above a power of two), in 4 bits also
+    each value's product with its scale (2^-11 again), and f32 arithmetic: scores
+    of magnitude up to 2^5 with 2^-20 of it wrong move p by 2^-15, sums and the
     hardware exponential by less: 2^-14 of the magnitude in all."""
-    terms = 2 * 2.0 ** -12 if q4 else eps / 2
+    terms = 2 * 2.0 ** -11 if q4 else eps / 2
     return eps / 2 * np.abs(want) + (terms + 2.0 ** -14) * mag + 2.0 ** -25

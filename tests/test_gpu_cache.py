@@ -247,6 +247,31 @@ def test_attend_many_sequences(kind):
     _check_attend(c, held, kind, "bf16", [1] * 300, lengths, 2, 33, 2)
 
 
+@pytest.mark.parametrize("kind,dtype", [("bf16", "bf16"), ("f16", "f16"), ("q4", "bf16")])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("count", [1, 4])
+def test_attend_many_tiles_per_block(kind, dtype, dim, count):
+    """Enough pages that every ring goes round many times and a block's range
+    covers whole sequences: 4 heads x about 2,800 pages."""
+    lengths = [5000 - 31 * i for i in range(40)]
+    c, held = _filled(kind, dtype, lengths, dim, 4, seed=17)
+    q = _rand(np.random.default_rng(5), 40 * count, 8, dim, dtype=dtype)
+    rows = _seq_rows(c, list(range(40)), [count] * 40, lengths)
+    for window, sinks in ((0, 0), (3000, 100)):
+        out = c.attend(0, rows, q, window=window, sinks=sinks)
+        c.check()
+        for s in (0, 7, 19, 20, 39):
+            a = slice(s * count, (s + 1) * count)
+            want, mag = ref.attend(_np(q[a]), *held[s], range(lengths[s] - count, lengths[s]), window, sinks)
+            assert (np.abs(_np(out[a]) - want) <= ref.attend_tolerance(want, mag, _eps(dtype), kind == "q4")).all()
+        # every sequence by itself: other cuts, the same sums up to roundings
+        for s in range(40):
+            a = slice(s * count, (s + 1) * count)
+            one = c.attend(0, _seq_rows(c, [s], [count], [lengths[s]]), q[a], window=window, sinks=sinks)
+            near = (_np(one) - _np(out[a])) / np.abs(_np(out[a])).max()
+            assert np.abs(near).max() <= 4 * _eps(dtype)
+
+
 @pytest.mark.parametrize("kind", ["bf16", "q4"])
 @pytest.mark.parametrize("count", [1, 40])
 def test_attend_strides_scale_and_rows_left_alone(kind, count):
