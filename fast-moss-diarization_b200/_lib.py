@@ -35,6 +35,7 @@ FINISH_STOP, FINISH_LENGTH, FINISH_ERROR = 0, 1, 2
 
 # cache formats (fmd_cache.h)
 CACHE_F16, CACHE_BF16, CACHE_Q4 = 1, 2, 4
+CACHE_WORKSPACE_ZERO = 65536
 
 # every symbol the header declares
 EXPORTS = [

@@ -382,7 +382,14 @@ class PagedCache:
         import torch
 
         n = int(self.lib.fmd_cache_attend_workspace(C.byref(self._c), n_heads, n_seqs, max_rows))
-        return torch.zeros(max(n, 16), dtype=torch.uint8, device=self.device)
+        return self._fresh_workspace(n)
+
+    def _fresh_workspace(self, n: int):
+        import torch
+
+        w = torch.empty(max(n, 16), dtype=torch.uint8, device=self.device)
+        w[:_lib.CACHE_WORKSPACE_ZERO].zero_()
+        return w
 
     def _workspace(self, n_heads: int, rows: CacheRows):
         import torch
@@ -392,11 +399,11 @@ class PagedCache:
             return None
         if torch.cuda.is_current_stream_capturing():
             # a graph's own: graphs replayed at the same time must not share one
-            return torch.zeros(n, dtype=torch.uint8, device=self.device)
+            return self._fresh_workspace(n)
         key = torch.cuda.current_stream(self.device).cuda_stream
         w = self._workspaces.get(key)
         if w is None or w.numel() < n:
-            w = self._workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            w = self._workspaces[key] = self._fresh_workspace(n)
         return w
 
     def attend(self, layer: int, rows: CacheRows, q, window: int = 0, sinks: int = 0, scale: float | None = None,

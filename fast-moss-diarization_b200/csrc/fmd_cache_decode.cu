@@ -55,11 +55,12 @@ constexpr int kDcSeqs = 256;      // sequences of one launch at most
 // workspace, since they are zero between calls of any shape.
 constexpr int kDcCounters = 16384;
 constexpr int kDcThreads = 160;   // 4 consumer warps, 1 producer warp
+constexpr int kDcQ4Ctas = 3;      // CTAs an SM holds over a 4-bit cache (one column tile)
 constexpr uint32_t kDcWait = 1u << 22;
 constexpr float kDcHeadroom = 8.f;  // log2: how far a score may exceed the reference
 
 struct DcSmem {
-  int stage_bytes, stages, red_off, red_stride;
+  int stage_bytes, stages, red_off, red_row;
 };
 
 struct DcArgs {
@@ -69,6 +70,7 @@ struct DcArgs {
   int* counters;    // [sequences][kv heads], zero between calls
   int seq0, seqs;   // the sequences of this launch
   int tile_rows;    // rows of a segment's tile at most
+  uint32_t f64;     // f16 pair (64, 64)
   DcSmem sm;
 };
 
@@ -85,10 +87,20 @@ FMD_DEV uint32_t h2mul(uint32_t a, uint32_t b) {
   __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<uint32_t*>(&r);
 }
-// nibble N of both 16-bit halves as the f16 pair 64 + c
-template <int N> FMD_DEV uint32_t nibble64(uint32_t w) {
+// Nibble N of both 16-bit halves as the f16 pair 64 + c. f64 = 0x54005400 comes in
+// a register: with two literal operands the and-or became two instructions
+// (145 of them for 16 keys instead of 64).
+template <int N> FMD_DEV uint32_t nibble64(uint32_t w, uint32_t f64) {
   const uint32_t x = N == 0 ? w << 4 : N == 1 ? w : N == 2 ? w >> 4 : w >> 8;
-  return (x & 0x00f000f0u) | 0x54005400u;
+  return (x & 0x00f000f0u) | f64;
+}
+// d = a x b + c (m16n8k16, f16), c left as it is
+FMD_DEV void mma_f16_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%11,%10,%11};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 FMD_DEV float ex2(float x) {
   float y;
@@ -106,7 +118,7 @@ FMD_DEV uint32_t dc_swz(int row, int ch) {
 
 // NT: 8-column tiles of (row, head) pairs.
 template <typename T, int D, bool Q4, int NT>
-__global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
+__global__ void __launch_bounds__(kDcThreads, Q4 && NT == 1 ? kDcQ4Ctas : 2)
     k_cache_decode(const __grid_constant__ CUtensorMap tmap, CacheView c, int layer, DcArgs p, int* status) {
   constexpr int KS = D / 16;                    // 16-wide steps of the head
   constexpr int MT = D / 16;                    // 16-dim tiles of the output
@@ -119,7 +131,7 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
   constexpr float kPScale = kHiLo ? 0.f : 7.f;    // log2 factor of P: f16 keeps what is 2^-21 of the reference
 
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   float* red = reinterpret_cast<float*>(smem + p.sm.red_off);
   __shared__ int s_prefix[kDcSeqs + 1], s_slot[kDcSeqs], s_pos[kDcSeqs], s_row[kDcSeqs], s_cnt[kDcSeqs];
   __shared__ __align__(8) uint64_t full[8], empty[8];
@@ -220,7 +232,7 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
   if (warp == 4) {
     // ---------------- producer ----------------
     bool ok = true;
-    int issued = 0;
+    int issued = 0, s = 0, round = 0;  // tile `issued` goes to stage s, used `round` times before
     for (int b0 = 0; b0 < ntl && ok; b0 += 32) {
       int lh = 0, lpage = -1;
       if (b0 + lane < ntl) {
@@ -235,8 +247,7 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
       const int cnt = min(32, ntl - b0);
       for (int i = 0; i < cnt; ++i) {
         const int h = __shfl_sync(0xffffffffu, lh, i), page = __shfl_sync(0xffffffffu, lpage, i);
-        const int tt = b0 + i, s = tt % stages;
-        if (tt >= stages && !mbar_wait_bounded(&empty[s], ((tt / stages) - 1) & 1, kDcWait)) {
+        if (round > 0 && !mbar_wait_bounded(&empty[s], (round - 1) & 1, kDcWait)) {
           ok = false;
           break;
         }
@@ -261,7 +272,8 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
           }
         }
         __syncwarp();
-        issued = tt + 1;
+        ++issued;
+        if (++s == stages) s = 0, ++round;
       }
     }
     if (lane == 0) {
@@ -275,21 +287,27 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
 
   // ---------------- consumers ----------------
   bool aborted = false;
-  const int group = p.a.n_heads / H;
+  const uint32_t f64 = p.f64;
+  const int gs = __ffs(p.a.n_heads / H) - 1;  // log2 of the query heads of a kv head
   const int koff = (warp % WPT) * 16 * U, which = warp / WPT;
   int cr, ch, cj;
   locate(x0, cr, ch, cj);
-  int ctr = s_prefix[cr + 1] - s_prefix[cr], pj0 = cj;
+  int ctr = s_prefix[cr + 1] - s_prefix[cr];
+  int nq = 0, p0 = 0, p1 = 0, stt = 0, wt0 = 0;  // of the current sequence: pairs, positions, tile split
   uint32_t qf[NT][KS][2];
   float qs[Q4 ? NT : 1][Q4 ? NB : 1][2];  // -72 x sum of the queries of each block, per column
   float sl[NT][2];                        // scale per column
   float o[NT][MT][4], m[NT][2], l[NT][2];
-  for (int tt = 0; tt < ntl; ++tt) {
-    const int s = tt % stages;
-    const bool first = tt == 0 || cj == 0, last = tt == ntl - 1 || cj == ctr - 1;
-    const int nq = s_cnt[cr] * group, p0 = s_pos[cr], p1 = p0 + s_cnt[cr] - 1;
-    if (first) {
-      pj0 = cj;
+  // this warp's next tile of the CTA's range, its stage and the stage's phase
+  int mine = which, s = which, phase = 0;
+  for (int x = 0; x < ntl;) {
+    // a piece: tiles cj .. cj + len - 1 of segment (cr, ch)
+    const int len = min(ctr - cj, ntl - x);
+    {
+      nq = s_cnt[cr] << gs;
+      p0 = s_pos[cr];
+      p1 = p0 + s_cnt[cr] - 1;
+      split(p0, stt, wt0);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         m[n][0] = m[n][1] = -INFINITY;
@@ -298,8 +316,8 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
         for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
         // B fragments: this thread's column is pair 8 n + g
         const int pr = n * 8 + g;
-        const T* q = (const T*)p.a.q + (size_t)(s_row[cr] + pr / group) * p.a.q_row +
-                     (size_t)(ch * group + pr % group) * p.a.q_head;
+        const T* q = (const T*)p.a.q + (size_t)(s_row[cr] + (pr >> gs)) * p.a.q_row +
+                     (size_t)((ch << gs) + (pr & ((1 << gs) - 1))) * p.a.q_head;
         if constexpr (!Q4) {
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks)
@@ -355,14 +373,13 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
         }
       }
     }
-    if (tt % U == which) {
-      if (!aborted && !mbar_wait_bounded(&full[s], (tt / stages) & 1, kDcWait)) aborted = true;
+    for (; mine < x + len; mine += U) {
+      if (!aborted && !mbar_wait_bounded(&full[s], phase, kDcWait)) aborted = true;
       // keys k0 .. k0 + KW - 1 of this warp; visible to some row: up to p1, from the
       // oldest window's start or among the sinks
-      int stt, wt0;
       constexpr int KW = 16 * U;
-      split(p0, stt, wt0);
-      const int k0 = (cj < stt ? cj : wt0 + cj - stt) * kPageTokens + koff;
+      const int jt = cj + mine - x;
+      const int k0 = (jt < stt ? jt : wt0 + jt - stt) * kPageTokens + koff;
       auto seen = [&](int k, int pos) { return k <= pos && (W == 0 || k > pos - W || k < S); };
       const bool whole = k0 + KW - 1 <= p0 && (W == 0 || k0 > p1 - W || k0 + KW - 1 < S);
       const bool any = k0 <= p1 && (W == 0 || k0 + KW - 1 > p0 - W || k0 < S);
@@ -405,12 +422,12 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
             for (int n = 0; n < NT; ++n) sc[n][u][0] = sc[n][u][1] = sc[n][u][2] = sc[n][u][3] = 0.f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-              const uint32_t a0[4] = {nibble64<0>(wa[b]), nibble64<0>(wb[b]), nibble64<1>(wa[b]), nibble64<1>(wb[b])};
-              const uint32_t a1[4] = {nibble64<2>(wa[b]), nibble64<2>(wb[b]), nibble64<3>(wa[b]), nibble64<3>(wb[b])};
+              const uint32_t a0[4] = {nibble64<0>(wa[b], f64), nibble64<0>(wb[b], f64), nibble64<1>(wa[b], f64), nibble64<1>(wb[b], f64)};
+              const uint32_t a1[4] = {nibble64<2>(wa[b], f64), nibble64<2>(wb[b], f64), nibble64<3>(wa[b], f64), nibble64<3>(wb[b], f64)};
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                float acc[4] = {qs[n][b][0], qs[n][b][1], qs[n][b][0], qs[n][b][1]};
-                mma16816<__half>(acc, a0, qf[n][2 * b][0], qf[n][2 * b][1]);
+                float acc[4];
+                mma_f16_from(acc, a0, qf[n][2 * b][0], qf[n][2 * b][1], qs[n][b][0], qs[n][b][1]);
                 mma16816<__half>(acc, a1, qf[n][2 * b + 1][0], qf[n][2 * b + 1][1]);
                 sc[n][u][0] = fmaf(acc[0], da[b], sc[n][u][0]);
                 sc[n][u][1] = fmaf(acc[1], da[b], sc[n][u][1]);
@@ -434,18 +451,37 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
         // scores in the exp2 domain; hidden ones are -inf
         float mx[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mx[n][0] = mx[n][1] = -INFINITY;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int u = 0; u < U; ++u)
 #pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][u][e] *= sl[n][e & 1];
+        uint32_t vis[U][2];  // bit masks of the value pairs (kb, kb + 1), (kb + 8, kb + 9) below
+#pragma unroll
+        for (int u = 0; u < U; ++u) vis[u][0] = vis[u][1] = 0xffffffffu;
+        if (!whole) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!seen(k0 + u * 16 + g + (e >> 1) * 8, p0 + ((n * 8 + 2 * t + (e & 1)) >> gs)))
+                  sc[n][u][e] = -INFINITY;
+#pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float x = sc[n][u][e] * sl[n][e & 1];
-              if (!whole && !seen(k0 + u * 16 + g + (e >> 1) * 8, p0 + (n * 8 + 2 * t + (e & 1)) / group)) x = -INFINITY;
-              sc[n][u][e] = x;
-              mx[n][e & 1] = fmaxf(mx[n][e & 1], x);
+              const int k = k0 + u * 16 + 2 * t + (e & 1) + (e >> 1) * 8;
+              if (!(k <= p1 && (W == 0 || k > p0 - W || k < S))) vis[u][e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
             }
+          }
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            mx[n][k] = fmaxf(sc[n][0][k], sc[n][0][2 + k]);
+            if constexpr (U == 2) mx[n][k] = fmaxf(mx[n][k], fmaxf(sc[n][U - 1][k], sc[n][U - 1][2 + k]));
+          }
         bool up = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) up |= mx[n][0] > m[n][0] + kDcHeadroom || mx[n][1] > m[n][1] + kDcHeadroom;
@@ -495,13 +531,6 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int kb = koff + u * 16 + 2 * t;  // this thread's keys: kb, kb + 1, kb + 8, kb + 9
-          const int ks0 = k0 + u * 16 + 2 * t;
-          bool vis[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = ks0 + (e & 1) + (e >> 1) * 8;
-            vis[e] = whole || (k <= p1 && (W == 0 || k > p0 - W || k < S));
-          }
           if constexpr (Q4) {
             const uint8_t* vs = vt + 64 * (D / 2);
             const int blk = NB == 4 ? g >> 1 : g >> 2;  // this thread's dims lie in one block
@@ -510,7 +539,7 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
             for (int b = 0; b < 2; ++b) {
               const uint32_t lo = *reinterpret_cast<const uint16_t*>(vs + ((kb + b * 8) * NB + blk) * 2);
               const uint32_t hi = *reinterpret_cast<const uint16_t*>(vs + ((kb + b * 8 + 1) * NB + blk) * 2);
-              d2[b] = (vis[2 * b] ? lo : 0u) | (vis[2 * b + 1] ? hi << 16 : 0u);
+              d2[b] = (lo | hi << 16) & vis[u][b];
             }
             uint32_t w[4][D / 64];
 #pragma unroll
@@ -532,11 +561,11 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
                 const uint32_t x = __byte_perm(w[0][i], w[1][i], sel), y = __byte_perm(w[2][i], w[3][i], sel);
                 const uint32_t k72 = 0x54805480u;  // f16 72
                 const uint32_t a0[4] = {
-                    h2mul(h2sub(nibble64<0>(x), k72), d2[0]), h2mul(h2sub(nibble64<1>(x), k72), d2[0]),
-                    h2mul(h2sub(nibble64<0>(y), k72), d2[1]), h2mul(h2sub(nibble64<1>(y), k72), d2[1])};
+                    h2mul(h2sub(nibble64<0>(x, f64), k72), d2[0]), h2mul(h2sub(nibble64<1>(x, f64), k72), d2[0]),
+                    h2mul(h2sub(nibble64<0>(y, f64), k72), d2[1]), h2mul(h2sub(nibble64<1>(y, f64), k72), d2[1])};
                 const uint32_t a1[4] = {
-                    h2mul(h2sub(nibble64<2>(x), k72), d2[0]), h2mul(h2sub(nibble64<3>(x), k72), d2[0]),
-                    h2mul(h2sub(nibble64<2>(y), k72), d2[1]), h2mul(h2sub(nibble64<3>(y), k72), d2[1])};
+                    h2mul(h2sub(nibble64<2>(x, f64), k72), d2[0]), h2mul(h2sub(nibble64<3>(x, f64), k72), d2[0]),
+                    h2mul(h2sub(nibble64<2>(y, f64), k72), d2[1]), h2mul(h2sub(nibble64<3>(y, f64), k72), d2[1])};
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                   mma16816<__half>(o[n][i * 4 + hf * 2], a0, pb[n][u][0], pb[n][u][1]);
@@ -544,15 +573,13 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
                 }
               }
           } else {
-            const uint32_t m0 = (vis[0] ? 0xffffu : 0u) | (vis[1] ? 0xffff0000u : 0u);
-            const uint32_t m1 = (vis[2] ? 0xffffu : 0u) | (vis[3] ? 0xffff0000u : 0u);
             // matrices: (keys 0-7, dims 0-7), (keys 0-7, dims 8-15), (keys 8-15, dims 0-7), ...
             const int row = koff + u * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
               uint32_t a[4];
               ldmatrix_x4_trans(a, va + dc_swz(row, 2 * i + ((lane >> 3) & 1)));
-              if (!whole) a[0] &= m0, a[1] &= m0, a[2] &= m1, a[3] &= m1;
+              if (!whole) a[0] &= vis[u][0], a[1] &= vis[u][0], a[2] &= vis[u][1], a[3] &= vis[u][1];
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 mma16816<M>(o[n][i], a, pb[n][u][0], pb[n][u][1]);
@@ -564,11 +591,12 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
+      if ((s += U) >= stages) s -= stages, phase ^= 1;
     }
 
-    if (last) {
+    {
       // ---- merge the 4 warps over this piece of the segment ----
-      const int rs = p.sm.red_stride;  // floats of a row: D + 2, odd multiple of 2
+      constexpr int rs = D + 2;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -595,7 +623,7 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
           }
         }
       named_sync(1, 128);
-      const bool inside = pj0 == 0 && cj == ctr - 1;
+      const bool inside = len == ctr;
       const long long seg0 = (long long)H * s_prefix[cr] + (long long)ch * ctr;
       const int pslot = 2 * cta + (seg0 < x0 ? 0 : 1);
       for (int i = tid; i < nq * (D / 2); i += 128) {
@@ -615,8 +643,8 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
         }
         if (inside) {
           if (!aborted) {
-            T* out = (T*)p.a.out + (size_t)(s_row[cr] + row / group) * p.a.out_row +
-                     (size_t)(ch * group + row % group) * p.a.out_head + d0;
+            T* out = (T*)p.a.out + (size_t)(s_row[cr] + (row >> gs)) * p.a.out_row +
+                     (size_t)((ch << gs) + (row & ((1 << gs) - 1))) * p.a.out_head + d0;
             *reinterpret_cast<uint32_t*>(out) = Act<T>::pack2(A0 / L, A1 / L);
           }
         } else {
@@ -637,25 +665,48 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
         }
         named_sync(1, 128);
         if (s_last) {
+          // weights of the pieces (one warp per row), then the weighted sums
+          const int np = cl - cf + 1, ws = p.sm.red_row;  // floats of `red` per row, > pieces
+          auto piece = [&](int k) {
+            return p.part + (size_t)(2 * (cf + k) + (k == 0 ? 1 : 0)) * p.tile_rows * (D + 2);
+          };
+          for (int row = warp; row < nq; row += 4) {
+            float Mx = -INFINITY, L = 0.f;
+            for (int k = lane; k < np; k += 32) {
+              const float x = __ldcg(piece(k) + row * (D + 2) + D);
+              red[row * ws + k] = x;
+              Mx = fmaxf(Mx, x);
+            }
+            Mx = warp_max(Mx);
+            const float base = Mx == -INFINITY ? 0.f : Mx;
+            for (int k = lane; k < np; k += 32) {
+              const float f = ex2(red[row * ws + k] - base);
+              red[row * ws + k] = f;
+              L = fmaf(__ldcg(piece(k) + row * (D + 2) + D + 1), f, L);
+            }
+            L = warp_sum(L);
+            if (lane == 0) red[row * ws + np] = L;
+          }
+          named_sync(1, 128);
           for (int i = tid; i < nq * (D / 2); i += 128) {
             const int row = i / (D / 2), d0 = (i % (D / 2)) * 2;
-            auto at = [&](int cc) {
-              return p.part + ((size_t)(2 * cc + (cc == cf ? 1 : 0)) * p.tile_rows + row) * (D + 2);
-            };
-            float Mx = -INFINITY;
-            for (int cc = cf; cc <= cl; ++cc) Mx = fmaxf(Mx, __ldcg(at(cc) + D));
-            const float base = Mx == -INFINITY ? 0.f : Mx;
-            float L = 0.f, A0 = 0.f, A1 = 0.f;
-            for (int cc = cf; cc <= cl; ++cc) {
-              const float* pt = at(cc);
-              const float f = ex2(__ldcg(pt + D) - base);
-              L = fmaf(__ldcg(pt + D + 1), f, L);
-              A0 = fmaf(__ldcg(pt + d0), f, A0);
-              A1 = fmaf(__ldcg(pt + d0 + 1), f, A1);
+            const float* w = red + row * ws;
+            float A0 = 0.f, A1 = 0.f;
+            const float* pt = piece(0) + row * (D + 2) + d0;
+            float2 x = __ldcg(reinterpret_cast<const float2*>(pt));
+            A0 = x.x * w[0], A1 = x.y * w[0];
+            pt = p.part + (size_t)2 * (cf + 1) * p.tile_rows * (D + 2) + row * (D + 2) + d0;
+            const size_t step = (size_t)2 * p.tile_rows * (D + 2);
+#pragma unroll 16
+            for (int k = 1; k < np; ++k, pt += step) {
+              x = __ldcg(reinterpret_cast<const float2*>(pt));
+              A0 = fmaf(x.x, w[k], A0);
+              A1 = fmaf(x.y, w[k], A1);
             }
             if (!aborted) {
-              T* out = (T*)p.a.out + (size_t)(s_row[cr] + row / group) * p.a.out_row +
-                       (size_t)(ch * group + row % group) * p.a.out_head + d0;
+              const float L = w[np];
+              T* out = (T*)p.a.out + (size_t)(s_row[cr] + (row >> gs)) * p.a.out_row +
+                       (size_t)((ch << gs) + (row & ((1 << gs) - 1))) * p.a.out_head + d0;
               *reinterpret_cast<uint32_t*>(out) = Act<T>::pack2(A0 / L, A1 / L);
             }
           }
@@ -664,7 +715,8 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
       }
       named_sync(1, 128);  // `red` is reused by the next piece
     }
-    if (++cj == ctr) {
+    x += len;
+    if ((cj += len) == ctr) {
       cj = 0;
       if (++ch == H) {
         ch = 0;
@@ -678,7 +730,7 @@ __global__ void __launch_bounds__(kDcThreads, Q4 ? (NT == 1 ? 3 : 2) : 2)
   if (aborted && lane == 0) report_timeout(status, kSiteCacheDecode);
 }
 
-int dc_ctas_per_sm(bool q4, int nt) { return q4 && nt == 1 ? 3 : 2; }
+int dc_ctas_per_sm(bool q4, int nt) { return q4 && nt == 1 ? kDcQ4Ctas : 2; }
 
 }  // namespace
 
@@ -726,6 +778,7 @@ cudaError_t launch_cache_decode(bool bf16, const CacheView& c, int layer, const 
   p.r = r;
   p.a = a;
   p.tile_rows = rows;
+  p.f64 = 0x54005400u;
   const int per_sm = dc_ctas_per_sm(q4, nt);
   const int grid = 148 * per_sm;
   p.counters = (int*)workspace;
@@ -734,8 +787,9 @@ cudaError_t launch_cache_decode(bool bf16, const CacheView& c, int layer, const 
   // as many stages as fit (at most 8) with per_sm CTAs in an SM's 227 KB
   const int blk = (int)c.block_bytes();
   p.sm.stage_bytes = 2 * blk;
-  p.sm.red_stride = D + 2;
-  const int red = 4 * rows * (D + 2) * 4;
+  // merge buffer: four warps' rows, or a weight per piece of a segment (at most one a CTA) and the sum
+  p.sm.red_row = std::max(4 * (D + 2), grid + 4);
+  const int red = rows * p.sm.red_row * 4;
   const int room = 227 * 1024 / per_sm - 8 * 1024 - red;  // static arrays, alignment, the CTA's reserve
   p.sm.stages = std::min(8, std::max(2, room / p.sm.stage_bytes));
   if (q4) p.sm.stages &= ~1;  // tiles alternate between two pairs of warps, and so must the stages

@@ -33,6 +33,7 @@ extern "C" {
 #endif
 
 #define FMD_CACHE_PAGE 64 /* positions of a page */
+#define FMD_CACHE_WORKSPACE_ZERO 65536
 
 /* ---- storage formats ------------------------------------------------------ */
 #define FMD_CACHE_F16 1  /* FMD_DT_F16  */
@@ -137,8 +138,9 @@ int64_t fmd_cache_attend_workspace(const fmd_cache* c, int32_t n_heads, int32_t 
  * sum of the values. The row's own key is in the cache (append first). Pages
  * outside every row's window and sinks are not looked up. Softmax statistics and
  * sums are f32. What a cached position that no row of the call sees holds, NaN
- * included, has no influence. `workspace` is 16-byte aligned and zero before its
- * first use; a call leaves it zero where the next one needs it so. */
+ * included, has no influence. `workspace` is 16-byte aligned; its first
+ * FMD_CACHE_WORKSPACE_ZERO bytes are zero before its first use, and every call
+ * leaves them zero, so calls of any shape and cache may take turns with it. */
 int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows,
                      const fmd_cache_attend_args* args, void* workspace, int64_t workspace_bytes, int32_t* status,
                      void* stream);
