@@ -473,7 +473,7 @@ int fmd_cache_read(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows
 int64_t fmd_cache_attend_workspace(const fmd_cache* c, int32_t n_heads, int32_t n_seqs, int32_t max_rows) {
   if (check_cache(c) || n_heads < 1 || n_heads % c->kv_heads || n_seqs < 1 || max_rows < 1) return 0;
   const CacheView v = view_of(c);
-  return cache_decode_fits(v, n_heads, max_rows) ? (int64_t)cache_decode_workspace(v, n_heads, n_seqs, max_rows) : 0;
+  return cache_decode_fits(v, n_heads, max_rows) ? (int64_t)cache_decode_workspace(v, n_heads, max_rows) : 0;
 }
 
 int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows, const fmd_cache_attend_args* a,

@@ -100,7 +100,7 @@ cudaError_t launch_cache_attend(bool bf16, const CacheView& c, int layer, const 
 
 // fmd_cache_decode.cu: at most 16 (row, head) pairs per kv head and sequence
 bool cache_decode_fits(const CacheView& c, int n_heads, int max_rows);
-size_t cache_decode_workspace(const CacheView& c, int n_heads, int n_seqs, int max_rows);
+size_t cache_decode_workspace(const CacheView& c, int n_heads, int max_rows);
 cudaError_t launch_cache_decode(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAttend& a,
                                 void* workspace, int* status, cudaStream_t s);
 
