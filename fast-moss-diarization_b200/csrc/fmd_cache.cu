@@ -473,7 +473,8 @@ int fmd_cache_read(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows
 int64_t fmd_cache_attend_workspace(const fmd_cache* c, int32_t n_heads, int32_t n_seqs, int32_t max_rows) {
   if (check_cache(c) || n_heads < 1 || n_heads % c->kv_heads || n_seqs < 1 || max_rows < 1) return 0;
   const CacheView v = view_of(c);
-  return cache_decode_fits(v, n_heads, max_rows) ? (int64_t)cache_decode_workspace(v, n_heads, max_rows) : 0;
+  return (int64_t)(cache_decode_fits(v, n_heads, max_rows) ? cache_decode_workspace(v, n_heads, max_rows)
+                                                           : cache_chunk_workspace(v, n_heads, n_seqs, max_rows));
 }
 
 int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows, const fmd_cache_attend_args* a,
@@ -495,8 +496,9 @@ int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
   if (!on_current_device(c->pool) || !on_current_device(a->q)) return FMD_EINVAL;
   CacheAttend p{a->q,     a->out,     a->q_row,  a->q_head, a->out_row, a->out_head,
                 a->scale, a->n_heads, a->window, a->sinks,  rows->max_rows};
-  return done(launch_cache_attend(a->dtype == FMD_DT_BF16, view_of(c), layer, rows_of(rows), p, workspace, status,
-                                  (cudaStream_t)stream));
+  const CacheView v = view_of(c);
+  return done((cache_decode_fits(v, a->n_heads, rows->max_rows) ? launch_cache_decode : launch_cache_chunk)(
+      a->dtype == FMD_DT_BF16, v, layer, rows_of(rows), p, workspace, status, (cudaStream_t)stream));
 }
 
 int fmd_cache_copy_pages(const fmd_cache* c, int32_t n, const int32_t* src, const int32_t* dst, void* stream) {

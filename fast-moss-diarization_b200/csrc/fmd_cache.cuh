@@ -2,6 +2,8 @@
 // cache operators and the decoder runtime.
 #pragma once
 
+#include <cuda.h>
+
 #include "../../include/fmd_cache.h"
 #include "fmd_common.cuh"
 
@@ -95,13 +97,17 @@ struct CacheAttend {
   float scale;
   int n_heads, window, sinks, max_rows;
 };
-cudaError_t launch_cache_attend(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAttend& a,
-                                void* workspace, int* status, cudaStream_t s);
-
 // fmd_cache_decode.cu: at most 16 (row, head) pairs per kv head and sequence
 bool cache_decode_fits(const CacheView& c, int n_heads, int max_rows);
 size_t cache_decode_workspace(const CacheView& c, int n_heads, int max_rows);
 cudaError_t launch_cache_decode(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAttend& a,
                                 void* workspace, int* status, cudaStream_t s);
+
+// the TMA map of a 16-bit cache's layer as [rows][head_dim], 64 x 64 boxes, 128-byte swizzle
+bool cache_tensor_map(CUtensorMap* m, const CacheView& c, int layer);
+// fmd_cache_chunk.cu: the others
+size_t cache_chunk_workspace(const CacheView& c, int n_heads, int n_seqs, int max_rows);
+cudaError_t launch_cache_chunk(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAttend& a,
+                               void* workspace, int* status, cudaStream_t s);
 
 }  // namespace fmd

@@ -1,0 +1,819 @@
+// Attention of many rows per sequence over the paged cache (prompt chunks): the
+// form of fmd_cache_attend for more than 16 (row, query head) pairs per kv head.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - m),  s_j = scale log2(e) q . k_j
+//
+// over the visible keys of each row. Every key tile is used by 256 pairs, so the
+// bound is arithmetic: 4 x head_dim flop per (pair, visible key) on the tensor
+// cores, and one exponential each on the special-function units, which at
+// head_dim 128 take as long (64 keys x 256 pairs: 1,082 cycles of tcgen05 at its
+// peak, 1,024 cycles of 16 exponentials a cycle).
+//
+// A work item is two consecutive tiles A, B of 128 pairs (row-major, then the
+// query heads of the kv head) of one sequence and kv head: each key tile (a page)
+// is read once for both. Its key tiles are those of the sinks, then those from
+// A's oldest window to B's newest row; a tile that one of A, B does not see is
+// skipped for it. With fewer items than SMs an item's key tiles are split into
+// parts, whose (m, l, o) go through the workspace; the last part to finish
+// merges them in order. Items go out latest rows first, dealt in turn.
+//
+//  * warp 0: copies of the page tiles into a ring (16 bits: 2D TMA with the
+//    128-byte swizzle; 4 bits: bulk copies of the blocks);
+//  * warp 1: tcgen05.mma, f32 accumulators in tensor memory: S_A(j), S_B(j), then
+//    O_A += P_A V (j - 1), O_B += ...: while one softmax group works on its scores
+//    the tensor core runs the other's products;
+//  * warps 2-5 / 6-9: the softmax of A / B, one thread per pair: a lazily moved
+//    reference m (2^8 of headroom), P as 16-bit values through shared memory, O in
+//    tensor memory, rescaled only when m moves;
+//  * 4 bits: warps 10-13 turn the codes into f16 tiles, (c - 8) d with one rounding,
+//    keys and values; the queries are then f16 too, scaled by a power of two per
+//    row.
+// Values of positions that no pair of the item sees are cleared in shared memory
+// before the product, so that what they hold (NaN x 0) has no influence.
+// Every wait is bounded; a timeout sets the status word, stops issuing work,
+// waits (bounded) for copies and MMAs in flight and frees tensor memory.
+#include <cuda.h>
+#include <float.h>
+
+#include <algorithm>
+
+#include "fmd_cache.cuh"
+#include "fmd_kernels.cuh"
+
+namespace fmd {
+
+namespace {
+
+constexpr int kCkBox = 8192;       // 64 rows x 128 bytes
+constexpr int kCkPBytes = 16384;   // P: 128 pairs x 64 keys x 2 bytes
+constexpr int kCkMaxStages = 4;
+constexpr uint32_t kCkWait = 1u << 24;
+constexpr float kCkHeadroom = 8.f;
+
+struct CkArgs {
+  CacheRows r;
+  CacheAttend a;
+  float* part;    // [items][parts][256][D + 2]
+  int* counters;  // [items], zero between calls
+  int tiles;      // 256-pair tiles of the longest sequence
+  int parts, stages;
+  uint32_t f64;   // f16 pair (64, 64)
+};
+
+FMD_DEV void ck_fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+FMD_DEV float ck_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two f32 lanes at once, each rounded as the scalar instruction rounds.
+FMD_DEV float2 ck_fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+FMD_DEV float2 ck_add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+// Descriptor of an MN-major operand with the 128-byte swizzle: 64 elements of the
+// MN dimension per 128-byte row, a row per K index, MN blocks kCkBox apart.
+FMD_DEV uint64_t ck_desc_mn(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((kCkBox >> 4) & 0x3FFFu) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+FMD_DEV uint32_t ck_sub_mul(uint32_t a, uint32_t b, uint32_t d) {
+  const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  const __half2 y = __hmul2(x, *reinterpret_cast<__half2*>(&d));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// One item part of a CTA: tiles A and B of a sequence and kv head, key tiles
+// [j0, j1) of the item's list.
+struct CkWork {
+  int slot, p0, r0, h;
+  int first[2], count[2];  // first pair and pairs (0: none) of A, B
+  int lo[2], hi[2];        // positions of their first and last row
+  int sinks, w0;           // the item's key tiles: sinks, then from w0
+  int j0, j1, item, part;
+  FMD_DEV int tile(int j) const { return j < sinks ? j : w0 + j - sinks; }
+  // does A / B see anything of key tile k?
+  FMD_DEV bool need(int x, int k, int W, int S) const {
+    const int k0 = k * kPageTokens;
+    return count[x] > 0 && k0 <= hi[x] && (W == 0 || k0 + kPageTokens - 1 > lo[x] - W || k0 < S);
+  }
+};
+
+// Work of round r of this CTA: 1 a work, 0 none (skip), -1 no more.
+FMD_DEV int ck_work(const CkArgs& p, const CacheView& c, int round, CkWork& w, int* status) {
+  const int H = c.kv_heads, G = gridDim.x;
+  const int ns = p.r.count();
+  const long long total = (long long)p.tiles * ns * H * p.parts;
+  const long long at = (long long)round * G + ((round & 1) ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);
+  if ((long long)round * G >= total) return -1;
+  if (at >= total) return 0;
+  w.part = (int)(at % p.parts);
+  const long long item = at / p.parts;
+  w.item = (int)item;
+  w.h = (int)(item % H);
+  const int seq = (int)(item / H % ns), tile = p.tiles - 1 - (int)(item / H / ns);
+  int n;
+  p.r.get(seq, w.slot, w.p0, w.r0, n);
+  if (n <= 0 || !cache_slot_ok(c, w.slot, status)) return 0;
+  if (n > p.a.max_rows || w.p0 < 0 || w.p0 > c.max_pages * kPageTokens - n) {
+    cache_report(status, n > p.a.max_rows ? FMD_EINVAL : FMD_EOVERFLOW);
+    return 0;
+  }
+  const int gs = __ffs(p.a.n_heads / H) - 1;
+  const long long pairs = (long long)n << gs;
+  const long long f = (long long)tile * 256;
+  if (f >= pairs) return 0;
+  const int W = p.a.window, S = W ? p.a.sinks : 0;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    w.first[x] = (int)(f + x * 128);
+    w.count[x] = (int)max(0LL, min(128LL, pairs - w.first[x]));
+    w.lo[x] = w.p0 + (w.first[x] >> gs);
+    w.hi[x] = w.p0 + ((w.first[x] + max(w.count[x], 1) - 1) >> gs);
+  }
+  const int oldest = W && w.lo[0] >= W ? w.lo[0] - W + 1 : 0;
+  w.w0 = oldest / kPageTokens;
+  w.sinks = (min(S, w.w0 * kPageTokens) + kPageTokens - 1) / kPageTokens;
+  const int T = w.sinks + (w.count[1] > 0 ? w.hi[1] : w.hi[0]) / kPageTokens - w.w0 + 1;
+  w.j0 = (int)((long long)T * w.part / p.parts);
+  w.j1 = (int)((long long)T * (w.part + 1) / p.parts);
+  return 1;
+}
+
+template <typename T, int D, bool Q4>
+__global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
+    k_cache_chunk(const __grid_constant__ CUtensorMap tmap, CacheView c, int layer, CkArgs p, int* status) {
+  using M = typename std::conditional<Q4, __half, T>::type;
+  constexpr int QB = 128 * D * 2;                             // one query tile
+  constexpr int BLK = Q4 ? 64 * (D / 2 + D / 16) : 64 * D * 2;  // K or V of a page as stored
+  constexpr int TB = 64 * D * 2;                              // K or V of a page as an operand
+  constexpr int NB = D / 32;
+  constexpr float kPScale = Act<M>::kIsBf16 ? 0.f : 7.f;      // log2 factor of P (f16 subnormals start at 2^-14)
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t q_full[2], kv_full[kCkMaxStages], kv_empty[kCkMaxStages], cv_full[2], cv_empty[2],
+      s_full[2][2], s_empty[2][2], p_full[2], pv_done[2], o_final[2], o_empty[2], mma_done;
+  __shared__ uint32_t tmem_s;
+  __shared__ int abort_s, bad_s[kCkMaxStages], cbad_s[2], last_s;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* qp = base;                      // Q_A | Q_B | P_A | P_B | stages | (4 bits) two operand tiles
+  uint8_t* pp = qp + 2 * QB;
+  uint8_t* kvp = pp + 2 * kCkPBytes;
+  uint8_t* cvp = kvp + p.stages * 2 * BLK;
+  const int stages = p.stages, H = c.kv_heads;
+  const int W = p.a.window, S = W ? p.a.sinks : 0;
+
+  griddep_wait();
+  griddep_launch();
+  if (p.r.count() <= 0) return;
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], Q4 ? 4 : 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&cv_full[x], 4);
+      mbar_init(&cv_empty[x], 1);
+      mbar_init(&q_full[x], 128);
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(&s_full[x][s], 1);
+        mbar_init(&s_empty[x][s], 128);
+      }
+      mbar_init(&p_full[x], 128);
+      mbar_init(&pv_done[x], 1);
+      mbar_init(&o_final[x], 1);
+      mbar_init(&o_empty[x], 128);
+    }
+    mbar_init(&mma_done, 1);
+    abort_s = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_s, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+  volatile int* abort_v = &abort_s;
+
+  if (warp == 0) {
+    // ---------------- copies ----------------
+    if (lane == 0) {
+      if (!Q4) prefetch_tmap(&tmap);
+      int issued = 0, s = 0, round_s = 0;
+      bool ok = true;
+      CkWork w;
+      for (int r = 0, k; ok && (k = ck_work(p, c, r, w, status)) >= 0; ++r) {
+        if (k == 0) continue;
+        const int* table = c.page_table + (size_t)w.slot * c.max_pages;
+        for (int j = w.j0; j < w.j1; ++j) {
+          if (round_s > 0 && (*abort_v || !mbar_wait_bounded(&kv_empty[s], (round_s - 1) & 1, kCkWait))) {
+            ok = false;
+            break;
+          }
+          const int page = table[w.tile(j)];
+          const bool bad = page < 0 || page >= c.n_pages;
+          bad_s[s] = bad;
+          if (bad) {
+            cache_report(status, FMD_EINVAL);
+            mbar_arrive(&kv_full[s]);
+          } else {
+            uint8_t* dst = kvp + s * 2 * BLK;
+            mbar_arrive_expect_tx(&kv_full[s], 2 * BLK);
+            if constexpr (Q4) {
+              bulk_load(dst, c.block(layer, page, 0, w.h), BLK, &kv_full[s]);
+              bulk_load(dst + BLK, c.block(layer, page, 1, w.h), BLK, &kv_full[s]);
+            } else {
+              const int yk = (page * 2 * H + w.h) * kPageTokens, yv = yk + H * kPageTokens;
+#pragma unroll
+              for (int b = 0; b < D / 64; ++b) {
+                tma_load_2d(dst + b * kCkBox, &tmap, b * 64, yk, &kv_full[s]);
+                tma_load_2d(dst + BLK + b * kCkBox, &tmap, b * 64, yv, &kv_full[s]);
+              }
+            }
+          }
+          ++issued;
+          if (++s == stages) s = 0, ++round_s;
+        }
+      }
+      if (!ok) *abort_v = 1;
+      // copies still in flight land before the CTA retires (bounded)
+      for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
+        mbar_wait_bounded(&kv_full[i % stages], (i / stages) & 1, kCkWait);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMAs: the whole warp runs the loop, the elected lane issues ----------------
+    constexpr bool kBf = Act<M>::kIsBf16;
+    constexpr uint32_t idesc_s = umma_idesc_f16(kBf, 128, 64);
+    constexpr uint32_t idesc_o = umma_idesc_f16(kBf, 128, D) | (1u << 16);  // B (V) MN-major
+    int items[2] = {0, 0}, sn[2] = {0, 0}, pn[2] = {0, 0};
+    int st = 0, ph = 0;  // operand tile of the next key tile: its stage (4 bits: buffer) and phase
+    const int ring = Q4 ? 2 : stages;
+    uint64_t* full = Q4 ? cv_full : kv_full;
+    uint64_t* empty = Q4 ? cv_empty : kv_empty;
+    uint8_t* tiles = Q4 ? cvp : kvp;
+    const uint32_t q_a = smem_u32(qp), p_a = smem_u32(pp);
+    bool ok = true;
+    CkWork w;
+    for (int r = 0, k; ok && (k = ck_work(p, c, r, w, nullptr)) >= 0; ++r) {
+      if (k == 0) continue;
+      bool started[2] = {false, false};  // O_x holds a product of this part
+      int prev = -1, prev_st = 0;        // key tile whose P V is still to be issued
+      auto pv = [&]() -> bool {
+        const uint32_t v = smem_u32(tiles) + prev_st * 2 * TB + TB;
+        for (int x = 0; x < 2; ++x) {
+          if (!w.need(x, prev, W, S)) continue;
+          if (!started[x] && items[x] >= 1 && (*abort_v || !mbar_wait_warp(&o_empty[x], (items[x] - 1) & 1, kCkWait)))
+            return false;
+          if (*abort_v || !mbar_wait_warp(&p_full[x], pn[x] & 1, kCkWait)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16(tmem + x * 256 + 128, umma_desc_sw128(p_a + x * kCkPBytes + kk * 32), ck_desc_mn(v + kk * 2048),
+                       idesc_o, started[x] || kk != 0);
+            umma_commit(&pv_done[x]);
+          }
+          __syncwarp();
+          started[x] = true;
+          ++pn[x];
+        }
+        if (elect_one()) umma_commit(&empty[prev_st]);  // the tile is free once its MMAs have read it
+        __syncwarp();
+        return true;
+      };
+      bool got_q[2] = {false, false};
+      for (int j = w.j0; ok && j < w.j1; ++j) {
+        const int kt = w.tile(j);
+        if (*abort_v || !mbar_wait_warp(&full[st], ph, kCkWait)) {
+          ok = false;
+          break;
+        }
+        uint8_t* tile = tiles + st * 2 * TB;
+        if constexpr (!Q4) {
+          // clear the values of positions that neither A nor B sees
+          const int k0 = kt * kPageTokens;
+          const int top = w.count[1] > 0 ? w.hi[1] : w.hi[0];
+          const bool bad = bad_s[st];
+          if (bad || k0 + 63 > top || (W && k0 <= w.lo[0] - W && k0 + 63 >= S)) {
+            for (int i = lane; i < 64 * (D / 64); i += 32) {
+              const int key = k0 + (i & 63);
+              if (bad || key > top || (W && key <= w.lo[0] - W && key >= S)) {
+                uint4* row = reinterpret_cast<uint4*>(tile + TB + (i >> 6) * kCkBox + (i & 63) * 128);
+#pragma unroll
+                for (int b = 0; b < 8; ++b) row[b] = make_uint4(0, 0, 0, 0);
+              }
+            }
+            ck_fence_async();
+            __syncwarp();
+          }
+        }
+        const uint32_t kk_a = smem_u32(tile);
+        for (int x = 0; x < 2; ++x) {
+          if (!w.need(x, kt, W, S)) continue;
+          if (!got_q[x]) {
+            if (*abort_v || !mbar_wait_warp(&q_full[x], items[x] & 1, kCkWait)) {
+              ok = false;
+              break;
+            }
+            got_q[x] = true;
+          }
+          const int sb = sn[x] & 1;
+          if (sn[x] >= 2 && (*abort_v || !mbar_wait_warp(&s_empty[x][sb], ((sn[x] >> 1) + 1) & 1, kCkWait))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_f16(tmem + x * 256 + sb * 64,
+                       umma_desc_sw128(q_a + x * QB + (kk >> 2) * 2 * kCkBox + (kk & 3) * 32),
+                       umma_desc_sw128(kk_a + (kk >> 2) * kCkBox + (kk & 3) * 32), idesc_s, kk != 0);
+            umma_commit(&s_full[x][sb]);
+          }
+          __syncwarp();
+          ++sn[x];
+        }
+        if (!ok) break;
+        if (prev >= 0 && !pv()) {
+          ok = false;
+          break;
+        }
+        prev = kt;
+        prev_st = st;
+        if (++st == ring) st = 0, ph ^= 1;
+      }
+      if (ok && prev >= 0 && !pv()) ok = false;
+      if (!ok) break;
+      for (int x = 0; x < 2; ++x)
+        if (started[x]) {
+          if (elect_one()) umma_commit(&o_final[x]);
+          __syncwarp();
+          ++items[x];
+        }
+    }
+    if (!ok) *abort_v = 1;
+    if (elect_one()) umma_commit(&mma_done);  // every MMA issued so far has completed when this fires
+    __syncwarp();
+    mbar_wait_warp(&mma_done, 0, kCkWait);
+  } else if (warp < 10) {
+    // ---------------- softmax and output of tile x: one thread per pair ----------------
+    const int x = (warp - 2) >> 2, q4 = warp & 3, row = q4 * 32 + lane;
+    const int gs = __ffs(p.a.n_heads / H) - 1;
+    const uint32_t lane_addr = tmem + ((uint32_t)(q4 * 32) << 16) + x * 256, o_addr = lane_addr + 128;
+    // tensor-memory loads and stores are warp-wide: a wait counts for all lanes or none
+    auto wwait = [&](uint64_t* bar, uint32_t parity) -> bool {
+      const bool mine = !*abort_v && mbar_wait_bounded(bar, parity, kCkWait);
+      return __all_sync(0xffffffffu, mine);
+    };
+    int sn = 0, pn = 0, items = 0;
+    bool ok = true;
+    int cb = 0;  // (4 bits) buffer of the next key tile; (16 bits) its stage
+    const int ring = Q4 ? 2 : stages;
+    CkWork w;
+    // a warp whose wait gave up goes on without work: the parts' barriers below count every warp
+    for (int r = 0, kd; (ok || p.parts > 1) && (kd = ck_work(p, c, r, w, nullptr)) >= 0; ++r) {
+      if (kd == 0) continue;
+      bool any = false;
+      for (int j = w.j0; j < w.j1 && !any && ok; ++j) any = w.need(x, w.tile(j), W, S);
+      float m_ref = -INFINITY, l = 0.f, scale = p.a.scale * 1.4426950408889634f;
+      const int pr = w.first[x] + row;
+      const bool live = row < w.count[x];
+      const int pos = w.p0 + (pr >> gs);
+      if (any) {
+        // ---- the query row into the operand tile. The last part's scores are complete (their
+        // s_full was waited for), so its queries are no longer read
+        const T* src = (const T*)p.a.q + (size_t)(w.r0 + (pr >> gs)) * p.a.q_row +
+                       (size_t)((w.h << gs) + (pr & ((1 << gs) - 1))) * p.a.q_head;
+        uint4 u[D / 8];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          u[i] = live ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
+        if constexpr (Q4) {
+          float amax = 0.f;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const uint32_t v[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = Act<T>::unpack2(v[e]);
+              amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+          // 2^e brings the largest magnitude to [1, 2)
+          const int e2 = min(126, amax > 0.f && amax <= FLT_MAX ? 127 - (int)(__float_as_uint(amax) >> 23) : 0);
+          const float up = __uint_as_float((uint32_t)(127 + e2) << 23);
+          scale *= __uint_as_float((uint32_t)(127 - e2) << 23);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            uint32_t v[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = Act<T>::unpack2(v[e]);
+              v[e] = Act<__half>::pack2(f.x * up, f.y * up);
+            }
+            u[i] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        uint8_t* dst = qp + x * QB + row * 128;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          *reinterpret_cast<uint4*>(dst + (i >> 3) * 2 * kCkBox + (((i & 7) ^ (row & 7)) << 4)) = u[i];
+        ck_fence_async();
+        mbar_arrive(&q_full[x]);
+      }
+      bool first = true;
+      for (int j = w.j0; j < w.j1 && ok; ++j) {
+        const int kt = w.tile(j), k0 = kt * kPageTokens, stage = cb;
+        if (++cb == ring) cb = 0;
+        if (!w.need(x, kt, W, S)) continue;
+        const int sb = sn & 1;
+        if (!wwait(&s_full[x][sb], (sn >> 1) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        float s[64];
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2) {
+          uint32_t v[32];
+          tmem_ld32(lane_addr + sb * 64 + h2 * 32, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[h2 * 32 + i] = __uint_as_float(v[i]);
+        }
+        tc_fence_before();
+        mbar_arrive(&s_empty[x][sb]);
+        ++sn;
+        const bool bad = Q4 ? cbad_s[stage] : bad_s[stage];
+        if (bad || k0 + 63 > pos || (W && k0 <= pos - W && k0 + 63 >= S)) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (bad || k0 + i > pos || (W && k0 + i <= pos - W && k0 + i >= S)) s[i] = -INFINITY;
+        }
+        float mc[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mc[i] = s[i];
+#pragma unroll
+        for (int i = 8; i < 64; ++i) mc[i & 7] = fmaxf(mc[i & 7], s[i]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mc[0] = fmaxf(mc[0], mc[i]);
+        const float mx = mc[0] * scale;  // the scale is positive
+        bool moves = false;
+        if (first) m_ref = mx;
+        else moves = mx > m_ref + kCkHeadroom;
+        if (__any_sync(0xffffffffu, moves)) {
+          // O is complete up to the last P V of this tile
+          if (!wwait(&pv_done[x], (pn - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const float f = moves ? ck_ex2(m_ref - mx) : 1.f;  // 0 when the row saw nothing yet
+#pragma unroll
+          for (int h2 = 0; h2 < D / 32; ++h2) {
+            uint32_t v[32];
+            tmem_ld32(o_addr + h2 * 32, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+            tmem_st32(o_addr + h2 * 32, v);
+          }
+          tmem_st_wait();
+          if (moves) {
+            l *= f;
+            m_ref = mx;
+          }
+        }
+        {
+          const float b = m_ref == -INFINITY ? 0.f : m_ref - kPScale;
+          float2 a4[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a4[i] = make_float2(0.f, 0.f);
+          const float2 sc2 = make_float2(scale, scale), nb = make_float2(-b, -b);
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) {
+            float2 v = ck_fma2(make_float2(s[i], s[i + 1]), sc2, nb);
+            v.x = ck_ex2(v.x);
+            v.y = ck_ex2(v.y);
+            s[i] = v.x;
+            s[i + 1] = v.y;
+            a4[(i >> 1) & 3] = ck_add2(a4[(i >> 1) & 3], v);
+          }
+          l += ((a4[0].x + a4[0].y) + (a4[1].x + a4[1].y)) + ((a4[2].x + a4[2].y) + (a4[3].x + a4[3].y));
+        }
+        // the P buffer was last read by the previous P V of this tile
+        if (pn >= 1 && !wwait(&pv_done[x], (pn - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        uint8_t* prow = pp + x * kCkPBytes + row * 128;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint4 v;
+          v.x = Act<M>::pack2(s[8 * i + 0], s[8 * i + 1]);
+          v.y = Act<M>::pack2(s[8 * i + 2], s[8 * i + 3]);
+          v.z = Act<M>::pack2(s[8 * i + 4], s[8 * i + 5]);
+          v.w = Act<M>::pack2(s[8 * i + 6], s[8 * i + 7]);
+          *reinterpret_cast<uint4*>(prow + ((i ^ (row & 7)) << 4)) = v;
+        }
+        ck_fence_async();
+        tc_fence_before();
+        mbar_arrive(&p_full[x]);
+        ++pn;
+        first = false;
+      }
+      if (ok && any) {
+        if (wwait(&o_final[x], items & 1)) tc_fence_after();
+        else ok = false;
+      }
+      if (!ok) {
+        any = false;
+        *abort_v = 1;
+      }
+      float* pt = p.parts > 1 ? p.part + (((size_t)w.item * p.parts + w.part) * 256 + x * 128 + row) * (D + 2) : nullptr;
+      const float inv = 1.f / l;
+      T* dst = (T*)p.a.out + (size_t)(w.r0 + (pr >> gs)) * p.a.out_row +
+               (size_t)((w.h << gs) + (pr & ((1 << gs) - 1))) * p.a.out_head;
+      if (any) {
+#pragma unroll
+        for (int h2 = 0; h2 < D / 32; ++h2) {
+          uint32_t v[32];
+          tmem_ld32(o_addr + h2 * 32, v);
+          tmem_ld_wait();
+          if (!live) {
+          } else if (pt) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              *reinterpret_cast<float2*>(pt + h2 * 32 + i) = make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint4 y;
+              y.x = Act<T>::pack2(__uint_as_float(v[8 * i + 0]) * inv, __uint_as_float(v[8 * i + 1]) * inv);
+              y.y = Act<T>::pack2(__uint_as_float(v[8 * i + 2]) * inv, __uint_as_float(v[8 * i + 3]) * inv);
+              y.z = Act<T>::pack2(__uint_as_float(v[8 * i + 4]) * inv, __uint_as_float(v[8 * i + 5]) * inv);
+              y.w = Act<T>::pack2(__uint_as_float(v[8 * i + 6]) * inv, __uint_as_float(v[8 * i + 7]) * inv);
+              *reinterpret_cast<uint4*>(dst + h2 * 32 + 8 * i) = y;
+            }
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&o_empty[x]);
+        ++items;
+      }
+      if (pt) {
+        if (live) *reinterpret_cast<float2*>(pt + D) = make_float2(m_ref, l);
+        // the last part of the item merges all, one warp per pair
+        named_sync(1, 256);
+        if (tid == 64) {
+          __threadfence();
+          last_s = atomicAdd(&p.counters[w.item], 1) == p.parts - 1;
+          if (last_s) {
+            __threadfence();
+            p.counters[w.item] = 0;
+          }
+        }
+        named_sync(1, 256);
+        const bool last = last_s;
+        if (last) {
+          const float* all = p.part + (size_t)w.item * p.parts * 256 * (D + 2);
+          for (int k = warp - 2; k < w.count[0] + w.count[1]; k += 8) {
+            auto at = [&](int sp) { return all + ((size_t)sp * 256 + k) * (D + 2); };
+            float Mx = -INFINITY;
+            for (int sp = 0; sp < p.parts; ++sp) Mx = fmaxf(Mx, __ldcg(at(sp) + D));
+            const float b = Mx == -INFINITY ? 0.f : Mx;
+            float L = 0.f;
+            float2 acc[D / 64];
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) acc[i] = make_float2(0.f, 0.f);
+            for (int sp = 0; sp < p.parts; ++sp) {
+              const float lw = __ldcg(at(sp) + D + 1);
+              if (lw == 0.f) continue;  // the part saw none of the pair's keys
+              const float f = ck_ex2(__ldcg(at(sp) + D) - b);
+              L = fmaf(lw, f, L);
+#pragma unroll
+              for (int i = 0; i < D / 64; ++i) {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(at(sp) + i * 64 + lane * 2));
+                acc[i].x = fmaf(v.x, f, acc[i].x);
+                acc[i].y = fmaf(v.y, f, acc[i].y);
+              }
+            }
+            const int pk = w.first[0] + k;
+            T* o = (T*)p.a.out + (size_t)(w.r0 + (pk >> gs)) * p.a.out_row +
+                   (size_t)((w.h << gs) + (pk & ((1 << gs) - 1))) * p.a.out_head;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i)
+              *reinterpret_cast<uint32_t*>(o + i * 64 + lane * 2) = Act<T>::pack2(acc[i].x / L, acc[i].y / L);
+          }
+        }
+      }
+    }
+    if (!ok) *abort_v = 1;
+  } else if constexpr (Q4) {
+    // ---------------- 4 bits: codes to f16 operand tiles ----------------
+    const int ct = tid - 320, cw = ct >> 5;
+    int s = 0, ph = 0, b = 0, round_b = 0;
+    bool ok = true;
+    const uint32_t f64 = p.f64, k72 = 0x54805480u;  // f16 64, 72
+    CkWork w;
+    for (int r = 0, k; ok && (k = ck_work(p, c, r, w, nullptr)) >= 0; ++r) {
+      if (k == 0) continue;
+      const int top = w.count[1] > 0 ? w.hi[1] : w.hi[0];
+      for (int j = w.j0; j < w.j1; ++j) {
+        const int k0 = w.tile(j) * kPageTokens;
+        if (*abort_v || !mbar_wait_warp(&kv_full[s], ph, kCkWait) ||
+            (round_b > 0 && !mbar_wait_warp(&cv_empty[b], (round_b - 1) & 1, kCkWait))) {
+          ok = false;
+          break;
+        }
+        const uint8_t* src = kvp + s * 2 * BLK;
+        uint8_t* dst = cvp + b * 2 * TB;
+        const bool bad = bad_s[s];
+        if (ct == 0) cbad_s[b] = bad;
+        // rows of 16 keys per warp; a lane takes chunk lane & 3 of key (lane >> 2)'s place:
+        // keys 4 apart in a quarter-warp, whose swizzled rows share no banks
+        if constexpr (NB == 4) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int kk = lane >> 2, key = cw * 16 + i * 8 + (kk & 1) * 4 + (kk >> 1), ch = lane & 3;
+            {
+              const uint4 u = *reinterpret_cast<const uint4*>(src + key * 64 + ch * 16);
+              const uint2 sc = *reinterpret_cast<const uint2*>(src + 4096 + key * 8);
+              const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+              const uint32_t d2[4] = {__byte_perm(sc.x, 0, 0x1010), __byte_perm(sc.x, 0, 0x3232),
+                                      __byte_perm(sc.y, 0, 0x1010), __byte_perm(sc.y, 0, 0x3232)};
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                uint4 o;
+                o.x = ck_sub_mul(((wd[g] << 4) & 0x00f000f0u) | f64, k72, d2[g]);
+                o.y = ck_sub_mul((wd[g] & 0x00f000f0u) | f64, k72, d2[g]);
+                o.z = ck_sub_mul(((wd[g] >> 4) & 0x00f000f0u) | f64, k72, d2[g]);
+                o.w = ck_sub_mul(((wd[g] >> 8) & 0x00f000f0u) | f64, k72, d2[g]);
+                const int oc = 4 * g + ch;
+                *reinterpret_cast<uint4*>(dst + (oc >> 3) * kCkBox + key * 128 + (((oc & 7) ^ (key & 7)) << 4)) = o;
+              }
+            }
+            {
+              const uint4 u = *reinterpret_cast<const uint4*>(src + BLK + key * 64 + ch * 16);
+              uint32_t d2 = *reinterpret_cast<const uint16_t*>(src + BLK + 4096 + key * 8 + ch * 2);
+              const int kp = k0 + key;
+              const bool hide = bad || kp > top || (W && kp <= w.lo[0] - W && kp >= S);
+              d2 = hide ? 0u : d2 | d2 << 16;
+              const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                // nibbles 2 i, 2 i + 1 side by side: bytes of the even and the odd ones interleaved
+                const uint32_t ev = (wd[g] << 4) & 0xf0f0f0f0u, od = wd[g] & 0xf0f0f0f0u;
+                uint4 o;
+                o.x = ck_sub_mul((__byte_perm(ev, od, 0x0400) & 0x00ff00ffu) | f64, k72, d2);
+                o.y = ck_sub_mul((__byte_perm(ev, od, 0x0501) & 0x00ff00ffu) | f64, k72, d2);
+                o.z = ck_sub_mul((__byte_perm(ev, od, 0x0602) & 0x00ff00ffu) | f64, k72, d2);
+                o.w = ck_sub_mul((__byte_perm(ev, od, 0x0703) & 0x00ff00ffu) | f64, k72, d2);
+                const int oc = 4 * ch + g;
+                *reinterpret_cast<uint4*>(dst + TB + (oc >> 3) * kCkBox + key * 128 + (((oc & 7) ^ (key & 7)) << 4)) = o;
+              }
+            }
+          }
+        } else {
+          // head_dim 64: 8-byte key chunks of two words, a value row of 8 words
+          const int kk = lane >> 2, ch = lane & 3;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int key = cw * 16 + i * 8 + (kk & 1) * 4 + (kk >> 1);
+            const uint2 u = *reinterpret_cast<const uint2*>(src + key * 32 + ch * 8);
+            const uint32_t sc = *reinterpret_cast<const uint32_t*>(src + 2048 + key * 4);
+            const uint32_t wd[2] = {u.x, u.y}, d2[2] = {__byte_perm(sc, 0, 0x1010), __byte_perm(sc, 0, 0x3232)};
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              uint4 o;
+              o.x = ck_sub_mul(((wd[g] << 4) & 0x00f000f0u) | f64, k72, d2[g]);
+              o.y = ck_sub_mul((wd[g] & 0x00f000f0u) | f64, k72, d2[g]);
+              o.z = ck_sub_mul(((wd[g] >> 4) & 0x00f000f0u) | f64, k72, d2[g]);
+              o.w = ck_sub_mul(((wd[g] >> 8) & 0x00f000f0u) | f64, k72, d2[g]);
+              *reinterpret_cast<uint4*>(dst + key * 128 + (((4 * g + ch) ^ (key & 7)) << 4)) = o;
+            }
+            const uint2 v = *reinterpret_cast<const uint2*>(src + BLK + key * 32 + ch * 8);
+            uint32_t dv = *reinterpret_cast<const uint16_t*>(src + BLK + 2048 + key * 4 + (ch >> 1) * 2);
+            const int kp = k0 + key;
+            const bool hide = bad || kp > top || (W && kp <= w.lo[0] - W && kp >= S);
+            dv = hide ? 0u : dv | dv << 16;
+            const uint32_t vd[2] = {v.x, v.y};
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const uint32_t ev = (vd[g] << 4) & 0xf0f0f0f0u, od = vd[g] & 0xf0f0f0f0u;
+              uint4 o;
+              o.x = ck_sub_mul((__byte_perm(ev, od, 0x0400) & 0x00ff00ffu) | f64, k72, dv);
+              o.y = ck_sub_mul((__byte_perm(ev, od, 0x0501) & 0x00ff00ffu) | f64, k72, dv);
+              o.z = ck_sub_mul((__byte_perm(ev, od, 0x0602) & 0x00ff00ffu) | f64, k72, dv);
+              o.w = ck_sub_mul((__byte_perm(ev, od, 0x0703) & 0x00ff00ffu) | f64, k72, dv);
+              *reinterpret_cast<uint4*>(dst + TB + key * 128 + (((2 * ch + g) ^ (key & 7)) << 4)) = o;
+            }
+          }
+        }
+        ck_fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&cv_full[b]);
+          mbar_arrive(&kv_empty[s]);
+        }
+        if (++s == stages) s = 0, ph ^= 1;
+        if (++b == 2) b = 0, ++round_b;
+      }
+    }
+    if (!ok) *abort_v = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && abort_s) report_timeout(status, kSiteCacheChunk);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+struct CkShape {
+  int tiles, parts, stages, grid, smem;
+  long long items;
+};
+
+// Parts of an item: enough for every SM when there are fewer items than SMs.
+CkShape ck_shape(const CacheView& c, int n_heads, int n_seqs, int max_rows) {
+  CkShape s;
+  const long long pairs = (long long)max_rows * (n_heads / c.kv_heads);
+  s.tiles = (int)((pairs + 255) / 256);
+  s.items = (long long)s.tiles * n_seqs * c.kv_heads;
+  s.parts = s.items >= 148 ? 1 : (int)(148 / s.items);
+  s.parts = std::min(s.parts, std::max(1, std::min(32, c.max_pages / 4)));
+  s.grid = (int)std::min<long long>(148, s.items * s.parts);
+  const bool q4 = c.format == FMD_CACHE_Q4;
+  const int tb = 64 * c.head_dim * 2, stage = 2 * (int)c.block_bytes();
+  s.stages = q4 ? 4 : 3;
+  s.smem = 1024 + 2 * 128 * c.head_dim * 2 + 2 * kCkPBytes + s.stages * stage + (q4 ? 2 * 2 * tb : 0);
+  return s;
+}
+
+}  // namespace
+
+// counters, then the parts
+size_t cache_chunk_workspace(const CacheView& c, int n_heads, int n_seqs, int max_rows) {
+  const CkShape s = ck_shape(c, n_heads, n_seqs, max_rows);
+  if (s.parts == 1) return 0;
+  return FMD_CACHE_WORKSPACE_ZERO + (size_t)s.items * s.parts * 256 * (c.head_dim + 2) * 4;
+}
+
+cudaError_t launch_cache_chunk(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAttend& a,
+                               void* workspace, int* status, cudaStream_t s) {
+  const bool q4 = c.format == FMD_CACHE_Q4;
+  const CkShape sh = ck_shape(c, a.n_heads, r.n_seqs, a.max_rows);
+  CUtensorMap map{};
+  if (!q4 && !cache_tensor_map(&map, c, layer)) return cudaErrorNotSupported;
+  CkArgs p;
+  p.r = r;
+  p.a = a;
+  p.counters = (int*)workspace;
+  p.part = (float*)((uint8_t*)workspace + FMD_CACHE_WORKSPACE_ZERO);
+  p.tiles = sh.tiles;
+  p.parts = sh.parts;
+  p.stages = sh.stages;
+  p.f64 = 0x54005400u;
+  auto go = [&](auto kern) -> cudaError_t {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sh.grid);
+    cfg.blockDim = dim3(q4 ? 448 : 320);
+    cfg.dynamicSmemBytes = sh.smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, map, c, layer, p, status);
+  };
+  auto by_d = [&](auto t, auto f) {
+    using T = decltype(t);
+    constexpr bool F = decltype(f)::value;
+    return c.head_dim == 128 ? go(k_cache_chunk<T, 128, F>) : go(k_cache_chunk<T, 64, F>);
+  };
+  auto by_f = [&](auto t) { return q4 ? by_d(t, std::true_type{}) : by_d(t, std::false_type{}); };
+  return bf16 ? by_f(__nv_bfloat16{}) : by_f(__half{});
+}
+
+}  // namespace fmd
