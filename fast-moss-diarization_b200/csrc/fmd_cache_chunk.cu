@@ -19,15 +19,16 @@
 //
 //  * warp 0: copies of the page tiles into a ring (16 bits: 2D TMA with the
 //    128-byte swizzle; 4 bits: bulk copies of the blocks);
-//  * warp 1: tcgen05.mma, f32 accumulators in tensor memory: S_A(j), S_B(j), then
-//    O_A += P_A V (j - 1), O_B += ...: while one softmax group works on its scores
-//    the tensor core runs the other's products;
-//  * warps 2-5 / 6-9: the softmax of A / B, one thread per pair: a lazily moved
+//  * warp 1 / 2: tcgen05.mma of A / B, f32 accumulators in tensor memory: S(j), then
+//    O += P V (j - 1). One warp for both spent 3,350 cycles a key tile, most of them on
+//    its waits and commits one after another, for 1,400 cycles of products;
+//  * warps 4-7 / 8-11: the softmax of A / B, one thread per pair: a lazily moved
 //    reference m (2^8 of headroom), P as 16-bit values through shared memory, O in
 //    tensor memory, rescaled only when m moves;
-//  * 4 bits: warps 10-13 turn the codes into f16 tiles, (c - 8) d with one rounding,
+//  * 4 bits: warps 12-19 turn the codes into f16 tiles, (c - 8) d with one rounding,
 //    keys and values; the queries are then f16 too, scaled by a power of two per
 //    row.
+// Registers go where they are needed: the softmax groups take what the others give.
 // Values of positions that no pair of the item sees are cleared in shared memory
 // before the product, so that what they hold (NaN x 0) has no influence.
 // Every wait is bounded; a timeout sets the status word, stops issuing work,
@@ -49,6 +50,12 @@ constexpr int kCkPBytes = 16384;   // P: 128 pairs x 64 keys x 2 bytes
 constexpr int kCkMaxStages = 4;
 constexpr uint32_t kCkWait = 1u << 24;
 constexpr float kCkHeadroom = 8.f;
+
+constexpr int ck_threads(bool q4) { return q4 ? 640 : 384; }
+// Registers of a thread at launch, of a softmax thread, of any other; the sums fit.
+//   16 bits: 384 x 168 = 256 x 208 + 128 x 88; 4 bits: 640 x 96 > 256 x 152 + 384 x 56
+template <int N> FMD_DEV void ck_more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N> FMD_DEV void ck_fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
 
 struct CkArgs {
   CacheRows r;
@@ -101,14 +108,35 @@ struct CkWork {
   int first[2], count[2];  // first pair and pairs (0: none) of A, B
   int lo[2], hi[2];        // positions of their first and last row
   int sinks, w0;           // the item's key tiles: sinks, then from w0
+  int lim, from[2], end[2];  // those A / B see: before lim, or from from[x] on, before end[x]
   int j0, j1, item, part;
   FMD_DEV int tile(int j) const { return j < sinks ? j : w0 + j - sinks; }
-  // does A / B see anything of key tile k?
-  FMD_DEV bool need(int x, int k, int W, int S) const {
-    const int k0 = k * kPageTokens;
-    return count[x] > 0 && k0 <= hi[x] && (W == 0 || k0 + kPageTokens - 1 > lo[x] - W || k0 < S);
-  }
 };
+// What concerns one of A, B, in registers of its own (a run-time index into
+// CkWork's arrays would put them in local memory).
+struct CkSide {
+  int first, count, lim, from, end;
+  FMD_DEV CkSide(const CkWork& w, int x)
+      : first(x ? w.first[1] : w.first[0]),
+        count(x ? w.count[1] : w.count[0]),
+        lim(w.lim),
+        from(x ? w.from[1] : w.from[0]),
+        end(x ? w.end[1] : w.end[0]) {}
+  FMD_DEV bool need(int j) const { return j < end && (j < lim || j >= from); }
+};
+
+// Bounded wait with one outcome for the warp; gives up early when another role has.
+FMD_DEV bool ck_wait(uint64_t* bar, uint32_t parity, volatile int* abort_v) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t i = 1; !ok && i < kCkWait; ++i) {
+      ok = mbar_try_wait(bar, parity);
+      if (!ok && (*abort_v || ((i & 63) == 0 && globaltimer_ns() - t0 > kWaitNsCap))) break;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
 
 // Work of round r of this CTA: 1 a work, 0 none (skip), -1 no more.
 FMD_DEV int ck_work(const CkArgs& p, const CacheView& c, int round, CkWork& w, int* status) {
@@ -146,23 +174,30 @@ FMD_DEV int ck_work(const CkArgs& p, const CacheView& c, int round, CkWork& w, i
   w.w0 = oldest / kPageTokens;
   w.sinks = (min(S, w.w0 * kPageTokens) + kPageTokens - 1) / kPageTokens;
   const int T = w.sinks + (w.count[1] > 0 ? w.hi[1] : w.hi[0]) / kPageTokens - w.w0 + 1;
+  w.lim = w.sinks + max(0, (min(S, w.hi[1]) + kPageTokens - 1) / kPageTokens - w.w0);
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    w.from[x] = w.sinks + (W && w.lo[x] >= W ? w.lo[x] - W + 1 : 0) / kPageTokens - w.w0;
+    w.end[x] = w.count[x] > 0 ? w.sinks + w.hi[x] / kPageTokens - w.w0 + 1 : 0;
+  }
   w.j0 = (int)((long long)T * w.part / p.parts);
   w.j1 = (int)((long long)T * (w.part + 1) / p.parts);
   return 1;
 }
 
 template <typename T, int D, bool Q4>
-__global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
+__global__ void __launch_bounds__(ck_threads(Q4), 1)
     k_cache_chunk(const __grid_constant__ CUtensorMap tmap, CacheView c, int layer, CkArgs p, int* status) {
   using M = typename std::conditional<Q4, __half, T>::type;
   constexpr int QB = 128 * D * 2;                             // one query tile
   constexpr int BLK = Q4 ? 64 * (D / 2 + D / 16) : 64 * D * 2;  // K or V of a page as stored
   constexpr int TB = 64 * D * 2;                              // K or V of a page as an operand
   constexpr int NB = D / 32;
+  constexpr int kMore = Q4 ? 152 : 208, kFew = Q4 ? 56 : 88;
   constexpr float kPScale = Act<M>::kIsBf16 ? 0.f : 7.f;      // log2 factor of P (f16 subnormals start at 2^-14)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full[2], kv_full[kCkMaxStages], kv_empty[kCkMaxStages], cv_full[2], cv_empty[2],
-      s_full[2][2], s_empty[2][2], p_full[2], pv_done[2], o_final[2], o_empty[2], mma_done;
+      s_full[2][2], s_empty[2][2], p_full[2], pv_done[2], o_final[2], o_empty[2], mma_done[2];
   __shared__ uint32_t tmem_s;
   __shared__ int abort_s, bad_s[kCkMaxStages], cbad_s[2], last_s;
 
@@ -181,11 +216,12 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], Q4 ? 4 : 1);
+      mbar_init(&kv_empty[s], Q4 ? 8 : 2);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&cv_full[x], 4);
-      mbar_init(&cv_empty[x], 1);
+      mbar_init(&cv_full[x], 8);
+      mbar_init(&cv_empty[x], 2);
+      mbar_init(&mma_done[x], 1);
       mbar_init(&q_full[x], 128);
       for (int s = 0; s < 2; ++s) {
         mbar_init(&s_full[x][s], 1);
@@ -196,7 +232,6 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
       mbar_init(&o_final[x], 1);
       mbar_init(&o_empty[x], 128);
     }
-    mbar_init(&mma_done, 1);
     abort_s = 0;
     fence_barrier_init();
   }
@@ -210,6 +245,8 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
   const uint32_t tmem = tmem_s;
   volatile int* abort_v = &abort_s;
 
+  if (warp < 4) {
+  ck_fewer_regs<kFew>();
   if (warp == 0) {
     // ---------------- copies ----------------
     if (lane == 0) {
@@ -255,132 +292,119 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
       for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
         mbar_wait_bounded(&kv_full[i % stages], (i / stages) & 1, kCkWait);
     }
-  } else if (warp == 1) {
-    // ---------------- MMAs: the whole warp runs the loop, the elected lane issues ----------------
+  } else if (warp == 1 || warp == 2) {
+    // ---------------- MMAs of tile x: the whole warp runs the loop, the elected lane issues ----------------
+    const int x = warp - 1;
     constexpr bool kBf = Act<M>::kIsBf16;
     constexpr uint32_t idesc_s = umma_idesc_f16(kBf, 128, 64);
     constexpr uint32_t idesc_o = umma_idesc_f16(kBf, 128, D) | (1u << 16);  // B (V) MN-major
-    int items[2] = {0, 0}, sn[2] = {0, 0}, pn[2] = {0, 0};
+    int items = 0, sn = 0, pn = 0;
     int st = 0, ph = 0;  // operand tile of the next key tile: its stage (4 bits: buffer) and phase
     const int ring = Q4 ? 2 : stages;
     uint64_t* full = Q4 ? cv_full : kv_full;
     uint64_t* empty = Q4 ? cv_empty : kv_empty;
     uint8_t* tiles = Q4 ? cvp : kvp;
-    const uint32_t q_a = smem_u32(qp), p_a = smem_u32(pp);
+    const uint32_t s_tmem = tmem + x * 256, o_tmem = s_tmem + 128;
+    // descriptors of the first operand tiles; addresses below 256 KB never carry out of
+    // the address field, so the others are sums
+    const uint64_t dq = umma_desc_sw128(smem_u32(qp) + x * QB), dp = umma_desc_sw128(smem_u32(pp) + x * kCkPBytes);
+    const uint64_t dk = umma_desc_sw128(smem_u32(tiles)), dv = ck_desc_mn(smem_u32(tiles) + TB);
     bool ok = true;
     CkWork w;
     for (int r = 0, k; ok && (k = ck_work(p, c, r, w, nullptr)) >= 0; ++r) {
       if (k == 0) continue;
-      bool started[2] = {false, false};  // O_x holds a product of this part
-      int prev = -1, prev_st = 0;        // key tile whose P V is still to be issued
-      auto pv = [&]() -> bool {
-        const uint32_t v = smem_u32(tiles) + prev_st * 2 * TB + TB;
-        for (int x = 0; x < 2; ++x) {
-          if (!w.need(x, prev, W, S)) continue;
-          if (!started[x] && items[x] >= 1 && (*abort_v || !mbar_wait_warp(&o_empty[x], (items[x] - 1) & 1, kCkWait)))
-            return false;
-          if (*abort_v || !mbar_wait_warp(&p_full[x], pn[x] & 1, kCkWait)) return false;
-          tc_fence_after();
-          if (elect_one()) {
+      const CkSide side(w, x);
+      const int top = w.count[1] > 0 ? w.hi[1] : w.hi[0], low = w.lo[0];
+      bool started = false, got_q = false;  // O holds a product, the queries are there
+      int prev_st = 0;                      // operand tile of key tile j - 1
+      for (int j = w.j0; j <= w.j1; ++j) {
+        if (j < w.j1) {
+          if (!(ok = ck_wait(&full[st], ph, abort_v))) break;
+          if (side.need(j)) {
+            // ---- S(j) = Q K^T
+            if constexpr (!Q4) {
+              // clear the values of positions that neither A nor B sees (both warps: the same zeros)
+              const int k0 = w.tile(j) * kPageTokens;
+              const bool bad = bad_s[st];
+              if (bad || k0 + 63 > top || (W && k0 <= low - W && k0 + 63 >= S)) {
+                for (int i = lane; i < 64 * (D / 64); i += 32) {
+                  const int key = k0 + (i & 63);
+                  if (bad || key > top || (W && key <= low - W && key >= S)) {
+                    uint4* row =
+                        reinterpret_cast<uint4*>(tiles + st * 2 * TB + TB + (i >> 6) * kCkBox + (i & 63) * 128);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_f16(tmem + x * 256 + 128, umma_desc_sw128(p_a + x * kCkPBytes + kk * 32), ck_desc_mn(v + kk * 2048),
-                       idesc_o, started[x] || kk != 0);
-            umma_commit(&pv_done[x]);
-          }
-          __syncwarp();
-          started[x] = true;
-          ++pn[x];
-        }
-        if (elect_one()) umma_commit(&empty[prev_st]);  // the tile is free once its MMAs have read it
-        __syncwarp();
-        return true;
-      };
-      bool got_q[2] = {false, false};
-      for (int j = w.j0; ok && j < w.j1; ++j) {
-        const int kt = w.tile(j);
-        if (*abort_v || !mbar_wait_warp(&full[st], ph, kCkWait)) {
-          ok = false;
-          break;
-        }
-        uint8_t* tile = tiles + st * 2 * TB;
-        if constexpr (!Q4) {
-          // clear the values of positions that neither A nor B sees
-          const int k0 = kt * kPageTokens;
-          const int top = w.count[1] > 0 ? w.hi[1] : w.hi[0];
-          const bool bad = bad_s[st];
-          if (bad || k0 + 63 > top || (W && k0 <= w.lo[0] - W && k0 + 63 >= S)) {
-            for (int i = lane; i < 64 * (D / 64); i += 32) {
-              const int key = k0 + (i & 63);
-              if (bad || key > top || (W && key <= w.lo[0] - W && key >= S)) {
-                uint4* row = reinterpret_cast<uint4*>(tile + TB + (i >> 6) * kCkBox + (i & 63) * 128);
-#pragma unroll
-                for (int b = 0; b < 8; ++b) row[b] = make_uint4(0, 0, 0, 0);
+                    for (int b = 0; b < 8; ++b) row[b] = make_uint4(0, 0, 0, 0);
+                  }
+                }
+                ck_fence_async();
+                __syncwarp();
               }
             }
-            ck_fence_async();
-            __syncwarp();
-          }
-        }
-        const uint32_t kk_a = smem_u32(tile);
-        for (int x = 0; x < 2; ++x) {
-          if (!w.need(x, kt, W, S)) continue;
-          if (!got_q[x]) {
-            if (*abort_v || !mbar_wait_warp(&q_full[x], items[x] & 1, kCkWait)) {
-              ok = false;
-              break;
+            if (!got_q) {
+              if (!(ok = ck_wait(&q_full[x], items & 1, abort_v))) break;
+              got_q = true;
             }
-            got_q[x] = true;
-          }
-          const int sb = sn[x] & 1;
-          if (sn[x] >= 2 && (*abort_v || !mbar_wait_warp(&s_empty[x][sb], ((sn[x] >> 1) + 1) & 1, kCkWait))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          if (elect_one()) {
+            const int sb = sn & 1;
+            if (sn >= 2 && !(ok = ck_wait(&s_empty[x][sb], ((sn >> 1) + 1) & 1, abort_v))) break;
+            tc_fence_after();
+            const uint64_t kd = dk + (uint64_t)(st * (2 * TB / 16));
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              umma_f16(tmem + x * 256 + sb * 64,
-                       umma_desc_sw128(q_a + x * QB + (kk >> 2) * 2 * kCkBox + (kk & 3) * 32),
-                       umma_desc_sw128(kk_a + (kk >> 2) * kCkBox + (kk & 3) * 32), idesc_s, kk != 0);
-            umma_commit(&s_full[x][sb]);
+              for (int kk = 0; kk < D / 16; ++kk)
+                umma_f16(s_tmem + sb * 64, dq + ((kk >> 2) * 2 * kCkBox + (kk & 3) * 32) / 16,
+                         kd + ((kk >> 2) * kCkBox + (kk & 3) * 32) / 16, idesc_s, kk != 0);
+              umma_commit(&s_full[x][sb]);
+            }
+            __syncwarp();
+            ++sn;
           }
-          __syncwarp();
-          ++sn[x];
         }
-        if (!ok) break;
-        if (prev >= 0 && !pv()) {
-          ok = false;
-          break;
+        if (j > w.j0) {
+          if (side.need(j - 1)) {
+            // ---- O += P(j - 1) V
+            if (!started && items >= 1 && !(ok = ck_wait(&o_empty[x], (items - 1) & 1, abort_v))) break;
+            if (!(ok = ck_wait(&p_full[x], pn & 1, abort_v))) break;
+            tc_fence_after();
+            const uint64_t vd = dv + (uint64_t)(prev_st * (2 * TB / 16));
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                umma_f16(o_tmem, dp + kk * 32 / 16, vd + kk * 2048 / 16, idesc_o, started || kk != 0);
+              umma_commit(&pv_done[x]);
+              umma_commit(&empty[prev_st]);  // this warp's products have read the tile when it fires
+            }
+            __syncwarp();
+            started = true;
+            ++pn;
+          } else if (lane == 0) {
+            mbar_arrive(&empty[prev_st]);
+          }
         }
-        prev = kt;
-        prev_st = st;
-        if (++st == ring) st = 0, ph ^= 1;
+        if (j < w.j1) {
+          prev_st = st;
+          if (++st == ring) st = 0, ph ^= 1;
+        }
       }
-      if (ok && prev >= 0 && !pv()) ok = false;
       if (!ok) break;
-      for (int x = 0; x < 2; ++x)
-        if (started[x]) {
-          if (elect_one()) umma_commit(&o_final[x]);
-          __syncwarp();
-          ++items[x];
-        }
+      if (started) {
+        if (elect_one()) umma_commit(&o_final[x]);
+        __syncwarp();
+        ++items;
+      }
     }
     if (!ok) *abort_v = 1;
-    if (elect_one()) umma_commit(&mma_done);  // every MMA issued so far has completed when this fires
+    if (elect_one()) umma_commit(&mma_done[x]);  // every MMA issued so far has completed when this fires
     __syncwarp();
-    mbar_wait_warp(&mma_done, 0, kCkWait);
-  } else if (warp < 10) {
+    mbar_wait_warp(&mma_done[x], 0, kCkWait);
+  }
+  } else if (warp < 12) {
+    ck_more_regs<kMore>();
     // ---------------- softmax and output of tile x: one thread per pair ----------------
-    const int x = (warp - 2) >> 2, q4 = warp & 3, row = q4 * 32 + lane;
+    const int x = (warp - 4) >> 2, q4 = warp & 3, row = q4 * 32 + lane;
     const int gs = __ffs(p.a.n_heads / H) - 1;
     const uint32_t lane_addr = tmem + ((uint32_t)(q4 * 32) << 16) + x * 256, o_addr = lane_addr + 128;
     // tensor-memory loads and stores are warp-wide: a wait counts for all lanes or none
-    auto wwait = [&](uint64_t* bar, uint32_t parity) -> bool {
-      const bool mine = !*abort_v && mbar_wait_bounded(bar, parity, kCkWait);
-      return __all_sync(0xffffffffu, mine);
-    };
+    auto wwait = [&](uint64_t* bar, uint32_t parity) -> bool { return ck_wait(bar, parity, abort_v); };
     int sn = 0, pn = 0, items = 0;
     bool ok = true;
     int cb = 0;  // (4 bits) buffer of the next key tile; (16 bits) its stage
@@ -389,11 +413,12 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
     // a warp whose wait gave up goes on without work: the parts' barriers below count every warp
     for (int r = 0, kd; (ok || p.parts > 1) && (kd = ck_work(p, c, r, w, nullptr)) >= 0; ++r) {
       if (kd == 0) continue;
+      const CkSide side(w, x);
       bool any = false;
-      for (int j = w.j0; j < w.j1 && !any && ok; ++j) any = w.need(x, w.tile(j), W, S);
+      for (int j = w.j0; j < w.j1 && !any && ok; ++j) any = side.need(j);
       float m_ref = -INFINITY, l = 0.f, scale = p.a.scale * 1.4426950408889634f;
-      const int pr = w.first[x] + row;
-      const bool live = row < w.count[x];
+      const int pr = side.first + row;
+      const bool live = row < side.count;
       const int pos = w.p0 + (pr >> gs);
       if (any) {
         // ---- the query row into the operand tile. The last part's scores are complete (their
@@ -439,9 +464,9 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
       }
       bool first = true;
       for (int j = w.j0; j < w.j1 && ok; ++j) {
-        const int kt = w.tile(j), k0 = kt * kPageTokens, stage = cb;
+        const int k0 = w.tile(j) * kPageTokens, stage = cb;
         if (++cb == ring) cb = 0;
-        if (!w.need(x, kt, W, S)) continue;
+        if (!side.need(j)) continue;
         const int sb = sn & 1;
         if (!wwait(&s_full[x][sb], (sn >> 1) & 1)) {
           ok = false;
@@ -581,7 +606,7 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
         if (live) *reinterpret_cast<float2*>(pt + D) = make_float2(m_ref, l);
         // the last part of the item merges all, one warp per pair
         named_sync(1, 256);
-        if (tid == 64) {
+        if (tid == 128) {
           __threadfence();
           last_s = atomicAdd(&p.counters[w.item], 1) == p.parts - 1;
           if (last_s) {
@@ -593,7 +618,7 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
         const bool last = last_s;
         if (last) {
           const float* all = p.part + (size_t)w.item * p.parts * 256 * (D + 2);
-          for (int k = warp - 2; k < w.count[0] + w.count[1]; k += 8) {
+          for (int k = warp - 4; k < w.count[0] + w.count[1]; k += 8) {
             auto at = [&](int sp) { return all + ((size_t)sp * 256 + k) * (D + 2); };
             float Mx = -INFINITY;
             for (int sp = 0; sp < p.parts; ++sp) Mx = fmaxf(Mx, __ldcg(at(sp) + D));
@@ -625,9 +650,11 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
       }
     }
     if (!ok) *abort_v = 1;
-  } else if constexpr (Q4) {
+  } else {
+    ck_fewer_regs<kFew>();
+    if constexpr (Q4) {
     // ---------------- 4 bits: codes to f16 operand tiles ----------------
-    const int ct = tid - 320, cw = ct >> 5;
+    const int cw = warp - 12;
     int s = 0, ph = 0, b = 0, round_b = 0;
     bool ok = true;
     const uint32_t f64 = p.f64, k72 = 0x54805480u;  // f16 64, 72
@@ -637,21 +664,20 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
       const int top = w.count[1] > 0 ? w.hi[1] : w.hi[0];
       for (int j = w.j0; j < w.j1; ++j) {
         const int k0 = w.tile(j) * kPageTokens;
-        if (*abort_v || !mbar_wait_warp(&kv_full[s], ph, kCkWait) ||
-            (round_b > 0 && !mbar_wait_warp(&cv_empty[b], (round_b - 1) & 1, kCkWait))) {
+        if (!ck_wait(&kv_full[s], ph, abort_v) ||
+            (round_b > 0 && !ck_wait(&cv_empty[b], (round_b - 1) & 1, abort_v))) {
           ok = false;
           break;
         }
         const uint8_t* src = kvp + s * 2 * BLK;
         uint8_t* dst = cvp + b * 2 * TB;
         const bool bad = bad_s[s];
-        if (ct == 0) cbad_s[b] = bad;
-        // rows of 16 keys per warp; a lane takes chunk lane & 3 of key (lane >> 2)'s place:
-        // keys 4 apart in a quarter-warp, whose swizzled rows share no banks
+        if (tid == 12 * 32) cbad_s[b] = bad;
+        // 8 keys per warp; a lane takes chunk lane & 3 of a key, keys 4 apart in a
+        // quarter-warp, whose swizzled rows share no banks
         if constexpr (NB == 4) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int kk = lane >> 2, key = cw * 16 + i * 8 + (kk & 1) * 4 + (kk >> 1), ch = lane & 3;
+          {
+            const int kk = lane >> 2, key = cw * 8 + (kk & 1) * 4 + (kk >> 1), ch = lane & 3;
             {
               const uint4 u = *reinterpret_cast<const uint4*>(src + key * 64 + ch * 16);
               const uint2 sc = *reinterpret_cast<const uint2*>(src + 4096 + key * 8);
@@ -693,9 +719,8 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
         } else {
           // head_dim 64: 8-byte key chunks of two words, a value row of 8 words
           const int kk = lane >> 2, ch = lane & 3;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int key = cw * 16 + i * 8 + (kk & 1) * 4 + (kk >> 1);
+          {
+            const int key = cw * 8 + (kk & 1) * 4 + (kk >> 1);
             const uint2 u = *reinterpret_cast<const uint2*>(src + key * 32 + ch * 8);
             const uint32_t sc = *reinterpret_cast<const uint32_t*>(src + 2048 + key * 4);
             const uint32_t wd[2] = {u.x, u.y}, d2[2] = {__byte_perm(sc, 0, 0x1010), __byte_perm(sc, 0, 0x3232)};
@@ -737,6 +762,7 @@ __global__ void __launch_bounds__(Q4 ? 448 : 320, 1)
       }
     }
     if (!ok) *abort_v = 1;
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -800,7 +826,7 @@ cudaError_t launch_cache_chunk(bool bf16, const CacheView& c, int layer, const C
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sh.grid);
-    cfg.blockDim = dim3(q4 ? 448 : 320);
+    cfg.blockDim = dim3(ck_threads(q4));
     cfg.dynamicSmemBytes = sh.smem;
     cfg.stream = s;
     cfg.attrs = &attr;
