@@ -196,10 +196,10 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
   constexpr int kMore = Q4 ? 152 : 208, kFew = Q4 ? 56 : 88;
   constexpr float kPScale = Act<M>::kIsBf16 ? 0.f : 7.f;      // log2 factor of P (f16 subnormals start at 2^-14)
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], kv_full[kCkMaxStages], kv_empty[kCkMaxStages], cv_full[2], cv_empty[2],
+  __shared__ __align__(8) uint64_t q_full[2], kv_full[kCkMaxStages], kv_empty[kCkMaxStages], cv_full[2][2], cv_empty[2][2],
       s_full[2][2], s_empty[2][2], p_full[2], pv_done[2], o_final[2], o_empty[2], mma_done[2];
   __shared__ uint32_t tmem_s;
-  __shared__ int abort_s, bad_s[kCkMaxStages], cbad_s[2], last_s;
+  __shared__ int abort_s, bad_s[kCkMaxStages], cbad_s[4], last_s;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -219,18 +219,20 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
       mbar_init(&kv_empty[s], Q4 ? 8 : 2);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&cv_full[x], 8);
-      mbar_init(&cv_empty[x], 2);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&cv_full[x][b], 8);
+        mbar_init(&cv_empty[x][b], 2);
+      }
       mbar_init(&mma_done[x], 1);
-      mbar_init(&q_full[x], 128);
+      mbar_init(&q_full[x], 4);
       for (int s = 0; s < 2; ++s) {
         mbar_init(&s_full[x][s], 1);
-        mbar_init(&s_empty[x][s], 128);
+        mbar_init(&s_empty[x][s], 4);
       }
-      mbar_init(&p_full[x], 128);
+      mbar_init(&p_full[x], 4);
       mbar_init(&pv_done[x], 1);
       mbar_init(&o_final[x], 1);
-      mbar_init(&o_empty[x], 128);
+      mbar_init(&o_empty[x], 4);
     }
     abort_s = 0;
     fence_barrier_init();
@@ -300,9 +302,11 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
     constexpr uint32_t idesc_o = umma_idesc_f16(kBf, 128, D) | (1u << 16);  // B (V) MN-major
     int items = 0, sn = 0, pn = 0;
     int st = 0, ph = 0;  // operand tile of the next key tile: its stage (4 bits: buffer) and phase
+    int prev_ph = 0;
     const int ring = Q4 ? 2 : stages;
-    uint64_t* full = Q4 ? cv_full : kv_full;
-    uint64_t* empty = Q4 ? cv_empty : kv_empty;
+    // 4 bits: keys and values come and go by themselves; keys are free long before values
+    uint64_t* full = Q4 ? cv_full[0] : kv_full;
+    uint64_t* empty = Q4 ? cv_empty[1] : kv_empty;
     uint8_t* tiles = Q4 ? cvp : kvp;
     const uint32_t s_tmem = tmem + x * 256, o_tmem = s_tmem + 128;
     // descriptors of the first operand tiles; addresses below 256 KB never carry out of
@@ -354,9 +358,12 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
                 umma_f16(s_tmem + sb * 64, dq + ((kk >> 2) * 2 * kCkBox + (kk & 3) * 32) / 16,
                          kd + ((kk >> 2) * kCkBox + (kk & 3) * 32) / 16, idesc_s, kk != 0);
               umma_commit(&s_full[x][sb]);
+              if (Q4) umma_commit(&cv_empty[0][st]);
             }
             __syncwarp();
             ++sn;
+          } else if (Q4 && lane == 0) {
+            mbar_arrive(&cv_empty[0][st]);
           }
         }
         if (j > w.j0) {
@@ -364,6 +371,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
             // ---- O += P(j - 1) V
             if (!started && items >= 1 && !(ok = ck_wait(&o_empty[x], (items - 1) & 1, abort_v))) break;
             if (!(ok = ck_wait(&p_full[x], pn & 1, abort_v))) break;
+            if (Q4 && !(ok = ck_wait(&cv_full[1][prev_st], prev_ph, abort_v))) break;
             tc_fence_after();
             const uint64_t vd = dv + (uint64_t)(prev_st * (2 * TB / 16));
             if (elect_one()) {
@@ -376,12 +384,15 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
             __syncwarp();
             started = true;
             ++pn;
-          } else if (lane == 0) {
-            mbar_arrive(&empty[prev_st]);
+          } else {
+            // (4 bits: the buffer is free only once it has been filled)
+            if (Q4 && !(ok = ck_wait(&cv_full[1][prev_st], prev_ph, abort_v))) break;
+            if (lane == 0) mbar_arrive(&empty[prev_st]);
           }
         }
         if (j < w.j1) {
           prev_st = st;
+          prev_ph = ph;
           if (++st == ring) st = 0, ph ^= 1;
         }
       }
@@ -407,8 +418,10 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
     auto wwait = [&](uint64_t* bar, uint32_t parity) -> bool { return ck_wait(bar, parity, abort_v); };
     int sn = 0, pn = 0, items = 0;
     bool ok = true;
-    int cb = 0;  // (4 bits) buffer of the next key tile; (16 bits) its stage
-    const int ring = Q4 ? 2 : stages;
+    // where the next key tile's flag is. 4 bits: key tile j mod 4, written again once S(j + 2) is
+    // done, before which this group's MMA warp has waited for P(j)
+    int cb = 0;
+    const int ring = Q4 ? 4 : stages;
     CkWork w;
     // a warp whose wait gave up goes on without work: the parts' barriers below count every warp
     for (int r = 0, kd; (ok || p.parts > 1) && (kd = ck_work(p, c, r, w, nullptr)) >= 0; ++r) {
@@ -460,7 +473,8 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
         for (int i = 0; i < D / 8; ++i)
           *reinterpret_cast<uint4*>(dst + (i >> 3) * 2 * kCkBox + (((i & 7) ^ (row & 7)) << 4)) = u[i];
         ck_fence_async();
-        mbar_arrive(&q_full[x]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[x]);
       }
       bool first = true;
       for (int j = w.j0; j < w.j1 && ok; ++j) {
@@ -483,7 +497,8 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
           for (int i = 0; i < 32; ++i) s[h2 * 32 + i] = __uint_as_float(v[i]);
         }
         tc_fence_before();
-        mbar_arrive(&s_empty[x][sb]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[x][sb]);
         ++sn;
         const bool bad = Q4 ? cbad_s[stage] : bad_s[stage];
         if (bad || k0 + 63 > pos || (W && k0 <= pos - W && k0 + 63 >= S)) {
@@ -559,7 +574,8 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
         }
         ck_fence_async();
         tc_fence_before();
-        mbar_arrive(&p_full[x]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
         ++pn;
         first = false;
       }
@@ -599,7 +615,8 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
           }
         }
         tc_fence_before();
-        mbar_arrive(&o_empty[x]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[x]);
         ++items;
       }
       if (pt) {
@@ -665,98 +682,81 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
       for (int j = w.j0; j < w.j1; ++j) {
         const int k0 = w.tile(j) * kPageTokens;
         if (!ck_wait(&kv_full[s], ph, abort_v) ||
-            (round_b > 0 && !ck_wait(&cv_empty[b], (round_b - 1) & 1, abort_v))) {
+            (round_b > 0 && !ck_wait(&cv_empty[0][b], (round_b - 1) & 1, abort_v))) {
           ok = false;
           break;
         }
         const uint8_t* src = kvp + s * 2 * BLK;
         uint8_t* dst = cvp + b * 2 * TB;
         const bool bad = bad_s[s];
-        if (tid == 12 * 32) cbad_s[b] = bad;
+        if (tid == 12 * 32) cbad_s[(round_b * 2 + b) & 3] = bad;
         // 8 keys per warp; a lane takes chunk lane & 3 of a key, keys 4 apart in a
         // quarter-warp, whose swizzled rows share no banks
-        if constexpr (NB == 4) {
-          {
-            const int kk = lane >> 2, key = cw * 8 + (kk & 1) * 4 + (kk >> 1), ch = lane & 3;
-            {
-              const uint4 u = *reinterpret_cast<const uint4*>(src + key * 64 + ch * 16);
-              const uint2 sc = *reinterpret_cast<const uint2*>(src + 4096 + key * 8);
-              const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
-              const uint32_t d2[4] = {__byte_perm(sc.x, 0, 0x1010), __byte_perm(sc.x, 0, 0x3232),
-                                      __byte_perm(sc.y, 0, 0x1010), __byte_perm(sc.y, 0, 0x3232)};
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                uint4 o;
-                o.x = ck_sub_mul(((wd[g] << 4) & 0x00f000f0u) | f64, k72, d2[g]);
-                o.y = ck_sub_mul((wd[g] & 0x00f000f0u) | f64, k72, d2[g]);
-                o.z = ck_sub_mul(((wd[g] >> 4) & 0x00f000f0u) | f64, k72, d2[g]);
-                o.w = ck_sub_mul(((wd[g] >> 8) & 0x00f000f0u) | f64, k72, d2[g]);
-                const int oc = 4 * g + ch;
-                *reinterpret_cast<uint4*>(dst + (oc >> 3) * kCkBox + key * 128 + (((oc & 7) ^ (key & 7)) << 4)) = o;
-              }
-            }
-            {
-              const uint4 u = *reinterpret_cast<const uint4*>(src + BLK + key * 64 + ch * 16);
-              uint32_t d2 = *reinterpret_cast<const uint16_t*>(src + BLK + 4096 + key * 8 + ch * 2);
-              const int kp = k0 + key;
-              const bool hide = bad || kp > top || (W && kp <= w.lo[0] - W && kp >= S);
-              d2 = hide ? 0u : d2 | d2 << 16;
-              const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                // nibbles 2 i, 2 i + 1 side by side: bytes of the even and the odd ones interleaved
-                const uint32_t ev = (wd[g] << 4) & 0xf0f0f0f0u, od = wd[g] & 0xf0f0f0f0u;
-                uint4 o;
-                o.x = ck_sub_mul((__byte_perm(ev, od, 0x0400) & 0x00ff00ffu) | f64, k72, d2);
-                o.y = ck_sub_mul((__byte_perm(ev, od, 0x0501) & 0x00ff00ffu) | f64, k72, d2);
-                o.z = ck_sub_mul((__byte_perm(ev, od, 0x0602) & 0x00ff00ffu) | f64, k72, d2);
-                o.w = ck_sub_mul((__byte_perm(ev, od, 0x0703) & 0x00ff00ffu) | f64, k72, d2);
-                const int oc = 4 * ch + g;
-                *reinterpret_cast<uint4*>(dst + TB + (oc >> 3) * kCkBox + key * 128 + (((oc & 7) ^ (key & 7)) << 4)) = o;
-              }
-            }
-          }
-        } else {
-          // head_dim 64: 8-byte key chunks of two words, a value row of 8 words
-          const int kk = lane >> 2, ch = lane & 3;
-          {
-            const int key = cw * 8 + (kk & 1) * 4 + (kk >> 1);
+        const int kk = lane >> 2, key = cw * 8 + (kk & 1) * 4 + (kk >> 1), ch = lane & 3;
+        constexpr int CB = 64 * D / 2;  // code bytes of a block
+        {
+          // a key chunk: word g holds dims 32 g + 8 ch .. + 7
+          uint32_t wd[NB], d2[NB];
+          if constexpr (NB == 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(src + key * 64 + ch * 16);
+            const uint2 sc = *reinterpret_cast<const uint2*>(src + CB + key * 8);
+            wd[0] = u.x, wd[1] = u.y, wd[2] = u.z, wd[3] = u.w;
+            d2[0] = __byte_perm(sc.x, 0, 0x1010), d2[1] = __byte_perm(sc.x, 0, 0x3232);
+            d2[2] = __byte_perm(sc.y, 0, 0x1010), d2[3] = __byte_perm(sc.y, 0, 0x3232);
+          } else {
             const uint2 u = *reinterpret_cast<const uint2*>(src + key * 32 + ch * 8);
-            const uint32_t sc = *reinterpret_cast<const uint32_t*>(src + 2048 + key * 4);
-            const uint32_t wd[2] = {u.x, u.y}, d2[2] = {__byte_perm(sc, 0, 0x1010), __byte_perm(sc, 0, 0x3232)};
+            const uint32_t sc = *reinterpret_cast<const uint32_t*>(src + CB + key * 4);
+            wd[0] = u.x, wd[1] = u.y;
+            d2[0] = __byte_perm(sc, 0, 0x1010), d2[1] = __byte_perm(sc, 0, 0x3232);
+          }
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              uint4 o;
-              o.x = ck_sub_mul(((wd[g] << 4) & 0x00f000f0u) | f64, k72, d2[g]);
-              o.y = ck_sub_mul((wd[g] & 0x00f000f0u) | f64, k72, d2[g]);
-              o.z = ck_sub_mul(((wd[g] >> 4) & 0x00f000f0u) | f64, k72, d2[g]);
-              o.w = ck_sub_mul(((wd[g] >> 8) & 0x00f000f0u) | f64, k72, d2[g]);
-              *reinterpret_cast<uint4*>(dst + key * 128 + (((4 * g + ch) ^ (key & 7)) << 4)) = o;
-            }
-            const uint2 v = *reinterpret_cast<const uint2*>(src + BLK + key * 32 + ch * 8);
-            uint32_t dv = *reinterpret_cast<const uint16_t*>(src + BLK + 2048 + key * 4 + (ch >> 1) * 2);
-            const int kp = k0 + key;
-            const bool hide = bad || kp > top || (W && kp <= w.lo[0] - W && kp >= S);
-            dv = hide ? 0u : dv | dv << 16;
-            const uint32_t vd[2] = {v.x, v.y};
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const uint32_t ev = (vd[g] << 4) & 0xf0f0f0f0u, od = vd[g] & 0xf0f0f0f0u;
-              uint4 o;
-              o.x = ck_sub_mul((__byte_perm(ev, od, 0x0400) & 0x00ff00ffu) | f64, k72, dv);
-              o.y = ck_sub_mul((__byte_perm(ev, od, 0x0501) & 0x00ff00ffu) | f64, k72, dv);
-              o.z = ck_sub_mul((__byte_perm(ev, od, 0x0602) & 0x00ff00ffu) | f64, k72, dv);
-              o.w = ck_sub_mul((__byte_perm(ev, od, 0x0703) & 0x00ff00ffu) | f64, k72, dv);
-              *reinterpret_cast<uint4*>(dst + TB + key * 128 + (((2 * ch + g) ^ (key & 7)) << 4)) = o;
-            }
+          for (int g = 0; g < NB; ++g) {
+            uint4 o;
+            o.x = ck_sub_mul(((wd[g] << 4) & 0x00f000f0u) | f64, k72, d2[g]);
+            o.y = ck_sub_mul((wd[g] & 0x00f000f0u) | f64, k72, d2[g]);
+            o.z = ck_sub_mul(((wd[g] >> 4) & 0x00f000f0u) | f64, k72, d2[g]);
+            o.w = ck_sub_mul(((wd[g] >> 8) & 0x00f000f0u) | f64, k72, d2[g]);
+            const int oc = 4 * g + ch;
+            *reinterpret_cast<uint4*>(dst + (oc >> 3) * kCkBox + key * 128 + (((oc & 7) ^ (key & 7)) << 4)) = o;
           }
         }
         ck_fence_async();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&cv_full[b]);
-          mbar_arrive(&kv_empty[s]);
+        if (lane == 0) mbar_arrive(&cv_full[0][b]);
+        // a value chunk: its words are dims in order
+        uint32_t wd[NB];
+        if constexpr (NB == 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src + BLK + key * 64 + ch * 16);
+          wd[0] = u.x, wd[1] = u.y, wd[2] = u.z, wd[3] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(src + BLK + key * 32 + ch * 8);
+          wd[0] = u.x, wd[1] = u.y;
         }
+        uint32_t dv = *reinterpret_cast<const uint16_t*>(src + BLK + CB + key * NB * 2 + (NB == 4 ? ch : ch >> 1) * 2);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_empty[s]);  // this warp has read its part of the stage
+        const int kp = k0 + key;
+        const bool hide = bad || kp > top || (W && kp <= w.lo[0] - W && kp >= S);
+        dv = hide ? 0u : dv | dv << 16;
+        if (round_b > 0 && !ck_wait(&cv_empty[1][b], (round_b - 1) & 1, abort_v)) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int g = 0; g < NB; ++g) {
+          // nibbles 2 i, 2 i + 1 side by side: bytes of the even and the odd ones interleaved
+          const uint32_t ev = (wd[g] << 4) & 0xf0f0f0f0u, od = wd[g] & 0xf0f0f0f0u;
+          uint4 o;
+          o.x = ck_sub_mul((__byte_perm(ev, od, 0x0400) & 0x00ff00ffu) | f64, k72, dv);
+          o.y = ck_sub_mul((__byte_perm(ev, od, 0x0501) & 0x00ff00ffu) | f64, k72, dv);
+          o.z = ck_sub_mul((__byte_perm(ev, od, 0x0602) & 0x00ff00ffu) | f64, k72, dv);
+          o.w = ck_sub_mul((__byte_perm(ev, od, 0x0703) & 0x00ff00ffu) | f64, k72, dv);
+          const int oc = NB * ch + g;
+          *reinterpret_cast<uint4*>(dst + TB + (oc >> 3) * kCkBox + key * 128 + (((oc & 7) ^ (key & 7)) << 4)) = o;
+        }
+        ck_fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&cv_full[1][b]);
         if (++s == stages) s = 0, ph ^= 1;
         if (++b == 2) b = 0, ++round_b;
       }
