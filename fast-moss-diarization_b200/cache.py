@@ -30,6 +30,12 @@ PAGE = 64
 _FORMATS = {"f16": _lib.CACHE_F16, "bf16": _lib.CACHE_BF16, "q4": _lib.CACHE_Q4}
 
 
+def _raw_stream(index: int) -> int:
+    import torch
+
+    return torch.cuda.current_stream(index).cuda_stream
+
+
 def _fail(message: str, status: int = _lib.FMD_EINVAL):
     raise _lib.FmdError(status, message)
 
@@ -52,10 +58,6 @@ class CacheRows:
         must be there: `PagedCache.reserve`)."""
         self.pos0.add_(n)
 
-    def to_c(self) -> _lib.CacheRows:
-        return _lib.CacheRows(self.slot.data_ptr(), self.pos0.data_ptr(),
-                              None if self.row0 is None else self.row0.data_ptr(), self.slot.shape[0], self.n_rows,
-                              self.max_rows, 0)
 
 
 class PagedCache:
@@ -100,7 +102,12 @@ class PagedCache:
         self.pool, self.page_table = pool, page_table
         self._c = _lib.Cache(pool.data_ptr(), page_table.data_ptr(), self.format, layers, n_pages, kv_heads, head_dim,
                              max_slots, max_pages_per_slot, 0)
+        self._ref = C.byref(self._c)
+        self._index = pool.get_device()
+        self._dtypes = ({torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16} if kind == "q4" else
+                        {{"f16": torch.float16, "bf16": torch.bfloat16}[kind]: self.format})
         self._status = torch.zeros(2, dtype=torch.int32, device=self.device)
+        self._status_at = self._status.data_ptr()
         self._workspaces: dict = {}
         # bookkeeping: pages of each open slot (-1: evicted), its length, names of each page
         self._pages: list = [None] * max_slots
@@ -264,8 +271,11 @@ class PagedCache:
     def _call(self, fn, *args) -> None:
         import torch
 
-        with torch.cuda.device(self.device):
-            st = fn(C.byref(self._c), *args, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        if torch.cuda.current_device() == self._index:
+            st = fn(self._ref, *args, _raw_stream(self._index))
+        else:
+            with torch.cuda.device(self._index):
+                st = fn(self._ref, *args, _raw_stream(self._index))
         if st != _lib.FMD_OK:
             raise _lib.FmdError(st, f"{fn.__name__}: {self.lib.fmd_status_string(st).decode()}")
 
@@ -277,35 +287,39 @@ class PagedCache:
             raise _lib.FmdError(st, "a slot, position or page was out of range")
 
     def _dtype(self, t, name: str) -> int:
-        import torch
-
-        codes = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
-        if t.dtype not in codes or (self.kind != "q4" and codes[t.dtype] != self.format):
+        code = self._dtypes.get(t.dtype)
+        if code is None:
             _fail(f"{name} must be {'float16 or bfloat16' if self.kind == 'q4' else self.kind}, not {t.dtype}")
-        return codes[t.dtype]
+        return code
 
-    def _heads(self, t, name: str, heads: int, like=None) -> tuple:
-        """(row stride, head stride) of a [rows, heads, head_dim] tensor."""
-        if t.dim() != 3 or t.shape[2] != self.head_dim or (heads and t.shape[1] != heads):
-            _fail(f"{name} must be [rows, {heads or 'heads'}, {self.head_dim}], not {tuple(t.shape)}")
-        if t.device != self.device:
+    def _heads(self, t, name: str, heads: int, rows: int, dtype) -> tuple:
+        """(address, row stride, head stride) of a [rows, heads, head_dim] tensor."""
+        shape = t.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads and shape[1] != heads):
+            _fail(f"{name} must be [rows, {heads or 'heads'}, {self.head_dim}], not {tuple(shape)}")
+        if t.get_device() != self._index:
             _fail(f"{name} must be on {self.device}")
-        if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0]):
+        if shape[0] != rows or t.dtype != dtype:
             _fail(f"{name} must have the rows and dtype of the others")
         row, head, dim = t.stride()
-        row, head = (0 if t.shape[0] <= 1 else row), (0 if t.shape[1] <= 1 else head)
-        if t.numel() and (dim != 1 or row % 8 or head % 8 or row < 0 or head < 0 or t.data_ptr() % 16):
+        if rows <= 1:
+            row = 0
+        if shape[1] <= 1:
+            head = 0
+        at = t.data_ptr()
+        if (dim != 1 or (row | head) & 7 or at & 15) and t.numel():
             _fail(f"{name}: heads must be contiguous, 16-byte aligned, with strides of multiples of 8 elements")
-        return row, head
+        return at, row, head
 
-    def _rows_c(self, rows: CacheRows, n: int) -> _lib.CacheRows:
-        c = rows.to_c()
+    def _rows_c(self, rows: CacheRows, n: int):
+        slot, row0 = rows.slot, rows.row0
         if rows.n_rows > n:
             _fail(f"the rows need {rows.n_rows} rows of the tensors, not {n}")
-        if rows.row0 is None and n < rows.slot.shape[0]:
-            _fail(f"{rows.slot.shape[0]} sequences need a row each, not {n}")
-        c.n_rows = n
-        return c
+        seqs = slot.shape[0]
+        if row0 is None and n < seqs:
+            _fail(f"{seqs} sequences need a row each, not {n}")
+        return C.byref(_lib.CacheRows(slot.data_ptr(), rows.pos0.data_ptr(), None if row0 is None else row0.data_ptr(),
+                                      seqs, n, rows.max_rows, 0))
 
     def append(self, layer: int, rows: CacheRows, k, v, q=None, q_norm=None, k_norm=None, eps: float = 1e-6, cos=None,
                sin=None, interleaved: bool = False, q_out=None):
@@ -316,42 +330,50 @@ class PagedCache:
         `interleaved`) applied to queries and keys in the same pass. Returns the
         normed and rotated queries (`q_out`, which may be `q`), or None without
         `q`. f32 arithmetic, one rounding per value."""
-        import torch
-
         if not 0 <= layer < self.layers:
             _fail(f"layer {layer} is out of range")
-        a = _lib.CacheAppendArgs(k=k.data_ptr(), v=v.data_ptr(), eps=eps, dtype=self._dtype(k, "k"),
-                                 interleaved=bool(interleaved))
-        a.k_row, a.k_head = self._heads(k, "k", self.kv_heads)
-        a.v_row, a.v_head = self._heads(v, "v", self.kv_heads, k)
+        code, dtype, n = self._dtype(k, "k"), k.dtype, k.shape[0]
+        k_at, k_row, k_head = self._heads(k, "k", self.kv_heads, n, dtype)
+        v_at, v_row, v_head = self._heads(v, "v", self.kv_heads, n, dtype)
+        q_at = o_at = qn_at = kn_at = cos_at = sin_at = None
+        q_row = q_head = o_row = o_head = heads = rot = table = 0
         if q is not None:
-            a.q_row, a.q_head = self._heads(q, "q", 0, k)
+            q_at, q_row, q_head = self._heads(q, "q", 0, n, dtype)
+            heads = q.shape[1]
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            a.q_out_row, a.q_out_head = self._heads(q_out, "q_out", q.shape[1], q)
-            a.q, a.q_out, a.n_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+                q_out = q.new_empty(q.shape)
+            o_at, o_row, o_head = self._heads(q_out, "q_out", heads, n, dtype)
         elif q_out is not None or q_norm is not None:
             _fail("q_out and q_norm need q")
-        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if w is not None:
-                if (w.dtype != k.dtype or tuple(w.shape) != (self.head_dim,) or not w.is_contiguous()
-                        or w.device != self.device or w.data_ptr() % 16):
-                    _fail(f"{name} must be an aligned contiguous [{self.head_dim}] tensor of the rows' dtype")
-                setattr(a, name, w.data_ptr())
+        if q_norm is not None:
+            qn_at = self._weight(q_norm, "q_norm", dtype)
+        if k_norm is not None:
+            kn_at = self._weight(k_norm, "k_norm", dtype)
         if (cos is None) != (sin is None):
             _fail("cos and sin go together")
         if cos is not None:
+            import torch
+
+            shape = cos.shape
             for t in (cos, sin):
-                if (t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or not t.is_contiguous()
-                        or t.device != self.device or t.data_ptr() % 16):
+                if (t.dtype != torch.float32 or len(shape) != 2 or t.shape != shape or not t.is_contiguous()
+                        or t.get_device() != self._index or t.data_ptr() & 15):
                     _fail("cos and sin must be aligned contiguous f32 tables [positions, pairs]")
-            if cos.shape[0] < 1 or cos.shape[1] % 4 or not 0 < cos.shape[1] <= self.head_dim // 2:
+            table, pairs = shape
+            rot = 2 * pairs
+            if table < 1 or pairs % 4 or not 0 < rot <= self.head_dim:
                 _fail("the rotated dims must be a multiple of 8, at most head_dim")
-            a.cos_table, a.sin_table = cos.data_ptr(), sin.data_ptr()
-            a.rot_dim, a.table_rows = 2 * cos.shape[1], cos.shape[0]
-        self._call(self.lib.fmd_cache_append, layer, C.byref(self._rows_c(rows, k.shape[0])), C.byref(a),
-                   C.c_void_p(self._status.data_ptr()))
+            cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+        args = _lib.CacheAppendArgs(k_at, v_at, q_at, o_at, k_row, k_head, v_row, v_head, q_row, q_head, o_row, o_head,
+                                    qn_at, kn_at, cos_at, sin_at, eps, code, heads, rot, table, bool(interleaved))
+        self._call(self.lib.fmd_cache_append, layer, self._rows_c(rows, n), C.byref(args), self._status_at)
         return q_out
+
+    def _weight(self, w, name: str, dtype) -> int:
+        if (w.dtype != dtype or w.dim() != 1 or w.shape[0] != self.head_dim or w.stride(0) != 1
+                or w.get_device() != self._index or w.data_ptr() & 15):
+            _fail(f"{name} must be an aligned contiguous [{self.head_dim}] tensor of the rows' dtype")
+        return w.data_ptr()
 
     def read(self, layer: int, rows: CacheRows, k_out=None, v_out=None, n_rows: int | None = None):
         """The cached keys and values of the rows' positions, f32
@@ -371,8 +393,8 @@ class PagedCache:
             if (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != self.device
                     or t.data_ptr() % 16):
                 _fail(f"outputs must be aligned contiguous f32 tensors {shape}")
-        self._call(self.lib.fmd_cache_read, layer, C.byref(self._rows_c(rows, n_rows)), C.c_void_p(k_out.data_ptr()),
-                   C.c_void_p(v_out.data_ptr()), C.c_void_p(self._status.data_ptr()))
+        self._call(self.lib.fmd_cache_read, layer, self._rows_c(rows, n_rows), k_out.data_ptr(), v_out.data_ptr(),
+                   self._status_at)
         return k_out, v_out
 
     def workspace(self, n_heads: int, n_seqs: int, max_rows: int = 1):
@@ -394,13 +416,13 @@ class PagedCache:
     def _workspace(self, n_heads: int, rows: CacheRows):
         import torch
 
-        n = int(self.lib.fmd_cache_attend_workspace(C.byref(self._c), n_heads, rows.slot.shape[0], rows.max_rows))
+        n = self.lib.fmd_cache_attend_workspace(self._ref, n_heads, rows.slot.shape[0], rows.max_rows)
         if n == 0:
             return None
         if torch.cuda.is_current_stream_capturing():
             # a graph's own: graphs replayed at the same time must not share one
             return self._fresh_workspace(n)
-        key = torch.cuda.current_stream(self.device).cuda_stream
+        key = _raw_stream(self._index)
         w = self._workspaces.get(key)
         if w is None or w.numel() < n:
             w = self._workspaces[key] = self._fresh_workspace(n)
@@ -413,29 +435,27 @@ class PagedCache:
         with `window` > 0 those with j > p - window or j < sinks. `scale` defaults
         to head_dim ** -0.5. Returns `out` (rows of padding and behind the last
         sequence are left as they were)."""
-        import torch
-
         if not 0 <= layer < self.layers:
             _fail(f"layer {layer} is out of range")
-        if window < 0 or sinks < 0 or window > 2**31 - 1 or sinks > 2**31 - 1:
+        if not 0 <= window < 2**31 or not 0 <= sinks < 2**31:
             _fail("window and sinks must be >= 0")
-        a = _lib.CacheAttendArgs(q=q.data_ptr(), dtype=self._dtype(q, "q"), window=window, sinks=sinks,
-                                 scale=self.head_dim ** -0.5 if scale is None else scale)
-        a.q_row, a.q_head = self._heads(q, "q", 0)
-        a.n_heads = q.shape[1]
-        if a.n_heads % self.kv_heads or a.n_heads // self.kv_heads not in (1, 2, 4, 8, 16):
-            _fail(f"heads must be {self.kv_heads} x 1, 2, 4, 8 or 16, not {a.n_heads}", _lib.FMD_ENOTSUP)
+        code, n = self._dtype(q, "q"), q.shape[0]
+        q_at, q_row, q_head = self._heads(q, "q", 0, n, q.dtype)
+        heads = q.shape[1]
+        if heads % self.kv_heads or heads // self.kv_heads not in (1, 2, 4, 8, 16):
+            _fail(f"heads must be {self.kv_heads} x 1, 2, 4, 8 or 16, not {heads}", _lib.FMD_ENOTSUP)
         if out is None:
-            out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        a.out_row, a.out_head = self._heads(out, "out", q.shape[1], q)
-        a.out = out.data_ptr()
+            out = q.new_zeros(q.shape)
+        o_at, o_row, o_head = self._heads(out, "out", heads, n, q.dtype)
+        rows_c = self._rows_c(rows, n)
         if workspace is None:
-            workspace = self._workspace(a.n_heads, rows)
-        elif workspace.dtype != torch.uint8 or workspace.device != self.device or not workspace.is_contiguous():
+            workspace = self._workspace(heads, rows)
+        elif workspace.dtype.itemsize != 1 or workspace.device != self.device or not workspace.is_contiguous():
             _fail("workspace must be a contiguous uint8 tensor of this device (PagedCache.workspace)")
         ws, nb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
-        self._call(self.lib.fmd_cache_attend, layer, C.byref(self._rows_c(rows, q.shape[0])), C.byref(a),
-                   C.c_void_p(ws), nb, C.c_void_p(self._status.data_ptr()))
+        args = _lib.CacheAttendArgs(q_at, o_at, q_row, q_head, o_row, o_head,
+                                    self.head_dim ** -0.5 if scale is None else scale, code, heads, window, sinks)
+        self._call(self.lib.fmd_cache_attend, layer, rows_c, C.byref(args), ws, nb, self._status_at)
         return out
 
     # -- pages ----------------------------------------------------------------------------
@@ -478,7 +498,7 @@ class PagedCache:
         m = len(dsts)
         ia = C.c_int32 * m
         self._call(self.lib.fmd_cache_fork, m, ia(*[src] * m), ia(*dsts), ia(*[n] * m), ia(*fresh),
-                   C.c_void_p(self._status.data_ptr()))
+                   self._status_at)
 
     def evict(self, slot: int, window: int, sinks: int = 0) -> int:
         """Free the slot's pages that no later row sees with this window and

@@ -1,6 +1,7 @@
 // The paged cache's row and page operators (include/fmd_cache.h): append, read,
 // fork, copy and compact.
 #include <algorithm>
+#include <climits>
 #include <cstring>
 
 #include "fmd_cache.cuh"
@@ -9,181 +10,253 @@ namespace fmd {
 
 namespace {
 
+// ---- rows ---------------------------------------------------------------------------
+//
+// append and read are bound by the bytes they move. A block takes one row (or a
+// part of its heads); L = D / 8 lanes take a head, 8 dims (16 bytes) each, so that
+// every access is a full sector; each lane has two heads' loads in flight before
+// it looks up the row's sequence, position and page, which they do not need.
+
+constexpr int kRowThreads = 256;
+
+// Row `row`'s position, slot and page (-1 where the row takes no part). POS_ONLY
+// leaves the page out.
+struct CacheRow {
+  int slot, pos, page;
+};
+FMD_DEV bool cache_row(const CacheView& c, const CacheRows& r, int row, CacheRow& o, int* status) {
+  const int n_seqs = r.count();
+  int lo = row;
+  if (r.row0) {
+    int hi = n_seqs - 1;  // the last sequence that starts at or before the row
+    lo = 0;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (r.row0[mid] <= row) lo = mid;
+      else hi = mid - 1;
+    }
+  }
+  if (lo >= n_seqs) return false;
+  int p0, r0, n;
+  r.get(lo, o.slot, p0, r0, n);
+  if (row < r0 || row >= r0 + n || !cache_slot_ok(c, o.slot, status)) return false;
+  // p0 near the largest integer must not wrap into the table
+  o.pos = p0 <= INT_MAX - (row - r0) ? p0 + (row - r0) : -1;
+  o.page = cache_page(c, o.slot, o.pos, status);
+  return o.page >= 0;
+}
+
+template <typename T> FMD_DEV void unpack8(uint4 u, float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Act<T>::unpack2(w[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
+// The 4-bit code words and scale of a head: lane l of its L lanes holds dims
+// 8 l .. 8 l + 7. The code is the exact floor(-8 x / m + 8.5): an estimate's
+// nearest integer B is decided by the sign of (8.5 - B) m - 8 x, one fused
+// multiply-add, instead of an IEEE division per value.
+template <int L> FMD_DEV uint32_t quantise8(const float (&x)[8], int l, bool key, __half* scale) {
+  const int lane = threadIdx.x & 31;
+  float a = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    a = fmaxf(a, fabsf(x[i]));
+    bad |= !(fabsf(x[i]) <= 3.4028234e38f);
+  }
+  float amax = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  float first = 0.f;  // this lane's first value of that magnitude
+#pragma unroll
+  for (int i = 7; i >= 0; --i)
+    if (fabsf(x[i]) == amax) first = x[i];
+  const uint32_t mates = 0xfu << (lane & ~3);
+  const uint32_t has = __ballot_sync(0xffffffffu, a == amax) & mates;
+  const bool any_bad = (__ballot_sync(0xffffffffu, bad) & mates) != 0;
+  const float m = __shfl_sync(0xffffffffu, first, has ? __ffs(has) - 1 : lane);
+  const float mag = fminf(fabsf(m), 65504.f), r = mag > 0.f ? -8.f / mag : 0.f;
+  uint32_t word = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float y = m < 0.f ? -x[e] : x[e];
+    const float t = fmaf(y, r, 8.5f), B = rintf(t);
+    float code = fmaf(8.5f - B, mag, -8.f * y) >= 0.f ? B : B - 1.f;
+    code = mag > 0.f ? fminf(fmaxf(code, 0.f), 15.f) : 8.f;
+    word |= (uint32_t)code << (4 * (key ? (e >> 1) + 4 * (e & 1) : e));
+  }
+  if ((l & 3) == 0)
+    *scale = any_bad ? __ushort_as_half(0x7fff) : __float2half_rn((m < 0.f ? mag : -mag) * 0.125f);
+  return word;
+}
+
 // ---- append -------------------------------------------------------------------------
 //
-// One warp per (row, head); lane l holds dims V l .. V l + V - 1, V = D / 32.
+// x * rsqrt(mean(x^2) + eps) * w, then (a, b) -> (a cos - b sin, b cos + a sin):
+// about 10 flop a byte at most, far below the memory's.
 template <typename T, int D, bool Q4>
-__global__ void __launch_bounds__(256) k_cache_append(CacheView c, int layer, CacheRows r, CacheAppend a, int* status) {
-  constexpr int V = D / 32;
-  const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kRowThreads)
+    k_cache_append(CacheView c, int layer, CacheRows r, CacheAppend a, int blocks, int* status) {
+  constexpr int L = D / 8, GROUPS = kRowThreads / L, HPG = 2;
+  griddep_wait();
+  griddep_launch();
+  const int row = blockIdx.x / blocks, part = blockIdx.x % blocks;
+  const int l = threadIdx.x % L, grp = threadIdx.x / L;
   const int heads = a.n_heads + 2 * c.kv_heads;
   const int n_seqs = r.count();
-  const int n_rows = r.row0 ? min(r.row0[n_seqs], r.n_rows) : min(n_seqs, r.n_rows);
-  const long long works = (long long)n_rows * heads;
-  for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < works; w += (long long)gridDim.x * 8) {
-    const int row = (int)(w / heads);
-    int head = (int)(w % heads);
-    int lo = 0;
-    if (r.row0) {
-      int hi = n_seqs - 1;  // the last sequence that starts at or before the row
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (r.row0[mid] <= row) lo = mid;
-        else hi = mid - 1;
-      }
-    } else {
-      lo = row;
+  if (row >= (r.row0 ? min(r.row0[n_seqs], r.n_rows) : min(n_seqs, r.n_rows))) return;
+  const int half = a.rot_dim / 2;
+  bool known = false;
+  CacheRow w{};
+  float cs[8], sn[8];
+  for (int h0 = part * GROUPS * HPG; h0 < heads; h0 += blocks * GROUPS * HPG) {
+    uint4 raw[HPG];
+#pragma unroll
+    for (int k = 0; k < HPG; ++k) {
+      const int h = h0 + k * GROUPS + grp;
+      if (h >= heads) continue;
+      const T* src = h < a.n_heads ? (const T*)a.q + row * a.q_row + h * a.q_head
+                     : h < a.n_heads + c.kv_heads
+                         ? (const T*)a.k + row * a.k_row + (h - a.n_heads) * a.k_head
+                         : (const T*)a.v + row * a.v_row + (h - a.n_heads - c.kv_heads) * a.v_head;
+      raw[k] = *reinterpret_cast<const uint4*>(src + l * 8);
     }
-    int slot, p0, r0, n;
-    r.get(lo, slot, p0, r0, n);
-    if (row < r0 || row >= r0 + n || !cache_slot_ok(c, slot, status)) continue;
-    const int pos = p0 + row - r0;
-    const int page = cache_page(c, slot, pos, status);
-    if (page < 0) continue;
-    if (a.rot_dim > 0 && pos >= a.table_rows) {
-      cache_report(status, FMD_EOVERFLOW);
-      continue;
-    }
-    const int part = head < a.n_heads ? 0 : head < a.n_heads + c.kv_heads ? 1 : 2;
-    if (part) head = (head - a.n_heads) % c.kv_heads;
-    const T* src = part == 0   ? (const T*)a.q + row * a.q_row + head * a.q_head
-                   : part == 1 ? (const T*)a.k + row * a.k_row + head * a.k_head
-                               : (const T*)a.v + row * a.v_row + head * a.v_head;
-    float x[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = Act<T>::to_f(src[lane * V + i]);
-    const T* nw = (const T*)(part == 0 ? a.q_norm : part == 1 ? a.k_norm : nullptr);
-    if (nw) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) ss = fmaf(x[i], x[i], ss);
-      const float rs = rsqrtf(warp_sum(ss) / D + a.eps);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[i] = x[i] * rs * Act<T>::to_f(nw[lane * V + i]);
-    }
-    if (part < 2 && a.rot_dim > 0) {
-      const float* cs = a.cos + (size_t)pos * (a.rot_dim / 2);
-      const float* sn = a.sin + (size_t)pos * (a.rot_dim / 2);
-      const int half = a.rot_dim / 2;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int d = lane * V + i;
-        // the other half's element: rot_dim is a multiple of 8, so it sits at the same i
-        const int other = a.interleaved ? lane : (d < half ? lane + half / V : lane - half / V);
-        const float y = __shfl_sync(0xffffffffu, x[i], other & 31);
-        if (d < a.rot_dim && !a.interleaved) {
-          const int f = d < half ? d : d - half;
-          x[i] = d < half ? x[i] * cs[f] - y * sn[f] : x[i] * cs[f] + y * sn[f];
+    if (!known) {
+      known = true;
+      if (!cache_row(c, r, row, w, status)) return;  // the same for the whole block
+      if (a.rot_dim > 0) {
+        if (w.pos >= a.table_rows) {
+          cache_report(status, FMD_EOVERFLOW);
+          return;
         }
-      }
-      if (a.interleaved) {
+        const float* ct = a.cos + (size_t)w.pos * half;
+        const float* st = a.sin + (size_t)w.pos * half;
+        // this lane's factors: of dims 8 l + i (halves), or of pairs 4 l + i / 2
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-          const int d = lane * V + i;
-          if (d < a.rot_dim) {
-            const float c0 = cs[d / 2], s0 = sn[d / 2], u = x[i], w0 = x[i + 1];
-            x[i] = u * c0 - w0 * s0;
-            x[i + 1] = w0 * c0 + u * s0;
+        for (int q4 = 0; q4 < 2; ++q4) {
+          const int d = l * 8 + q4 * 4;
+          if (d >= a.rot_dim) continue;
+          if (!a.interleaved) {
+            const int f = d < half ? d : d - half;  // half is a multiple of 4
+            const float4 cv = *reinterpret_cast<const float4*>(ct + f), sv = *reinterpret_cast<const float4*>(st + f);
+            cs[4 * q4] = cv.x, cs[4 * q4 + 1] = cv.y, cs[4 * q4 + 2] = cv.z, cs[4 * q4 + 3] = cv.w;
+            sn[4 * q4] = sv.x, sn[4 * q4 + 1] = sv.y, sn[4 * q4 + 2] = sv.z, sn[4 * q4 + 3] = sv.w;
+          } else {
+            const float2 cv = *reinterpret_cast<const float2*>(ct + d / 2),
+                         sv = *reinterpret_cast<const float2*>(st + d / 2);
+            cs[4 * q4] = cs[4 * q4 + 1] = cv.x, cs[4 * q4 + 2] = cs[4 * q4 + 3] = cv.y;
+            sn[4 * q4] = sn[4 * q4 + 1] = sv.x, sn[4 * q4 + 2] = sn[4 * q4 + 3] = sv.y;
           }
         }
       }
     }
-    if (part == 0 || !Q4) {
-      T* dst = part == 0 ? (T*)a.q_out + row * a.qo_row + head * a.qo_head
-                         : (T*)c.block(layer, page, part - 1, head) + (size_t)(pos % kPageTokens) * D;
 #pragma unroll
-      for (int i = 0; i < V; ++i) dst[lane * V + i] = Act<T>::from_f(x[i]);
-    } else {
-      // the first value of largest magnitude of the lane's 32-dim block
-      float m = 0.f;
-      int at = 1 << 20;
-      bool bad = false;
+    for (int k = 0; k < HPG; ++k) {
+      int h = h0 + k * GROUPS + grp;
+      const bool live = h < heads;  // the lanes of a warp stay together for the shuffles
+      const int kind = h < a.n_heads ? 0 : h < a.n_heads + c.kv_heads ? 1 : 2;
+      if (kind) h = (h - a.n_heads) % c.kv_heads;
+      if (!__any_sync(0xffffffffu, live)) continue;
+      float x[8];
+      unpack8<T>(raw[k], x);
+      const T* nw = (const T*)(kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr);
+      float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        bad |= !(fabsf(x[i]) <= 3.4e38f);
-        if (fabsf(x[i]) > fabsf(m)) m = x[i], at = lane * V + i;
+      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (live && nw) {
+        const float rs = rsqrtf(ss / D + a.eps);
+        float wv[8];
+        unpack8<T>(*reinterpret_cast<const uint4*>(nw + l * 8), wv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * rs * wv[i];
       }
+      if (a.rot_dim > 0) {
+        float y[8];  // the other of each pair
+        if (a.interleaved) {
 #pragma unroll
-      for (int o = 16 / V; o > 0; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o);
-        const int oat = __shfl_xor_sync(0xffffffffu, at, o);
-        if (fabsf(om) > fabsf(m) || (fabsf(om) == fabsf(m) && oat < at)) m = om, at = oat;
-        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
-      }
-      m = fminf(fmaxf(m, -65504.f), 65504.f);
-      uint32_t word = 0;
+          for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+        } else if (half % 8 == 0) {
+          const int src = l < half / 8 ? l + half / 8 : l - half / 8;
+          const int from = (threadIdx.x & 31 & ~(L - 1)) + (src & (L - 1));
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float t = m == 0.f ? 8.5f : __fdiv_rn(-8.f * x[i], m) + 8.5f;
-        const uint32_t code = (uint32_t)fminf(fmaxf(floorf(t), 0.f), 15.f);
-        const int e = (lane * V + i) & 7;
-        word |= code << (4 * (part == 1 ? (e >> 1) + 4 * (e & 1) : e));
-      }
+          for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], from);
+        } else {
+          // halves of 4 (mod 8) dims: up from dim d to d + half, down from d to d - half
+          const int base = threadIdx.x & 31 & ~(L - 1), q8 = half / 8;
 #pragma unroll
-      for (int o = 1; o < 8 / V; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-      uint8_t* blk = c.block(layer, page, part - 1, head);
-      const int d0 = lane * V, pr = pos % kPageTokens;
-      if (d0 % 8 == 0) {
-        const int wi = part == 1 ? ((d0 % 32) / 8) * (D / 32) + d0 / 32 : d0 / 8;
-        reinterpret_cast<uint32_t*>(blk + pr * (D / 2))[wi] = word;
+          for (int i = 0; i < 8; ++i) {
+            const float up = __shfl_sync(0xffffffffu, x[i ^ 4], base + ((l + q8 + (i >> 2)) & (L - 1)));
+            const float down = __shfl_sync(0xffffffffu, x[i ^ 4], base + ((l - q8 - 1 + (i >> 2)) & (L - 1)));
+            y[i] = l * 8 + i < half ? up : down;
+          }
+        }
+        if (kind < 2) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int d = l * 8 + i;
+            const bool plus = a.interleaved ? (i & 1) : d >= half;  // b cos + a sin, else a cos - b sin
+            if (d < a.rot_dim) x[i] = x[i] * cs[i] + (plus ? y[i] : -y[i]) * sn[i];
+          }
+        }
       }
-      if (d0 % 32 == 0)
-        reinterpret_cast<__half*>(blk + kPageTokens * (D / 2))[pr * (D / 32) + d0 / 32] =
-            bad ? __ushort_as_half(0x7fff) : __float2half_rn(m * -0.125f);
+      uint8_t* blk = live && kind ? c.block(layer, w.page, kind - 1, h) : nullptr;
+      const int pr = w.pos % kPageTokens;
+      if (Q4) {
+        __half unused;
+        __half* sc = blk ? reinterpret_cast<__half*>(blk + kPageTokens * (D / 2)) + pr * (D / 32) + l / 4 : &unused;
+        const uint32_t word = quantise8<L>(x, l, kind == 1, sc);
+        if (blk)
+          reinterpret_cast<uint32_t*>(blk + pr * (D / 2))[kind == 1 ? (l & 3) * (D / 32) + l / 4 : l] = word;
+      }
+      if (live && (kind == 0 || !Q4)) {
+        T* dst = kind == 0 ? (T*)a.q_out + row * a.qo_row + h * a.qo_head : (T*)blk + (size_t)pr * D;
+        uint4 u;
+        u.x = Act<T>::pack2(x[0], x[1]);
+        u.y = Act<T>::pack2(x[2], x[3]);
+        u.z = Act<T>::pack2(x[4], x[5]);
+        u.w = Act<T>::pack2(x[6], x[7]);
+        *reinterpret_cast<uint4*>(dst + l * 8) = u;
+      }
     }
   }
 }
 
 // ---- read ---------------------------------------------------------------------------
 template <int D>
-__global__ void __launch_bounds__(256) k_cache_read(CacheView c, int layer, CacheRows r, float* k, float* v, int* status) {
+__global__ void __launch_bounds__(kRowThreads)
+    k_cache_read(CacheView c, int layer, CacheRows r, float* k, float* v, int* status) {
+  constexpr int L = D / 8, GROUPS = kRowThreads / L;
+  griddep_wait();
+  griddep_launch();
+  const int row = blockIdx.x, l = threadIdx.x % L, grp = threadIdx.x / L;
   const int n_seqs = r.count();
-  const int n_rows = r.row0 ? min(r.row0[n_seqs], r.n_rows) : min(n_seqs, r.n_rows);
-  const int chunks = D / 8;  // 8 values a thread
-  const long long works = (long long)n_rows * 2 * c.kv_heads * chunks;
-  for (long long w = (long long)blockIdx.x * blockDim.x + threadIdx.x; w < works;
-       w += (long long)gridDim.x * blockDim.x) {
-    const int ch = (int)(w % chunks);
-    const int head = (int)(w / chunks % c.kv_heads);
-    const int kv = (int)(w / (chunks * c.kv_heads) & 1);
-    const int row = (int)(w / (2LL * chunks * c.kv_heads));
-    int lo = r.row0 ? 0 : row;
-    if (r.row0) {
-      int hi = n_seqs - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (r.row0[mid] <= row) lo = mid;
-        else hi = mid - 1;
-      }
-    }
-    int slot, p0, r0, n;
-    r.get(lo, slot, p0, r0, n);
-    if (row < r0 || row >= r0 + n || !cache_slot_ok(c, slot, status)) continue;
-    const int pos = p0 + row - r0;
-    const int page = cache_page(c, slot, pos, status);
-    if (page < 0) continue;
-    const uint8_t* blk = c.block(layer, page, kv, head);
-    const int pr = pos % kPageTokens;
+  if (row >= (r.row0 ? min(r.row0[n_seqs], r.n_rows) : min(n_seqs, r.n_rows))) return;
+  CacheRow w;
+  if (!cache_row(c, r, row, w, status)) return;
+  const int pr = w.pos % kPageTokens;
+  for (int h = grp; h < 2 * c.kv_heads; h += GROUPS) {
+    const int kv = h >= c.kv_heads, head = kv ? h - c.kv_heads : h;
+    const uint8_t* blk = c.block(layer, w.page, kv, head);
     float x[8];
     if (c.format == FMD_CACHE_Q4) {
-      const int wi = kv == 0 ? (ch % 4) * (D / 32) + ch / 4 : ch;
-      const uint32_t word = reinterpret_cast<const uint32_t*>(blk + pr * (D / 2))[wi];
+      const uint32_t word = reinterpret_cast<const uint32_t*>(blk + pr * (D / 2))[kv ? l : (l & 3) * (D / 32) + l / 4];
       const float d =
-          __half2float(reinterpret_cast<const __half*>(blk + kPageTokens * (D / 2))[pr * (D / 32) + ch / 4]);
+          __half2float(reinterpret_cast<const __half*>(blk + kPageTokens * (D / 2))[pr * (D / 32) + l / 4]);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        x[e] = (float)((int)(word >> (4 * (kv == 0 ? (e >> 1) + 4 * (e & 1) : e)) & 15) - 8) * d;
+        x[e] = (float)((int)(word >> (4 * (kv ? e : (e >> 1) + 4 * (e & 1))) & 15) - 8) * d;
     } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(blk + ((size_t)pr * D + ch * 8) * 2);
-      const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = c.format == FMD_CACHE_BF16 ? Act<__nv_bfloat16>::unpack2(uu[e]) : Act<__half>::unpack2(uu[e]);
-        x[2 * e] = f.x;
-        x[2 * e + 1] = f.y;
-      }
+      const uint4 u = *reinterpret_cast<const uint4*>(blk + ((size_t)pr * D + l * 8) * 2);
+      if (c.format == FMD_CACHE_BF16) unpack8<__nv_bfloat16>(u, x);
+      else unpack8<__half>(u, x);
     }
-    float4* dst = reinterpret_cast<float4*>((kv ? v : k) + ((size_t)row * c.kv_heads + head) * D + ch * 8);
+    float4* dst = reinterpret_cast<float4*>((kv ? v : k) + ((size_t)row * c.kv_heads + head) * D + l * 8);
     dst[0] = make_float4(x[0], x[1], x[2], x[3]);
     dst[1] = make_float4(x[4], x[5], x[6], x[7]);
   }
@@ -193,7 +266,7 @@ __global__ void __launch_bounds__(256) k_cache_read(CacheView c, int layer, Cach
 
 constexpr int kCopyBatch = 128;  // host pairs of one launch, passed by value
 struct CopyList {
-  int src[kCopyBatch], dst[kCopyBatch], rows[kCopyBatch];
+  int src[kCopyBatch], dst[kCopyBatch];
 };
 struct ForkList {
   int src[kCopyBatch], dst[kCopyBatch], len[kCopyBatch], page[kCopyBatch];
@@ -211,16 +284,35 @@ FMD_DEV void copy_block_rows(const CacheView& c, const uint8_t* src, uint8_t* ds
   }
 }
 
-// grid (pairs, layers x 2 x kv heads)
-__global__ void __launch_bounds__(128) k_cache_copy(CacheView c, CopyList l) {
-  const int i = blockIdx.x, bk = blockIdx.y % (2 * c.kv_heads), layer = blockIdx.y / (2 * c.kv_heads);
-  const int s = l.src[i], d = l.dst[i];
-  copy_block_rows(c, c.block(layer, s, 0, 0) + bk * c.block_bytes(), c.block(layer, d, 0, 0) + bk * c.block_bytes(),
-                  l.rows[i], threadIdx.x, blockDim.x);
+// Whole pages [bytes] of a layer: a block's threads keep eight 16-byte loads each in
+// flight before the stores.
+FMD_DEV void copy_page(const uint8_t* src, uint8_t* dst, size_t bytes) {
+  const int4* s = reinterpret_cast<const int4*>(src);
+  int4* d = reinterpret_cast<int4*>(dst);
+  const int n = (int)(bytes / 16), nt = blockDim.x;
+  int i = threadIdx.x;
+  for (; i + 7 * nt < n; i += 8 * nt) {
+    int4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = __ldcs(s + i + k * nt);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) __stcs(d + i + k * nt, v[k]);
+  }
+  for (; i < n; i += nt) __stcs(d + i, __ldcs(s + i));
 }
 
-__global__ void __launch_bounds__(128) k_cache_fork(CacheView c, int* table, ForkList l, int* status) {
-  const int i = blockIdx.x, bk = blockIdx.y % (2 * c.kv_heads), layer = blockIdx.y / (2 * c.kv_heads);
+__global__ void __launch_bounds__(256) k_cache_copy(CacheView c, int layers, CopyList l, int n) {
+  const long long works = (long long)n * layers;
+  for (long long w = blockIdx.x; w < works; w += gridDim.x) {
+    const int i = (int)(w % n), layer = (int)(w / n);
+    copy_page(c.block(layer, l.src[i], 0, 0), c.block(layer, l.dst[i], 0, 0), c.page_bytes());
+  }
+}
+
+// Block (i, b): fork i's table entries (b = 0) and its share of the blocks whose
+// rows are copied, a warp each.
+__global__ void __launch_bounds__(256) k_cache_fork(CacheView c, int layers, int* table, ForkList l, int* status) {
+  const int i = blockIdx.x, lane = threadIdx.x & 31;
   const int full = l.len[i] / kPageTokens, part = l.len[i] % kPageTokens;
   const int* from = table + (size_t)l.src[i] * c.max_pages;
   int* to = table + (size_t)l.dst[i] * c.max_pages;
@@ -228,14 +320,17 @@ __global__ void __launch_bounds__(128) k_cache_fork(CacheView c, int* table, For
     for (int k = threadIdx.x; k < full; k += blockDim.x) to[k] = from[k];
     if (threadIdx.x == 0 && part) to[full] = l.page[i];
   }
-  if (part) {
-    const int s = from[full];
-    if (s < 0 || s >= c.n_pages) {
-      cache_report(status, FMD_EINVAL);
-      return;
-    }
-    copy_block_rows(c, c.block(layer, s, 0, 0) + bk * c.block_bytes(),
-                    c.block(layer, l.page[i], 0, 0) + bk * c.block_bytes(), part, threadIdx.x, blockDim.x);
+  if (!part) return;
+  const int s = from[full];
+  if (s < 0 || s >= c.n_pages) {
+    cache_report(status, FMD_EINVAL);
+    return;
+  }
+  const long long blocks = (long long)layers * 2 * c.kv_heads;
+  const size_t bb = c.block_bytes();
+  for (long long b = (long long)blockIdx.y * 8 + (threadIdx.x >> 5); b < blocks; b += (long long)gridDim.y * 8) {
+    const int layer = (int)(b / (2 * c.kv_heads)), bk = (int)(b % (2 * c.kv_heads));
+    copy_block_rows(c, c.block(layer, s, 0, 0) + bk * bb, c.block(layer, l.page[i], 0, 0) + bk * bb, part, lane, 32);
   }
 }
 
@@ -319,13 +414,10 @@ __global__ void k_compact_remap(CacheView c, int* table, const int* n_entries, c
 __global__ void __launch_bounds__(256) k_compact_move(CacheView c, int layers, const int* src, const int* dst,
                                                       const int* counts) {
   const int n = counts[1];
-  const size_t pb = c.page_bytes();
   const long long works = (long long)n * layers;
   for (long long w = blockIdx.x; w < works; w += gridDim.x) {
     const int i = (int)(w % n), layer = (int)(w / n);
-    const int4* s = (const int4*)c.block(layer, src[i], 0, 0);
-    int4* d = (int4*)c.block(layer, dst[i], 0, 0);
-    for (size_t k = threadIdx.x; k < pb / 16; k += blockDim.x) d[k] = s[k];
+    copy_page(c.block(layer, src[i], 0, 0), c.block(layer, dst[i], 0, 0), c.page_bytes());
   }
 }
 
@@ -338,19 +430,38 @@ cudaError_t launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, c
   cfg.stream = s;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
+// The same with programmatic stream serialisation, for kernels that begin with griddep_wait.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_dep(void (*kern)(KArgs...), dim3 grid, dim3 block, cudaStream_t s, Args&&... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
 
 }  // namespace
 
 cudaError_t launch_cache_append(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAppend& a,
                                 int* status, cudaStream_t s) {
-  const long long works = (long long)r.n_rows * (a.n_heads + 2 * c.kv_heads);
-  const int grid = (int)std::min<long long>((works + 7) / 8, 148 * 8);
+  // Blocks of a row: one, or with few rows as many as its heads fill (append_one: 2
+  // heads a lane and one block for 32 heads would leave 147 SMs without work)
+  const int per_block = kRowThreads / (c.head_dim / 8) * 2;
+  const int most = (a.n_heads + 2 * c.kv_heads + per_block - 1) / per_block;
+  const int blocks = r.n_rows >= 148 ? 1 : most;
+  if ((long long)r.n_rows * blocks > INT_MAX) return cudaErrorInvalidConfiguration;
+  const dim3 grid(r.n_rows * blocks);
   auto go = [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     return c.format == FMD_CACHE_Q4
-               ? launch(k_cache_append<T, D, true>, dim3(grid), dim3(256), 0, s, c, layer, r, a, status)
-               : launch(k_cache_append<T, D, false>, dim3(grid), dim3(256), 0, s, c, layer, r, a, status);
+               ? launch_dep(k_cache_append<T, D, true>, grid, dim3(kRowThreads), s, c, layer, r, a, blocks, status)
+               : launch_dep(k_cache_append<T, D, false>, grid, dim3(kRowThreads), s, c, layer, r, a, blocks, status);
   };
   auto dim = [&](auto t) {
     return c.head_dim == 128 ? go(t, std::integral_constant<int, 128>{}) : go(t, std::integral_constant<int, 64>{});
@@ -464,10 +575,8 @@ int fmd_cache_read(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows
   if (!k || !v || !aligned16(k) || !aligned16(v)) return FMD_EINVAL;
   if (rows->n_seqs == 0 || rows->n_rows == 0) return FMD_OK;
   if (!on_current_device(c->pool) || !on_current_device(k)) return FMD_EINVAL;
-  const long long works = (long long)rows->n_rows * 2 * c->kv_heads * (c->head_dim / 8);
-  const int grid = (int)std::min<long long>((works + 255) / 256, 148 * 16);
-  return done(launch(c->head_dim == 128 ? k_cache_read<128> : k_cache_read<64>, dim3(grid), dim3(256), 0,
-                     (cudaStream_t)stream, view_of(c), layer, rows_of(rows), k, v, status));
+  return done(launch_dep(c->head_dim == 128 ? k_cache_read<128> : k_cache_read<64>, dim3(rows->n_rows),
+                         dim3(kRowThreads), (cudaStream_t)stream, view_of(c), layer, rows_of(rows), k, v, status));
 }
 
 int64_t fmd_cache_attend_workspace(const fmd_cache* c, int32_t n_heads, int32_t n_seqs, int32_t max_rows) {
@@ -514,9 +623,9 @@ int fmd_cache_copy_pages(const fmd_cache* c, int32_t n, const int32_t* src, cons
     const int m = std::min(kCopyBatch, n - i);
     std::memcpy(l.src, src + i, m * sizeof(int));
     std::memcpy(l.dst, dst + i, m * sizeof(int));
-    for (int k = 0; k < m; ++k) l.rows[k] = kPageTokens;
-    const cudaError_t e = launch(k_cache_copy, dim3(m, c->layers * 2 * c->kv_heads), dim3(128), 0,
-                                 (cudaStream_t)stream, view_of(c), l);
+    const int grid = (int)std::min<long long>((long long)m * c->layers, 148 * 8);
+    const cudaError_t e = launch(k_cache_copy, dim3(grid), dim3(256), 0, (cudaStream_t)stream, view_of(c), c->layers,
+                                 l, m);
     if (e != cudaSuccess) return done(e);
   }
   return FMD_OK;
@@ -543,8 +652,10 @@ int fmd_cache_fork(const fmd_cache* c, int32_t n, const int32_t* src_slot, const
     std::memcpy(l.dst, dst_slot + i, m * sizeof(int));
     std::memcpy(l.len, len + i, m * sizeof(int));
     std::memcpy(l.page, new_page + i, m * sizeof(int));
-    const cudaError_t e = launch(k_cache_fork, dim3(m, c->layers * 2 * c->kv_heads), dim3(128), 0,
-                                 (cudaStream_t)stream, view_of(c), c->page_table, l, status);
+    // a warp per copied block, at most about eight blocks of threads an SM
+    const int by = (int)std::min<long long>(((long long)c->layers * 2 * c->kv_heads + 7) / 8, std::max(1, 148 * 8 / m));
+    const cudaError_t e = launch(k_cache_fork, dim3(m, by), dim3(256), 0, (cudaStream_t)stream, view_of(c), c->layers,
+                                 c->page_table, l, status);
     if (e != cudaSuccess) return done(e);
   }
   return FMD_OK;
