@@ -12,23 +12,28 @@ namespace {
 
 // ---- rows ---------------------------------------------------------------------------
 //
-// append and read are bound by the bytes they move. A block takes one row (or a
-// part of its heads); L = D / 8 lanes take a head, 8 dims (16 bytes) each, so that
-// every access is a full sector; each lane has two heads' loads in flight before
-// it looks up the row's sequence, position and page, which they do not need.
+// append and read are bound by the bytes they move, as long as their instructions
+// stay few. A block of two warps takes one row (with few rows, some of its heads);
+// L = D / 8 lanes take a head, 8 dims (16 bytes) each, so that every access is a
+// full sector, and each lane has HPG heads' loads in flight before it looks up the
+// row's sequence, position and page, which they do not need. Two warps, not eight:
+// that lookup and the addresses cost about 400 instructions a warp, as much as
+// four heads.
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 64;
+constexpr int kRowHeads = 2;  // heads a lane has in flight, with many rows
 
-// Row `row`'s position, slot and page (-1 where the row takes no part). POS_ONLY
-// leaves the page out.
+// What a row is stored as: its position's place in a page, and the page's first
+// block in the layer. False where the row takes no part.
 struct CacheRow {
-  int slot, pos, page;
+  int pos;
+  uint8_t* page;
 };
-FMD_DEV bool cache_row(const CacheView& c, const CacheRows& r, int row, CacheRow& o, int* status) {
+FMD_DEV bool cache_row(const CacheView& c, const CacheRows& r, int layer, int row, CacheRow& o, int* status) {
   const int n_seqs = r.count();
   int lo = row;
   if (r.row0) {
-    int hi = n_seqs - 1;  // the last sequence that starts at or before the row
+    int hi = n_seqs;  // the last sequence that starts at or before the row; n_seqs: behind the last
     lo = 0;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -36,16 +41,17 @@ FMD_DEV bool cache_row(const CacheView& c, const CacheRows& r, int row, CacheRow
       else hi = mid - 1;
     }
   }
-  if (lo >= n_seqs) return false;
-  int p0, r0, n;
-  r.get(lo, o.slot, p0, r0, n);
-  if (row < r0 || row >= r0 + n || !cache_slot_ok(c, o.slot, status)) return false;
+  if (lo >= n_seqs || row >= r.n_rows) return false;
+  int slot, p0, r0, n;
+  r.get(lo, slot, p0, r0, n);
+  if (row < r0 || row >= r0 + n || !cache_slot_ok(c, slot, status)) return false;
   // p0 near the largest integer must not wrap into the table
   o.pos = p0 <= INT_MAX - (row - r0) ? p0 + (row - r0) : -1;
-  o.page = cache_page(c, o.slot, o.pos, status);
-  return o.page >= 0;
+  const int page = cache_page(c, slot, o.pos, status);
+  if (page < 0) return false;
+  o.page = c.block(layer, page, 0, 0);
+  return true;
 }
-
 template <typename T> FMD_DEV void unpack8(uint4 u, float (&x)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -56,78 +62,91 @@ template <typename T> FMD_DEV void unpack8(uint4 u, float (&x)[8]) {
   }
 }
 
-// The 4-bit code words and scale of a head: lane l of its L lanes holds dims
+// The 4-bit code word and scale of a head: lane l of its L lanes holds dims
 // 8 l .. 8 l + 7. The code is the exact floor(-8 x / m + 8.5): an estimate's
-// nearest integer B is decided by the sign of (8.5 - B) m - 8 x, one fused
-// multiply-add, instead of an IEEE division per value.
-template <int L> FMD_DEV uint32_t quantise8(const float (&x)[8], int l, bool key, __half* scale) {
+// nearest integer B is decided by the sign of (8.5 - B) |m| - 8 sgn(m) x, one fused
+// multiply-add, instead of an IEEE division per value. Every lane of the warp calls.
+FMD_DEV uint32_t quantise8(float (&x)[8], bool key, __half& scale) {
   const int lane = threadIdx.x & 31;
-  float a = 0.f;
-  bool bad = false;
+  float hi = x[0], lo = x[0], z = 0.f * x[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    a = fmaxf(a, fabsf(x[i]));
-    bad |= !(fabsf(x[i]) <= 3.4028234e38f);
+  for (int i = 1; i < 8; ++i) {
+    hi = fmaxf(hi, x[i]);
+    lo = fminf(lo, x[i]);
+    z = fmaf(0.f, x[i], z);  // NaN once a value is NaN or infinite
   }
-  float amax = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  float first = 0.f;  // this lane's first value of that magnitude
 #pragma unroll
-  for (int i = 7; i >= 0; --i)
-    if (fabsf(x[i]) == amax) first = x[i];
-  const uint32_t mates = 0xfu << (lane & ~3);
-  const uint32_t has = __ballot_sync(0xffffffffu, a == amax) & mates;
-  const bool any_bad = (__ballot_sync(0xffffffffu, bad) & mates) != 0;
-  const float m = __shfl_sync(0xffffffffu, first, has ? __ffs(has) - 1 : lane);
-  const float mag = fminf(fabsf(m), 65504.f), r = mag > 0.f ? -8.f / mag : 0.f;
+  for (int o = 1; o < 4; o <<= 1) {
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    z += __shfl_xor_sync(0xffffffffu, z, o);
+  }
+  float mag = fmaxf(hi, -lo);
+  float sgn = hi >= -lo ? 1.f : -1.f;
+  if (__any_sync(0xffffffffu, hi == -lo)) {
+    // both signs reach the magnitude: the first value counts
+    float first = 0.f;
+    bool has = false;
+#pragma unroll
+    for (int i = 7; i >= 0; --i)
+      if (fabsf(x[i]) == mag) first = x[i], has = true;
+    const uint32_t with = __ballot_sync(0xffffffffu, has) & (0xfu << (lane & ~3));
+    first = __shfl_sync(0xffffffffu, first, with ? __ffs(with) - 1 : lane);
+    if (hi == -lo) sgn = first < 0.f ? -1.f : 1.f;
+  }
+  if (__any_sync(0xffffffffu, mag > 65504.f)) {
+    mag = fminf(mag, 65504.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -65504.f), 65504.f);
+  }
+  const float m8 = -8.f * sgn, r = mag > 0.f ? __fdividef(m8, mag) : 0.f;
   uint32_t word = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float y = m < 0.f ? -x[e] : x[e];
-    const float t = fmaf(y, r, 8.5f), B = rintf(t);
-    float code = fmaf(8.5f - B, mag, -8.f * y) >= 0.f ? B : B - 1.f;
-    code = mag > 0.f ? fminf(fmaxf(code, 0.f), 15.f) : 8.f;
-    word |= (uint32_t)code << (4 * (key ? (e >> 1) + 4 * (e & 1) : e));
+    const float t = fmaf(x[e], r, 8.5f) + 12582912.f;  // 1.5 x 2^23: the nearest integer in the low bits
+    const float B = t - 12582912.f;
+    int code = (int)(__float_as_uint(t) & 31u);
+    if (fmaf(8.5f - B, mag, m8 * x[e]) < 0.f) --code;
+    code = min(code, 15);
+    word += (uint32_t)code << (4 * (key ? (e >> 1) + 4 * (e & 1) : e));
   }
-  if ((l & 3) == 0)
-    *scale = any_bad ? __ushort_as_half(0x7fff) : __float2half_rn((m < 0.f ? mag : -mag) * 0.125f);
+  scale = z == z ? __float2half_rn(mag * (sgn * -0.125f)) : __ushort_as_half(0x7fff);
   return word;
 }
 
 // ---- append -------------------------------------------------------------------------
 //
 // x * rsqrt(mean(x^2) + eps) * w, then (a, b) -> (a cos - b sin, b cos + a sin):
-// about 10 flop a byte at most, far below the memory's.
-template <typename T, int D, bool Q4>
+// about 10 flop a byte at most, far below the memory's. The queries', keys' and
+// values' heads are passed over one after the other, so that what is done with a
+// head is the same for the whole block.
+template <typename T, int D, bool Q4, int HPG>
 __global__ void __launch_bounds__(kRowThreads)
-    k_cache_append(CacheView c, int layer, CacheRows r, CacheAppend a, int blocks, int* status) {
-  constexpr int L = D / 8, GROUPS = kRowThreads / L, HPG = 2;
+    k_cache_append(CacheView c, int layer, CacheRows r, CacheAppend a, int* status) {
+  constexpr int L = D / 8, GROUPS = kRowThreads / L, PER = GROUPS * HPG;
+  constexpr int BB = Q4 ? kPageTokens * (D / 2 + D / 16) : kPageTokens * D * 2;
   griddep_wait();
   griddep_launch();
-  const int row = blockIdx.x / blocks, part = blockIdx.x % blocks;
-  const int l = threadIdx.x % L, grp = threadIdx.x / L;
-  const int heads = a.n_heads + 2 * c.kv_heads;
-  const int n_seqs = r.count();
-  if (row >= (r.row0 ? min(r.row0[n_seqs], r.n_rows) : min(n_seqs, r.n_rows))) return;
+  const int row = blockIdx.x, l = threadIdx.x % L, grp = threadIdx.x / L;
+  const int H = c.kv_heads, nq = (a.n_heads + PER - 1) / PER, nk = (H + PER - 1) / PER;
   const int half = a.rot_dim / 2;
   bool known = false;
   CacheRow w{};
   float cs[8], sn[8];
-  for (int h0 = part * GROUPS * HPG; h0 < heads; h0 += blocks * GROUPS * HPG) {
+  for (int it = blockIdx.y; it < nq + 2 * nk; it += gridDim.y) {
+    const int kind = it < nq ? 0 : it < nq + nk ? 1 : 2;  // queries, keys, values
+    const int h0 = (it - (kind == 0 ? 0 : kind == 1 ? nq : nq + nk)) * PER + grp, n = kind ? H : a.n_heads;
+    const T* src = (const T*)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
+                   row * (kind == 0 ? a.q_row : kind == 1 ? a.k_row : a.v_row) + l * 8;
+    const long long step = kind == 0 ? a.q_head : kind == 1 ? a.k_head : a.v_head;
     uint4 raw[HPG];
 #pragma unroll
-    for (int k = 0; k < HPG; ++k) {
-      const int h = h0 + k * GROUPS + grp;
-      if (h >= heads) continue;
-      const T* src = h < a.n_heads ? (const T*)a.q + row * a.q_row + h * a.q_head
-                     : h < a.n_heads + c.kv_heads
-                         ? (const T*)a.k + row * a.k_row + (h - a.n_heads) * a.k_head
-                         : (const T*)a.v + row * a.v_row + (h - a.n_heads - c.kv_heads) * a.v_head;
-      raw[k] = *reinterpret_cast<const uint4*>(src + l * 8);
-    }
+    for (int k = 0; k < HPG; ++k)
+      if (h0 + k * GROUPS < n && row < r.n_rows)
+        raw[k] = *reinterpret_cast<const uint4*>(src + (h0 + k * GROUPS) * step);
     if (!known) {
       known = true;
-      if (!cache_row(c, r, row, w, status)) return;  // the same for the whole block
+      if (!cache_row(c, r, layer, row, w, status)) return;  // the same for the whole block
       if (a.rot_dim > 0) {
         if (w.pos >= a.table_rows) {
           cache_report(status, FMD_EOVERFLOW);
@@ -135,60 +154,81 @@ __global__ void __launch_bounds__(kRowThreads)
         }
         const float* ct = a.cos + (size_t)w.pos * half;
         const float* st = a.sin + (size_t)w.pos * half;
-        // this lane's factors: of dims 8 l + i (halves), or of pairs 4 l + i / 2
+        // this lane's factors: of dims 8 l + i (halves), or of pairs 4 l + i / 2; the
+        // sine takes the sign that its place in the pair has
 #pragma unroll
         for (int q4 = 0; q4 < 2; ++q4) {
           const int d = l * 8 + q4 * 4;
-          if (d >= a.rot_dim) continue;
-          if (!a.interleaved) {
-            const int f = d < half ? d : d - half;  // half is a multiple of 4
-            const float4 cv = *reinterpret_cast<const float4*>(ct + f), sv = *reinterpret_cast<const float4*>(st + f);
-            cs[4 * q4] = cv.x, cs[4 * q4 + 1] = cv.y, cs[4 * q4 + 2] = cv.z, cs[4 * q4 + 3] = cv.w;
-            sn[4 * q4] = sv.x, sn[4 * q4 + 1] = sv.y, sn[4 * q4 + 2] = sv.z, sn[4 * q4 + 3] = sv.w;
-          } else {
-            const float2 cv = *reinterpret_cast<const float2*>(ct + d / 2),
-                         sv = *reinterpret_cast<const float2*>(st + d / 2);
-            cs[4 * q4] = cs[4 * q4 + 1] = cv.x, cs[4 * q4 + 2] = cs[4 * q4 + 3] = cv.y;
-            sn[4 * q4] = sn[4 * q4 + 1] = sv.x, sn[4 * q4 + 2] = sn[4 * q4 + 3] = sv.y;
+          float4 cv = make_float4(1.f, 1.f, 1.f, 1.f), sv = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (d < a.rot_dim) {
+            if (!a.interleaved) {
+              const int f = d < half ? d : d - half;  // half is a multiple of 4
+              cv = *reinterpret_cast<const float4*>(ct + f);
+              sv = *reinterpret_cast<const float4*>(st + f);
+              if (d < half) sv = make_float4(-sv.x, -sv.y, -sv.z, -sv.w);
+            } else {
+              const float2 c2 = *reinterpret_cast<const float2*>(ct + d / 2);
+              const float2 s2 = *reinterpret_cast<const float2*>(st + d / 2);
+              cv = make_float4(c2.x, c2.x, c2.y, c2.y);
+              sv = make_float4(-s2.x, s2.x, -s2.y, s2.y);
+            }
           }
+          cs[4 * q4] = cv.x, cs[4 * q4 + 1] = cv.y, cs[4 * q4 + 2] = cv.z, cs[4 * q4 + 3] = cv.w;
+          sn[4 * q4] = sv.x, sn[4 * q4 + 1] = sv.y, sn[4 * q4 + 2] = sv.z, sn[4 * q4 + 3] = sv.w;
         }
       }
     }
+    const int pr = w.pos % kPageTokens;
+    // head h of the output, this lane's 16 bytes (4 bits: the head's block)
+    uint8_t* dst;
+    long long dst_step;
+    if (kind == 0) {
+      dst = (uint8_t*)((T*)a.q_out + row * a.qo_row + l * 8);
+      dst_step = a.qo_head * 2;
+    } else {
+      dst = w.page + (kind - 1) * H * BB + (Q4 ? 0 : pr * (D * 2) + l * 16);
+      dst_step = BB;
+    }
+    const T* nw = (const T*)(kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr);
+    const bool turn = a.rot_dim > 0 && kind < 2;
+    if ((!Q4 || kind == 0) && !nw && !turn) {
+      // stored as it is
+#pragma unroll
+      for (int k = 0; k < HPG; ++k)
+        if (h0 + k * GROUPS < n) *reinterpret_cast<uint4*>(dst + (h0 + k * GROUPS) * dst_step) = raw[k];
+      continue;
+    }
+    float wv[8];
+    if (nw) unpack8<T>(*reinterpret_cast<const uint4*>(nw + l * 8), wv);
 #pragma unroll
     for (int k = 0; k < HPG; ++k) {
-      int h = h0 + k * GROUPS + grp;
-      const bool live = h < heads;  // the lanes of a warp stay together for the shuffles
-      const int kind = h < a.n_heads ? 0 : h < a.n_heads + c.kv_heads ? 1 : 2;
-      if (kind) h = (h - a.n_heads) % c.kv_heads;
+      const bool live = h0 + k * GROUPS < n;  // the lanes of a warp stay together for the shuffles
       if (!__any_sync(0xffffffffu, live)) continue;
       float x[8];
-      unpack8<T>(raw[k], x);
-      const T* nw = (const T*)(kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr);
-      float ss = 0.f;
+      unpack8<T>(live ? raw[k] : make_uint4(0, 0, 0, 0), x);
+      if (nw) {
+        float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (live && nw) {
-        const float rs = rsqrtf(ss / D + a.eps);
-        float wv[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(nw + l * 8), wv);
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float rs = rsqrtf(ss * (1.f / D) + a.eps);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = x[i] * rs * wv[i];
       }
-      if (a.rot_dim > 0) {
+      if (turn) {
         float y[8];  // the other of each pair
+        const int base = threadIdx.x & 31 & ~(L - 1);
         if (a.interleaved) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
         } else if (half % 8 == 0) {
-          const int src = l < half / 8 ? l + half / 8 : l - half / 8;
-          const int from = (threadIdx.x & 31 & ~(L - 1)) + (src & (L - 1));
+          const int from = base + ((l < half / 8 ? l + half / 8 : l - half / 8) & (L - 1));
 #pragma unroll
           for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], from);
         } else {
           // halves of 4 (mod 8) dims: up from dim d to d + half, down from d to d - half
-          const int base = threadIdx.x & 31 & ~(L - 1), q8 = half / 8;
+          const int q8 = half / 8;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float up = __shfl_sync(0xffffffffu, x[i ^ 4], base + ((l + q8 + (i >> 2)) & (L - 1)));
@@ -196,69 +236,92 @@ __global__ void __launch_bounds__(kRowThreads)
             y[i] = l * 8 + i < half ? up : down;
           }
         }
-        if (kind < 2) {
+        // dims behind rot_dim stay (their factors are 1 and 0, but what they would meet may be NaN)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int d = l * 8 + i;
-            const bool plus = a.interleaved ? (i & 1) : d >= half;  // b cos + a sin, else a cos - b sin
-            if (d < a.rot_dim) x[i] = x[i] * cs[i] + (plus ? y[i] : -y[i]) * sn[i];
-          }
+        for (int i = 0; i < 8; i += 4)
+          if (l * 8 + i < a.rot_dim)
+#pragma unroll
+            for (int e = i; e < i + 4; ++e) x[e] = fmaf(y[e], sn[e], x[e] * cs[e]);
+      }
+      uint8_t* at = dst + (h0 + k * GROUPS) * dst_step;
+      if (Q4 && kind) {
+        __half sc;
+        const uint32_t word = quantise8(x, kind == 1, sc);
+        if (live) {
+          reinterpret_cast<uint32_t*>(at + pr * (D / 2))[kind == 1 ? (l & 3) * (D / 32) + l / 4 : l] = word;
+          if ((l & 3) == 0)
+            reinterpret_cast<__half*>(at + kPageTokens * (D / 2))[pr * (D / 32) + l / 4] = sc;
         }
-      }
-      uint8_t* blk = live && kind ? c.block(layer, w.page, kind - 1, h) : nullptr;
-      const int pr = w.pos % kPageTokens;
-      if (Q4) {
-        __half unused;
-        __half* sc = blk ? reinterpret_cast<__half*>(blk + kPageTokens * (D / 2)) + pr * (D / 32) + l / 4 : &unused;
-        const uint32_t word = quantise8<L>(x, l, kind == 1, sc);
-        if (blk)
-          reinterpret_cast<uint32_t*>(blk + pr * (D / 2))[kind == 1 ? (l & 3) * (D / 32) + l / 4 : l] = word;
-      }
-      if (live && (kind == 0 || !Q4)) {
-        T* dst = kind == 0 ? (T*)a.q_out + row * a.qo_row + h * a.qo_head : (T*)blk + (size_t)pr * D;
+      } else if (live) {
         uint4 u;
         u.x = Act<T>::pack2(x[0], x[1]);
         u.y = Act<T>::pack2(x[2], x[3]);
         u.z = Act<T>::pack2(x[4], x[5]);
         u.w = Act<T>::pack2(x[6], x[7]);
-        *reinterpret_cast<uint4*>(dst + l * 8) = u;
+        *reinterpret_cast<uint4*>(at) = u;
       }
     }
   }
 }
 
 // ---- read ---------------------------------------------------------------------------
-template <int D>
+template <int D, int FORMAT>
 __global__ void __launch_bounds__(kRowThreads)
     k_cache_read(CacheView c, int layer, CacheRows r, float* k, float* v, int* status) {
-  constexpr int L = D / 8, GROUPS = kRowThreads / L;
+  constexpr int L = D / 8, GROUPS = kRowThreads / L, HPG = 4;
+  constexpr bool Q4 = FORMAT == FMD_CACHE_Q4;
+  constexpr int BB = Q4 ? kPageTokens * (D / 2 + D / 16) : kPageTokens * D * 2;
   griddep_wait();
   griddep_launch();
   const int row = blockIdx.x, l = threadIdx.x % L, grp = threadIdx.x / L;
-  const int n_seqs = r.count();
-  if (row >= (r.row0 ? min(r.row0[n_seqs], r.n_rows) : min(n_seqs, r.n_rows))) return;
   CacheRow w;
-  if (!cache_row(c, r, row, w, status)) return;
-  const int pr = w.pos % kPageTokens;
-  for (int h = grp; h < 2 * c.kv_heads; h += GROUPS) {
-    const int kv = h >= c.kv_heads, head = kv ? h - c.kv_heads : h;
-    const uint8_t* blk = c.block(layer, w.page, kv, head);
-    float x[8];
-    if (c.format == FMD_CACHE_Q4) {
-      const uint32_t word = reinterpret_cast<const uint32_t*>(blk + pr * (D / 2))[kv ? l : (l & 3) * (D / 32) + l / 4];
-      const float d =
-          __half2float(reinterpret_cast<const __half*>(blk + kPageTokens * (D / 2))[pr * (D / 32) + l / 4]);
+  if (!cache_row(c, r, layer, row, w, status)) return;
+  const int pr = w.pos % kPageTokens, H = c.kv_heads;
+  float* kd = k + (size_t)row * H * D + l * 8;
+  float* vd = v + (size_t)row * H * D + l * 8;
+  for (int h0 = blockIdx.y * GROUPS * HPG; h0 < 2 * H; h0 += gridDim.y * GROUPS * HPG) {
+    uint4 raw[HPG];
+    uint32_t word[HPG];
+    __half d[HPG];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        x[e] = (float)((int)(word >> (4 * (kv ? e : (e >> 1) + 4 * (e & 1))) & 15) - 8) * d;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(blk + ((size_t)pr * D + l * 8) * 2);
-      if (c.format == FMD_CACHE_BF16) unpack8<__nv_bfloat16>(u, x);
-      else unpack8<__half>(u, x);
+    for (int i = 0; i < HPG; ++i) {
+      const int h = h0 + i * GROUPS + grp;
+      if (h >= 2 * H) continue;
+      const uint8_t* blk = w.page + h * BB;
+      if constexpr (Q4) {
+        word[i] = reinterpret_cast<const uint32_t*>(blk + pr * (D / 2))[h >= H ? l : (l & 3) * (D / 32) + l / 4];
+        d[i] = reinterpret_cast<const __half*>(blk + kPageTokens * (D / 2))[pr * (D / 32) + l / 4];
+      } else {
+        raw[i] = *reinterpret_cast<const uint4*>(blk + pr * (D * 2) + l * 16);
+      }
     }
-    float4* dst = reinterpret_cast<float4*>((kv ? v : k) + ((size_t)row * c.kv_heads + head) * D + l * 8);
-    dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-    dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+#pragma unroll
+    for (int i = 0; i < HPG; ++i) {
+      const int h = h0 + i * GROUPS + grp;
+      if (h >= 2 * H) continue;
+      float x[8];
+      if constexpr (Q4) {
+        const float s = __half2float(d[i]);
+        // a key's nibbles to dim order, so that one path reads both
+        uint32_t t = word[i];
+        if (h < H) {
+          const uint32_t even = t & 0x0000ffffu, odd = t >> 16;  // dims 0 2 4 6 | 1 3 5 7
+          uint32_t e = (even | even << 8) & 0x00ff00ffu, o = (odd | odd << 8) & 0x00ff00ffu;
+          e = (e | e << 4) & 0x0f0f0f0fu;
+          o = (o | o << 4) & 0x0f0f0f0fu;
+          t = e | o << 4;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (float)((int)(t >> (4 * e) & 15) - 8) * s;
+      } else if constexpr (FORMAT == FMD_CACHE_BF16) {
+        unpack8<__nv_bfloat16>(raw[i], x);
+      } else {
+        unpack8<__half>(raw[i], x);
+      }
+      float4* dst = reinterpret_cast<float4*>(h < H ? kd + h * D : vd + (h - H) * D);
+      __stcs(dst, make_float4(x[0], x[1], x[2], x[3]));
+      __stcs(dst + 1, make_float4(x[4], x[5], x[6], x[7]));
+    }
   }
 }
 
@@ -449,19 +512,19 @@ cudaError_t launch_dep(void (*kern)(KArgs...), dim3 grid, dim3 block, cudaStream
 
 cudaError_t launch_cache_append(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAppend& a,
                                 int* status, cudaStream_t s) {
-  // Blocks of a row: one, or with few rows as many as its heads fill (append_one: 2
-  // heads a lane and one block for 32 heads would leave 147 SMs without work)
-  const int per_block = kRowThreads / (c.head_dim / 8) * 2;
-  const int most = (a.n_heads + 2 * c.kv_heads + per_block - 1) / per_block;
-  const int blocks = r.n_rows >= 148 ? 1 : most;
-  if ((long long)r.n_rows * blocks > INT_MAX) return cudaErrorInvalidConfiguration;
-  const dim3 grid(r.n_rows * blocks);
+  // With few rows a lane takes one head and a row as many blocks as its heads fill:
+  // append_one (32 heads) 5.9 us with 4 heads a lane, 4.3 so; append_prompts (10,007
+  // rows) the other way round.
+  const bool few = r.n_rows < 148 * 4;
+  const int g = kRowThreads / (c.head_dim / 8);
+  const int passes = (a.n_heads + g - 1) / g + 2 * ((c.kv_heads + g - 1) / g);
+  const dim3 grid(r.n_rows, few ? passes : 1);
   auto go = [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
-    return c.format == FMD_CACHE_Q4
-               ? launch_dep(k_cache_append<T, D, true>, grid, dim3(kRowThreads), s, c, layer, r, a, blocks, status)
-               : launch_dep(k_cache_append<T, D, false>, grid, dim3(kRowThreads), s, c, layer, r, a, blocks, status);
+    auto on = [&](auto kern) { return launch_dep(kern, grid, dim3(kRowThreads), s, c, layer, r, a, status); };
+    if (c.format == FMD_CACHE_Q4) return few ? on(k_cache_append<T, D, true, 1>) : on(k_cache_append<T, D, true, kRowHeads>);
+    return few ? on(k_cache_append<T, D, false, 1>) : on(k_cache_append<T, D, false, kRowHeads>);
   };
   auto dim = [&](auto t) {
     return c.head_dim == 128 ? go(t, std::integral_constant<int, 128>{}) : go(t, std::integral_constant<int, 64>{});
@@ -575,8 +638,17 @@ int fmd_cache_read(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows
   if (!k || !v || !aligned16(k) || !aligned16(v)) return FMD_EINVAL;
   if (rows->n_seqs == 0 || rows->n_rows == 0) return FMD_OK;
   if (!on_current_device(c->pool) || !on_current_device(k)) return FMD_EINVAL;
-  return done(launch_dep(c->head_dim == 128 ? k_cache_read<128> : k_cache_read<64>, dim3(rows->n_rows),
-                         dim3(kRowThreads), (cudaStream_t)stream, view_of(c), layer, rows_of(rows), k, v, status));
+  // blocks of a row: as in append
+  const int per_block = kRowThreads / (c->head_dim / 8) * 4, most = (2 * c->kv_heads + per_block - 1) / per_block;
+  const dim3 grid(rows->n_rows, rows->n_rows < 148 * 4 ? most : 1);
+  auto go = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return launch_dep(c->format == FMD_CACHE_Q4     ? k_cache_read<D, FMD_CACHE_Q4>
+                      : c->format == FMD_CACHE_BF16 ? k_cache_read<D, FMD_CACHE_BF16>
+                                                    : k_cache_read<D, FMD_CACHE_F16>,
+                      grid, dim3(kRowThreads), (cudaStream_t)stream, view_of(c), layer, rows_of(rows), k, v, status);
+  };
+  return done(c->head_dim == 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 64>{}));
 }
 
 int64_t fmd_cache_attend_workspace(const fmd_cache* c, int32_t n_heads, int32_t n_seqs, int32_t max_rows) {
