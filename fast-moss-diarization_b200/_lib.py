@@ -36,11 +36,14 @@ FINISH_STOP, FINISH_LENGTH, FINISH_ERROR = 0, 1, 2
 # cache formats (fmd_cache.h)
 CACHE_F16, CACHE_BF16, CACHE_Q4 = 1, 2, 4
 CACHE_WORKSPACE_ZERO = 65536
+# KV pool formats of a decoder handle (fmd_decoder.h)
+KV_ACT, KV_Q4 = 0, 4
 
 # every symbol the header declares
 EXPORTS = [
     "fmd_create", "fmd_destroy", "fmd_last_error", "fmd_status_string", "fmd_version", "fmd_load_weights",
     "fmd_kv_reserve", "fmd_cache_bytes", "fmd_memory_bytes", "fmd_embed", "fmd_splice_audio", "fmd_slot_open", "fmd_slot_release",
+    "fmd_kv_options", "fmd_slot_fork", "fmd_kv_compact",
     "fmd_slot_len", "fmd_prefill", "fmd_decode_step", "fmd_engine_load", "fmd_engine_start", "fmd_engine_step",
     "fmd_engine_run", "fmd_engine_fetch",
     "fmd_generate", "fmd_debug_weight", "fmd_debug_kv", "fmd_q8_0_quantize", "fmd_q8_0_quantize_device", "fmd_greedy_pick_noalloc",
@@ -183,6 +186,9 @@ def load() -> C.CDLL:
         "fmd_splice_audio": (C.c_int, [P, IP, I64, P, I64, I32, I32, P]),
         "fmd_slot_open": (C.c_int, [P, I32, I32]),
         "fmd_slot_release": (C.c_int, [P, I32]),
+        "fmd_kv_options": (C.c_int, [P, I32, I32, I32]),
+        "fmd_slot_fork": (C.c_int, [P, I32, I32, I32]),
+        "fmd_kv_compact": (C.c_int, [P, IP]),
         "fmd_slot_len": (C.c_int, [P, I32, IP]),
         "fmd_prefill": (C.c_int, [P, I32, IP, IP, P, I32, C.POINTER(C.c_float), IP]),
         "fmd_decode_step": (C.c_int, [P, I32, IP, IP, C.POINTER(C.c_float), IP]),

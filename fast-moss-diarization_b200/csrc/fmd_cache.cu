@@ -140,10 +140,12 @@ __global__ void __launch_bounds__(kRowThreads)
                    row * (kind == 0 ? a.q_row : kind == 1 ? a.k_row : a.v_row) + l * 8;
     const long long step = kind == 0 ? a.q_head : kind == 1 ? a.k_head : a.v_head;
     uint4 raw[HPG];
+    if (!a.staged) {
 #pragma unroll
-    for (int k = 0; k < HPG; ++k)
-      if (h0 + k * GROUPS < n && row < r.n_rows)
-        raw[k] = *reinterpret_cast<const uint4*>(src + (h0 + k * GROUPS) * step);
+      for (int k = 0; k < HPG; ++k)
+        if (h0 + k * GROUPS < n && row < r.n_rows)
+          raw[k] = *reinterpret_cast<const uint4*>(src + (h0 + k * GROUPS) * step);
+    }
     if (!known) {
       known = true;
       if (!cache_row(c, r, layer, row, w, status)) return;  // the same for the whole block
@@ -179,6 +181,15 @@ __global__ void __launch_bounds__(kRowThreads)
       }
     }
     const int pr = w.pos % kPageTokens;
+    if (a.staged) {
+      // the same block of the staging pool, which has 16-bit blocks
+      const uint8_t* at = a.staged + ((w.page - c.block(layer, 0, 0, 0)) / BB + (kind - 1) * H) * (kPageTokens * D * 2) +
+                          pr * (D * 2) + l * 16;
+#pragma unroll
+      for (int k = 0; k < HPG; ++k)
+        if (h0 + k * GROUPS < n)
+          raw[k] = *reinterpret_cast<const uint4*>(at + (size_t)(h0 + k * GROUPS) * (kPageTokens * D * 2));
+    }
     // head h of the output, this lane's 16 bytes (4 bits: the head's block)
     uint8_t* dst;
     long long dst_step;
@@ -532,6 +543,36 @@ cudaError_t launch_cache_append(bool bf16, const CacheView& c, int layer, const 
   return bf16 ? dim(__nv_bfloat16{}) : dim(__half{});
 }
 
+cudaError_t launch_cache_fork_one(const CacheView& c, int layers, int* table, int src, int dst, int len, int page,
+                                  cudaStream_t s) {
+  ForkList l{};
+  l.src[0] = src;
+  l.dst[0] = dst;
+  l.len[0] = len;
+  l.page[0] = page;
+  const int by = (int)std::min<long long>(((long long)layers * 2 * c.kv_heads + 7) / 8, 148 * 8);
+  return launch(k_cache_fork, dim3(1, by), dim3(256), 0, s, c, layers, table, l, (int*)nullptr);
+}
+
+// bitmap, map, src, dst, counts
+size_t cache_compact_workspace(int n_pages) {
+  return 4 * (((size_t)n_pages + 31) / 32 + 3 * (size_t)n_pages + 4);
+}
+
+cudaError_t launch_cache_compact(const CacheView& c, int layers, int* table, const int* n_entries, void* workspace,
+                                 int* n_used, int* status, cudaStream_t s) {
+  const size_t words = ((size_t)c.n_pages + 31) / 32, P = c.n_pages;
+  uint32_t* bits = (uint32_t*)workspace;
+  int *map = (int*)bits + words, *src = map + P, *dst = src + P, *counts = dst + P;
+  cudaError_t e = cudaMemsetAsync(bits, 0, words * 4, s);
+  if (e == cudaSuccess) e = launch(k_compact_mark, dim3(c.max_slots), dim3(256), 0, s, c, n_entries, bits, status);
+  if (e == cudaSuccess)
+    e = launch(k_compact_plan, dim3(1), dim3(1024), 0, s, c.n_pages, bits, map, src, dst, counts, n_used);
+  if (e == cudaSuccess) e = launch(k_compact_remap, dim3(c.max_slots), dim3(256), 0, s, c, table, n_entries, map, counts);
+  if (e == cudaSuccess) e = launch(k_compact_move, dim3(148 * 8), dim3(256), 0, s, c, layers, src, dst, counts);
+  return e;
+}
+
 }  // namespace fmd
 
 // =====================================================================================
@@ -626,7 +667,7 @@ int fmd_cache_append(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
   if (!on_current_device(c->pool) || !on_current_device(a->k)) return FMD_EINVAL;
   CacheAppend p{a->q,      a->k,      a->v,     a->q_out,     a->q_row,     a->q_head, a->k_row,
                 a->k_head, a->v_row,  a->v_head, a->q_out_row, a->q_out_head, a->q_norm, a->k_norm,
-                a->cos_table, a->sin_table, a->eps, a->n_heads, a->rot_dim, a->table_rows, a->interleaved};
+                a->cos_table, a->sin_table, a->eps, a->n_heads, a->rot_dim, a->table_rows, a->interleaved, nullptr};
   return done(launch_cache_append(a->dtype == FMD_DT_BF16, view_of(c), layer, rows_of(rows), p, status,
                                   (cudaStream_t)stream));
 }
@@ -733,11 +774,9 @@ int fmd_cache_fork(const fmd_cache* c, int32_t n, const int32_t* src_slot, const
   return FMD_OK;
 }
 
-// bitmap, map, src, dst, counts
 int64_t fmd_cache_compact_workspace(const fmd_cache* c) {
   if (!c || c->n_pages < 1) return 0;
-  const int64_t words = ((int64_t)c->n_pages + 31) / 32;
-  return 4 * (words + 3 * (int64_t)c->n_pages + 4);
+  return (int64_t)cache_compact_workspace(c->n_pages);
 }
 
 int fmd_cache_compact(const fmd_cache* c, const int32_t* n_entries, void* workspace, int64_t workspace_bytes,
@@ -747,18 +786,8 @@ int fmd_cache_compact(const fmd_cache* c, const int32_t* n_entries, void* worksp
   if (!n_entries || !workspace || !n_used || workspace_bytes < fmd_cache_compact_workspace(c) || !aligned16(workspace))
     return FMD_EINVAL;
   if (!on_current_device(c->pool) || !on_current_device(workspace)) return FMD_EINVAL;
-  const size_t words = ((size_t)c->n_pages + 31) / 32, P = c->n_pages;
-  uint32_t* bits = (uint32_t*)workspace;
-  int *map = (int*)bits + words, *src = map + P, *dst = src + P, *counts = dst + P;
-  cudaStream_t s = (cudaStream_t)stream;
-  const CacheView v = view_of(c);
-  cudaError_t e = cudaMemsetAsync(bits, 0, words * 4, s);
-  if (e == cudaSuccess) e = launch(k_compact_mark, dim3(c->max_slots), dim3(256), 0, s, v, n_entries, bits, status);
-  if (e == cudaSuccess) e = launch(k_compact_plan, dim3(1), dim3(1024), 0, s, c->n_pages, bits, map, src, dst, counts, n_used);
-  if (e == cudaSuccess)
-    e = launch(k_compact_remap, dim3(c->max_slots), dim3(256), 0, s, v, c->page_table, n_entries, map, counts);
-  if (e == cudaSuccess) e = launch(k_compact_move, dim3(148 * 8), dim3(256), 0, s, v, c->layers, src, dst, counts);
-  return done(e);
+  return done(launch_cache_compact(view_of(c), c->layers, c->page_table, n_entries, workspace, n_used, status,
+                                   (cudaStream_t)stream));
 }
 
 }  // extern "C"

@@ -26,7 +26,8 @@ struct CacheView {
 
 // The sequences of a launch. blk_n == nullptr: the public form (slot and pos0
 // by sequence, row0 null or [n + 1]). Else the decoder's prefill blocks: block
-// i has blk_n[i] rows from row row0[i], slot and pos0 are by row.
+// i has blk_n[i] rows from row row0[i], slot and pos0 are by row; an even block
+// and the next one, if it goes on in the same slot, are one sequence.
 struct CacheRows {
   const int* slot;
   const int* pos0;
@@ -43,6 +44,11 @@ struct CacheRows {
       n = blk_n[i];
       sl = slot[r0];
       p0 = pos0[r0];
+      if (i & 1) {
+        if (slot[row0[i - 1]] == sl) n = 0;  // part of the block before
+      } else if (i + 1 < count() && slot[row0[i + 1]] == sl) {
+        n += blk_n[i + 1];
+      }
     } else {
       r0 = row0 ? row0[i] : i;
       n = row0 ? row0[i + 1] - r0 : 1;
@@ -86,9 +92,20 @@ struct CacheAppend {
   const float *cos, *sin;
   float eps;
   int n_heads, rot_dim, table_rows, interleaved;
+  // keys and values come from a 16-bit pool of one layer with the same page table
+  // (k and v are not read)
+  const uint8_t* staged;
 };
 cudaError_t launch_cache_append(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAppend& a,
                                 int* status, cudaStream_t s);
+
+// Copies the rows behind the full pages of `len` positions of a fork (fmd_cache_fork, one).
+cudaError_t launch_cache_fork_one(const CacheView& c, int layers, int* table, int src, int dst, int len, int page,
+                                  cudaStream_t s);
+// fmd_cache_compact
+size_t cache_compact_workspace(int n_pages);
+cudaError_t launch_cache_compact(const CacheView& c, int layers, int* table, const int* n_entries, void* workspace,
+                                 int* n_used, int* status, cudaStream_t s);
 
 struct CacheAttend {
   const void* q;

@@ -150,7 +150,7 @@ FMD_DEV int ck_work(const CkArgs& p, const CacheView& c, int round, CkWork& w, i
   const long long item = at / p.parts;
   w.item = (int)item;
   w.h = (int)(item % H);
-  const int seq = (int)(item / H % ns), tile = p.tiles - 1 - (int)(item / H / ns);
+  const int seq = ns - 1 - (int)(item / H % ns), tile = p.tiles - 1 - (int)(item / H / ns);
   int n;
   p.r.get(seq, w.slot, w.p0, w.r0, n);
   if (n <= 0 || !cache_slot_ok(c, w.slot, status)) return 0;

@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "../../include/fmd_decoder.h"
+#include "fmd_cache.cuh"
 #include "fmd_kernels.cuh"
 #include "fmd_scheduler.cuh"
 #include "fmd_watch.h"
@@ -123,7 +124,16 @@ struct fmd_handle {
   bool reserved = false;
   int max_slots = 0, max_rows = 0, n_pages = 0, max_pages_per_slot = 0;
   int pb_max = 0, di_max = 0, di_grid = 0;
-  KvView kv{};
+  KvView kv{};             // what the projections write: the pool, or (4 bits) one layer of 16-bit staging
+  // fmd_kv_options: a cache in 4 bits, attention with a window and sinks. Either
+  // puts the steps' attention on the cache operators (fmd_cache.cuh) instead of
+  // k_attn_decode_tma / k_attn_prefill_*.
+  bool kv_q4 = false;
+  int kv_window = 0, kv_sinks = 0;
+  bool cache_ops() const { return kv_q4 || kv_window > 0; }
+  CacheView cache{};        // the pool as the cache operators see it
+  void* cache_ws = nullptr;
+  std::vector<int> page_names;  // slots that name a page (host allocator)
   alignas(64) CUtensorMap kv_tmap;  // the KV pool as [rows][128] for TMA tile loads
   // activation operands of the mixed-step tensor-core projections
   alignas(64) CUtensorMap amap_xn, amap_ctx, amap_hbuf;
@@ -568,6 +578,35 @@ DecodeView decode_view(fmd_handle* h, int half) {
   return v;
 }
 
+// Steps on the cache operators, one layer: the rows' staged keys and values into
+// the 4-bit pool, then the attention of the decode rows and, in mixed steps, of the
+// prefill blocks.
+void cache_layer(fmd_handle* h, int l, int max_rows, const int* n_rows_ptr, bool mixed, cudaStream_t s) {
+  const Plan& p = h->plan;
+  const bool bf = h->at == kBF16;
+  cudaError_t e = cudaSuccess;
+  if (h->kv_q4) {
+    const CacheRows rows{p.row_slot, p.row_pos, nullptr, nullptr, n_rows_ptr, max_rows, max_rows};
+    CacheAppend a{};
+    a.staged = (const uint8_t*)h->kv.base;
+    e = launch_cache_append(bf, h->cache, l, rows, a, h->d_status, s);
+    trace(h, "cache_append", l);
+  }
+  const int hd = h->Hq() * kHeadDim;
+  CacheAttend a{h->qbuf, h->ctx, hd, kHeadDim, hd, kHeadDim, h->attn_scale, h->Hq(), h->kv_window, h->kv_sinks, 1};
+  const CacheRows decode{p.row_slot, p.row_pos, nullptr, nullptr, &p.counts->n_decode, h->max_slots, h->max_rows};
+  if (e == cudaSuccess) e = launch_cache_decode(bf, h->cache, l, decode, a, h->cache_ws, h->d_status, s);
+  trace(h, "cache_decode", l);
+  if (mixed) {
+    // pairs of blocks: the two 128-pair tiles of an item
+    a.max_rows = 2 * kRowsPerPBlock;
+    const CacheRows blocks{p.row_slot, p.row_pos, p.pb_row0, p.pb_n, &p.counts->n_pblocks, h->pb_max, h->max_rows};
+    if (e == cudaSuccess) e = launch_cache_chunk(bf, h->cache, l, blocks, a, h->cache_ws, h->d_status, s);
+    trace(h, "cache_chunk", l);
+  }
+  if (e != cudaSuccess) h->launch_refused = true;
+}
+
 // The layer loop of a decode-only pass over the rows of `v` on stream `s`.
 void decode_layers(fmd_handle* h, const DecodeView& v, cudaStream_t s, bool probe_attn) {
   const fmd_config& c = h->cfg;
@@ -601,14 +640,17 @@ void decode_layers(fmd_handle* h, const DecodeView& v, cudaStream_t s, bool prob
       qkv.norm_w = Ly.in_norm;
       qkv.qn_w = Ly.q_norm;
       qkv.kn_w = Ly.k_norm;
-      qkv.layer = l;
+      qkv.layer = h->kv_q4 ? 0 : l;
       if (!launch_gemv(h->at, kGemvQkv, true, Ly.qkv, v.x, H, nullptr, nrows, R, qkv, h->d_status, s)) h->launch_refused = true;
       trace(h, "qkv", l);
     }
     const bool probe = probe_attn && h->record_attn_events && l == h->attn_probe_layer();
     if (probe) cudaEventRecordWithFlags(h->attn_events[0], s, cudaEventRecordExternal);
-    launch_attn_decode_tma(h->at, &h->kv_tmap, v.plan, v.grid, h->Hq(), h->Hkv(), v.qbuf, h->kv, l,
-                           h->attn_scale, v.pacc, v.pml, v.counters, v.ctx, h->d_status, s);
+    if (h->cache_ops())
+      cache_layer(h, l, R, nrows, false, s);
+    else
+      launch_attn_decode_tma(h->at, &h->kv_tmap, v.plan, v.grid, h->Hq(), h->Hkv(), v.qbuf, h->kv, l,
+                             h->attn_scale, v.pacc, v.pml, v.counters, v.ctx, h->d_status, s);
     if (probe) cudaEventRecordWithFlags(h->attn_events[1], s, cudaEventRecordExternal);
     trace(h, "attn_decode", l);
     if (h->chain_ok) {
@@ -728,7 +770,7 @@ void run_forward(fmd_handle* h, float* logits_dev, const void* arena, bool decod
     pq.cos = h->rope_cos;
     pq.sin = h->rope_sin;
     pq.q_out = h->qbuf;
-    pq.layer = l;
+    pq.layer = h->kv_q4 ? 0 : l;
     pq.Hq = h->Hq();
     pq.Hkv = h->Hkv();
     pq.eps = eps;
@@ -738,16 +780,19 @@ void run_forward(fmd_handle* h, float* logits_dev, const void* arena, bool decod
       const PartSplit sp_qkv = mixed_linear(h, L.qkv, L.tc_qkv, h->xn, h->amap_xn, H);
       trace(h, "qkv", l);
       launch_qkv_epilogue(h->at, h->plan, row_grid, h->part, sp_qkv, ss, h->Hq(), h->Hkv(), L.q_norm, L.k_norm,
-                          h->rope_cos, h->rope_sin, h->qbuf, h->kv, l, eps, s);
+                          h->rope_cos, h->rope_sin, h->qbuf, h->kv, h->kv_q4 ? 0 : l, eps, s);
       trace(h, "qkv_epi", l);
     }
     const bool probe = h->record_attn_events && l == h->attn_probe_layer();
     if (probe) cudaEventRecordWithFlags(h->attn_events[0], s, cudaEventRecordExternal);
-    launch_attn_decode_tma(h->at, &h->kv_tmap, h->plan, h->di_grid, h->Hq(), h->Hkv(), h->qbuf, h->kv, l,
-                           h->attn_scale, h->pacc, h->pml, h->attn_counters, h->ctx, h->d_status, s);
+    if (h->cache_ops())
+      cache_layer(h, l, R, nrows, true, s);
+    else
+      launch_attn_decode_tma(h->at, &h->kv_tmap, h->plan, h->di_grid, h->Hq(), h->Hkv(), h->qbuf, h->kv, l,
+                             h->attn_scale, h->pacc, h->pml, h->attn_counters, h->ctx, h->d_status, s);
     if (probe) cudaEventRecordWithFlags(h->attn_events[1], s, cudaEventRecordExternal);
     trace(h, "attn_decode", l);
-    launch_attn_prefill_tc(h->at, &h->kv_tmap, &h->qmap, h->plan, h->pb_max, h->Hq(), h->Hkv(), h->kv, l,
+    if (!h->cache_ops()) launch_attn_prefill_tc(h->at, &h->kv_tmap, &h->qmap, h->plan, h->pb_max, h->Hq(), h->Hkv(), h->kv, l,
                            h->attn_scale, h->ctx, h->d_status, s, h->pf_pp_allowed ? h->n_sm : 0);
     trace(h, "attn_prefill", l);
     const PartSplit sp_o = run_proj(L.tc_o, h->amap_ctx, kProjF32, pf32)
@@ -934,6 +979,7 @@ int ensure_pages(fmd_handle* h, int slot, int upto_len) {
   while (h->slot_npages[slot] < need) {
     if (h->free_pages.empty()) return fail(h, FMD_ENOMEM, "KV pool exhausted");
     h->h_page_table[(size_t)slot * h->max_pages_per_slot + h->slot_npages[slot]] = h->free_pages.back();
+    h->page_names[h->free_pages.back()] = 1;
     h->free_pages.pop_back();
     h->slot_npages[slot] += 1;
     changed = true;
@@ -1125,6 +1171,17 @@ int fmd_memory_bytes(const fmd_handle* h, int64_t* weights, int64_t* kv_pool, in
   return FMD_OK;
 }
 
+int fmd_kv_options(fmd_handle* h, int32_t format, int32_t window, int32_t sinks) {
+  if (!h) return FMD_EINVAL;
+  if (h->reserved) return fail(h, FMD_EBUSY, "set the cache options before reserving the KV pool");
+  if (format != FMD_KV_ACT && format != FMD_KV_Q4) return fail(h, FMD_EINVAL, "the cache format is the activation dtype or 4 bits");
+  if (window < 0 || sinks < 0) return fail(h, FMD_EINVAL, "window and sinks must be >= 0");
+  h->kv_q4 = format == FMD_KV_Q4;
+  h->kv_window = window;
+  h->kv_sinks = sinks;
+  return FMD_OK;
+}
+
 int fmd_kv_reserve(fmd_handle* h, int32_t max_slots, int64_t max_tokens_total, int32_t max_rows_per_step) {
   if (!h) return FMD_EINVAL;
   if (!h->loaded) return fail(h, FMD_EBUSY, "load weights before reserving the KV pool");
@@ -1144,8 +1201,9 @@ int fmd_kv_reserve(fmd_handle* h, int32_t max_slots, int64_t max_tokens_total, i
   if (pages > (1LL << 30)) return fail(h, FMD_ENOMEM, "KV pool too large");
   h->n_pages = (int)pages;
   int rc;
-  // KV pool
-  const size_t kv_elems = (size_t)c.num_hidden_layers * h->n_pages * 2 * c.num_key_value_heads * kPageTokens * kHeadDim;
+  // KV pool; in 4 bits, the pool and one layer of 16-bit staging that the projections write
+  const size_t kv_elems = (size_t)(h->kv_q4 ? 1 : c.num_hidden_layers) * h->n_pages * 2 * c.num_key_value_heads *
+                          kPageTokens * kHeadDim;
   void* kvp;
   if ((rc = dev_alloc(h, kv_elems * 2, &kvp, &h->kv_bytes))) return rc;
   CK(cudaMemset(kvp, 0, kv_elems * 2));
@@ -1153,8 +1211,22 @@ int fmd_kv_reserve(fmd_handle* h, int32_t max_slots, int64_t max_tokens_total, i
   h->kv.n_pages = h->n_pages;
   h->kv.max_pages_per_slot = h->max_pages_per_slot;
   h->kv.kv_heads = c.num_key_value_heads;
+  h->cache = CacheView{(uint8_t*)kvp,  nullptr,
+                       h->kv_q4        ? FMD_CACHE_Q4
+                       : h->at == kBF16 ? FMD_CACHE_BF16
+                                        : FMD_CACHE_F16,
+                       h->n_pages,     c.num_key_value_heads,
+                       kHeadDim,       max_slots,
+                       h->max_pages_per_slot};
+  if (h->kv_q4) {
+    void* q4p;
+    const size_t bytes = (size_t)c.num_hidden_layers * h->n_pages * h->cache.page_bytes();
+    if ((rc = dev_alloc(h, bytes, &q4p, &h->kv_bytes))) return rc;
+    CK(cudaMemset(q4p, 0, bytes));
+    h->cache.pool = (uint8_t*)q4p;
+  }
   {
-    const uint64_t rows = (uint64_t)c.num_hidden_layers * h->n_pages * 2 * c.num_key_value_heads * kPageTokens;
+    const uint64_t rows = (uint64_t)(h->kv_q4 ? 1 : c.num_hidden_layers) * h->n_pages * 2 * c.num_key_value_heads * kPageTokens;
     if (rows > (uint64_t)INT32_MAX) return fail(h, FMD_ENOTSUP, "KV pool too large for 32-bit TMA row coordinates");
     void* fn = nullptr;
     if ((rc = tmap_encoder(h, &fn))) return rc;
@@ -1173,6 +1245,8 @@ int fmd_kv_reserve(fmd_handle* h, int32_t max_slots, int64_t max_tokens_total, i
   CK(cudaMemset(pt, 0, (size_t)max_slots * h->max_pages_per_slot * 4));
   h->d_page_table = (int*)pt;
   h->kv.page_table = h->d_page_table;
+  h->cache.page_table = h->d_page_table;
+  h->page_names.assign(h->n_pages, 0);
   h->h_page_table.assign((size_t)max_slots * h->max_pages_per_slot, 0);
   h->free_pages.clear();
   for (int i = h->n_pages - 1; i >= 0; --i) h->free_pages.push_back(i);
@@ -1193,7 +1267,7 @@ int fmd_kv_reserve(fmd_handle* h, int32_t max_slots, int64_t max_tokens_total, i
   // the persistent layer tail: Q8_0 weights, decode steps of <= 64 rows, one
   // CTA per SM with the layer's weights resident in shared memory
   h->chain_ok = false;
-  if (h->q8 && h->chain_allowed && max_slots <= kChainMaxRows && c.num_hidden_layers > 0) {
+  if (h->q8 && h->chain_allowed && max_slots <= kChainMaxRows && c.num_hidden_layers > 0 && !h->cache_ops()) {
     // every layer has the shapes of layer 0
     char why[160] = "";
     h->chain_ok = chain_plan(h->at, make_chain(h, 0), h->n_sm, max_slots, &h->chain_clusters, &h->chain_smem, why,
@@ -1222,7 +1296,7 @@ int fmd_kv_reserve(fmd_handle* h, int32_t max_slots, int64_t max_tokens_total, i
   h->pacc = (float*)p;
   h->pml = h->pacc + (size_t)2 * h->di_grid * 2 * kHeadDim;
   // a split decode step: the second half's attention partials, both halves' row counts
-  h->split_ok = h->split_allowed && !h->chain_ok && max_slots >= 16 && max_slots % 2 == 0;
+  h->split_ok = h->split_allowed && !h->chain_ok && !h->cache_ops() && max_slots >= 16 && max_slots % 2 == 0;
   if (h->split_ok) {
     if ((rc = A(attn_decode_partial_floats(h->di_grid) * 4, &p))) return rc;
     h->pacc2 = (float*)p;
@@ -1251,6 +1325,13 @@ int fmd_kv_reserve(fmd_handle* h, int32_t max_slots, int64_t max_tokens_total, i
   if ((rc = A(4 * sizeof(int), &p))) return rc;
   CK(cudaMemset(p, 0, 4 * sizeof(int)));
   h->d_status = (int*)p;
+  if (h->cache_ops()) {
+    const size_t n = std::max(cache_decode_workspace(h->cache, h->Hq(), 1),
+                              cache_chunk_workspace(h->cache, h->Hq(), h->pb_max, 2 * kRowsPerPBlock));
+    if ((rc = A(n, &p))) return rc;
+    CK(cudaMemset(p, 0, n));
+    h->cache_ws = p;
+  }
   if (h->chain_ok) {
     const size_t n = (size_t)c.num_hidden_layers * kChainSyncInts * sizeof(int);
     if ((rc = A(n, &p))) return rc;
@@ -1381,11 +1462,79 @@ int fmd_slot_open(fmd_handle* h, int32_t slot, int32_t capacity) {
 int fmd_slot_release(fmd_handle* h, int32_t slot) {
   if (!h) return FMD_EINVAL;
   if (!h->reserved || slot < 0 || slot >= h->max_slots) return fail(h, FMD_EINVAL, "bad slot");
-  for (int k = 0; k < h->slot_npages[slot]; ++k)
-    h->free_pages.push_back(h->h_page_table[(size_t)slot * h->max_pages_per_slot + k]);
+  for (int k = 0; k < h->slot_npages[slot]; ++k) {
+    const int page = h->h_page_table[(size_t)slot * h->max_pages_per_slot + k];
+    if (--h->page_names[page] == 0) h->free_pages.push_back(page);  // no fork shares it
+  }
   h->slot_npages[slot] = 0;
   h->slot_cap[slot] = -1;
   h->slot_len[slot] = 0;
+  return FMD_OK;
+}
+
+int fmd_slot_fork(fmd_handle* h, int32_t src, int32_t dst, int32_t capacity) {
+  int rc = check_ready(h);
+  if (rc) return rc;
+  if (src < 0 || src >= h->max_slots || dst < 0 || dst >= h->max_slots) return fail(h, FMD_EINVAL, "bad slot");
+  if (h->slot_cap[src] < 0) return fail(h, FMD_EINVAL, "fork of a closed slot");
+  if (h->slot_cap[dst] >= 0) return fail(h, FMD_EBUSY, "slot already open");
+  const int len = h->slot_len[src], full = len / kPageTokens;
+  if (capacity < 1 || capacity < len) return fail(h, FMD_EINVAL, "capacity is smaller than the forked sequence");
+  if (capacity > h->max_pages_per_slot * kPageTokens)
+    return fail(h, FMD_EOVERFLOW, "capacity exceeds the RoPE table length");
+  const int need = (capacity + kPageTokens - 1) / kPageTokens - full;
+  if ((int)h->free_pages.size() < need) return fail(h, FMD_ENOMEM, "KV pool has too few free pages");
+  CK(cudaSetDevice(h->device));
+  int* from = h->h_page_table.data() + (size_t)src * h->max_pages_per_slot;
+  int* to = h->h_page_table.data() + (size_t)dst * h->max_pages_per_slot;
+  for (int k = 0; k < full; ++k) {
+    to[k] = from[k];
+    ++h->page_names[to[k]];
+  }
+  h->slot_npages[dst] = full;
+  h->slot_cap[dst] = capacity;
+  h->slot_len[dst] = len;
+  if ((rc = ensure_pages(h, dst, capacity))) return rc;
+  if (need == 0)  // nothing was taken: the table's row is still to be written
+    CK(cudaMemcpyAsync(h->d_page_table + (size_t)dst * h->max_pages_per_slot, to, full * sizeof(int),
+                       cudaMemcpyHostToDevice, h->stream));
+  if (len % kPageTokens)
+    CK(launch_cache_fork_one(h->cache, h->cfg.num_hidden_layers, h->d_page_table, src, dst, len, to[full], h->stream));
+  return sync_check(h);
+}
+
+int fmd_kv_compact(fmd_handle* h, int32_t* n_used) {
+  int rc = check_ready(h);
+  if (rc) return rc;
+  bool open = false;
+  for (int s = 0; s < h->max_slots; ++s) open |= h->slot_cap[s] >= 0;
+  if (n_used) *n_used = 0;
+  if (!open) return FMD_OK;
+  CK(cudaSetDevice(h->device));
+  void* ws = nullptr;
+  const size_t plan = (cache_compact_workspace(h->n_pages) + 15) / 16 * 16;
+  CK(cudaMalloc(&ws, plan + ((size_t)h->max_slots + 1) * sizeof(int)));
+  int* entries = (int*)((uint8_t*)ws + plan);
+  int used = 0;
+  const size_t table = h->h_page_table.size() * sizeof(int);
+  cudaError_t e = cudaMemcpyAsync(entries, h->slot_npages.data(), h->max_slots * sizeof(int), cudaMemcpyHostToDevice,
+                                  h->stream);
+  if (e == cudaSuccess)
+    e = launch_cache_compact(h->cache, h->cfg.num_hidden_layers, h->d_page_table, entries, ws, entries + h->max_slots,
+                             nullptr, h->stream);
+  if (e == cudaSuccess)
+    e = cudaMemcpyAsync(&used, entries + h->max_slots, sizeof(int), cudaMemcpyDeviceToHost, h->stream);
+  if (e == cudaSuccess)
+    e = cudaMemcpyAsync(h->h_page_table.data(), h->d_page_table, table, cudaMemcpyDeviceToHost, h->stream);
+  rc = e != cudaSuccess ? fail(h, FMD_EIO, std::string("compaction: ") + cudaGetErrorString(e)) : sync_check(h);
+  cudaFree(ws);
+  if (rc) return rc;
+  std::fill(h->page_names.begin(), h->page_names.end(), 0);
+  for (int s = 0; s < h->max_slots; ++s)
+    for (int k = 0; k < h->slot_npages[s]; ++k) ++h->page_names[h->h_page_table[(size_t)s * h->max_pages_per_slot + k]];
+  h->free_pages.clear();
+  for (int i = h->n_pages - 1; i >= used; --i) h->free_pages.push_back(i);
+  if (n_used) *n_used = used;
   return FMD_OK;
 }
 
@@ -1838,6 +1987,30 @@ int fmd_debug_kv(fmd_handle* h, int32_t slot, int32_t layer, int32_t pos, int32_
   CK(cudaSetDevice(h->device));
   const int Hkv = h->Hkv();
   const size_t rowb = kHeadDim * 2;
+  if (h->kv_q4) {
+    // the values that the 4-bit cache holds, rounded to the activation dtype
+    int* seq = nullptr;
+    float* f = nullptr;
+    const size_t half = (size_t)n * Hkv * kHeadDim;
+    if (n == 0) return FMD_OK;
+    CK(cudaMalloc((void**)&f, 2 * half * 4 + 16));
+    seq = (int*)(f + 2 * half);
+    const int desc[4] = {slot, pos, 0, n};
+    std::vector<float> host(2 * half);
+    const fmd_cache c{h->cache.pool, h->d_page_table,   FMD_CACHE_Q4,   h->cfg.num_hidden_layers, h->n_pages,
+                      Hkv,           kHeadDim,          h->max_slots,   h->max_pages_per_slot,    0};
+    const fmd_cache_rows r{seq, seq + 1, seq + 2, 1, n, n, 0};
+    cudaError_t e = cudaMemcpyAsync(seq, desc, sizeof(desc), cudaMemcpyHostToDevice, h->stream);
+    int rc = e == cudaSuccess ? fmd_cache_read(&c, layer, &r, f, f + half, nullptr, h->stream) : FMD_EIO;
+    if (rc == FMD_OK) e = cudaMemcpyAsync(host.data(), f, 2 * half * 4, cudaMemcpyDeviceToHost, h->stream);
+    rc = rc != FMD_OK || e != cudaSuccess ? fail(h, FMD_EIO, "reading the 4-bit cache failed") : sync_check(h);
+    cudaFree(f);
+    if (rc) return rc;
+    for (size_t i = 0; i < 2 * half; ++i)
+      ((uint16_t*)(i < half ? k_out : v_out))[i < half ? i : i - half] =
+          h->at == kBF16 ? f32_to_bf16_bits(host[i]) : f32_to_f16_bits(host[i]);
+    return FMD_OK;
+  }
   for (int i = 0; i < n; ++i) {
     const int p = pos + i;
     const int page = h->h_page_table[(size_t)slot * h->max_pages_per_slot + p / kPageTokens];

@@ -123,9 +123,16 @@ class Qwen3Decoder:
         keep.append(layers)
         self._check(self.lib.fmd_load_weights(self._h, C.byref(ws)))
 
-    def reserve(self, max_slots: int, max_tokens: int, max_rows: int) -> None:
+    def reserve(self, max_slots: int, max_tokens: int, max_rows: int, kv: str = "act", window: int = 0,
+                sinks: int = 0) -> None:
         """`Qwen3::new_caches` sizing: a paged pool of `max_tokens` positions for
-        `max_slots` sequences; up to `max_rows` token rows per forward pass."""
+        `max_slots` sequences; up to `max_rows` token rows per forward pass. `kv`:
+        "act" (the activation dtype) or "q4" (4 bits); with `window` > 0 a position
+        sees the newest `window` positions and the first `sinks` (`fmd_kv_options`)."""
+        fmt = {"act": _lib.KV_ACT, "q4": _lib.KV_Q4}.get(kv)
+        if fmt is None:
+            raise _lib.FmdError(_lib.FMD_EINVAL, f"kv must be 'act' or 'q4', not {kv!r}")
+        self._check(self.lib.fmd_kv_options(self._h, fmt, window, sinks))
         self._check(self.lib.fmd_kv_reserve(self._h, max_slots, max_tokens, max_rows))
         self.max_slots = max_slots
 
@@ -172,6 +179,18 @@ class Qwen3Decoder:
 
     def release_slot(self, slot: int) -> None:
         self._check(self.lib.fmd_slot_release(self._h, slot))
+
+    def fork_slot(self, src: int, dst: int, capacity: int) -> None:
+        """Open `dst` as a fork of `src` (`fmd_slot_fork`): hypotheses of one
+        prompt share its pages."""
+        self._check(self.lib.fmd_slot_fork(self._h, src, dst, capacity))
+
+    def compact_kv(self) -> int:
+        """Move the open slots' pages to the front of the pool (`fmd_kv_compact`);
+        returns how many are in use."""
+        n = C.c_int32()
+        self._check(self.lib.fmd_kv_compact(self._h, C.byref(n)))
+        return n.value
 
     def slot_len(self, slot: int) -> int:
         n = C.c_int32()

@@ -162,6 +162,19 @@ int fmd_version(void);
  * reference does (from the f32 value). Q8_0 sources are repacked as-is. */
 int fmd_load_weights(fmd_handle* h, const fmd_weights* w);
 
+/* What the KV pool holds and how much of it the attention reads; before
+ * fmd_kv_reserve, no reference counterpart (its cache is dense and fully read,
+ * qwen3.rs:33-108). `format`: FMD_KV_ACT (the activation dtype, the default) or
+ * FMD_KV_Q4 (4.5 bits a value, fmd_cache.h: 3.6 times the positions in the same
+ * memory, plus one layer of 16-bit staging). `window` > 0: a position p sees the
+ * positions j > p - window and, of the older ones, the first `sinks`. Positions
+ * keep their rotation. Steps with either option run their attention on the
+ * operators of fmd_cache.h; the persistent layer tail and split decode steps are
+ * off then. */
+#define FMD_KV_ACT 0
+#define FMD_KV_Q4 4
+int fmd_kv_options(fmd_handle* h, int32_t format, int32_t window, int32_t sinks);
+
 /* Replaces `Qwen3::new_caches` (qwen3.rs:415-428): reserves a paged KV pool of
  * `max_tokens_total` token positions shared by `max_slots` sequences, and work
  * buffers for up to `max_rows_per_step` token rows per forward pass. Returns
@@ -198,6 +211,15 @@ int fmd_splice_audio(fmd_handle* h, const int32_t* token_ids, int64_t n_ids, con
 int fmd_slot_open(fmd_handle* h, int32_t slot, int32_t capacity);
 /* Release a slot's pages (`KvCache::truncate(0)` + drop, qwen3.rs:105-107). */
 int fmd_slot_release(fmd_handle* h, int32_t slot);
+/* Open slot `dst` as a fork of `src` with room for `capacity` positions (at least
+ * src's length): full pages are shared, the rows behind them are copied in every
+ * layer. No reference counterpart. FMD_ENOMEM when the pool has too few free
+ * pages for the rest. */
+int fmd_slot_fork(fmd_handle* h, int32_t src, int32_t dst, int32_t capacity);
+/* Move the pages of the open slots to the front of the pool (the number in use
+ * goes to *n_used, which may be NULL): what they hold is then one range of each
+ * layer, for a snapshot of the pool. Not while an engine run is under way. */
+int fmd_kv_compact(fmd_handle* h, int32_t* n_used);
 /* Current cached length of a slot (`KvCache::len`, qwen3.rs:57-59). */
 int fmd_slot_len(fmd_handle* h, int32_t slot, int32_t* len);
 
