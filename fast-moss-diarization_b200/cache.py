@@ -284,7 +284,8 @@ class PagedCache:
         st = int(self._status[0].item())
         if st != 0:
             self._status.zero_()
-            raise _lib.FmdError(st, "a slot, position or page was out of range")
+            raise _lib.FmdError(st, "a device-side wait gave up" if st == _lib.FMD_ETIMEDOUT else
+                                "a slot, position or page was out of range")
 
     def _dtype(self, t, name: str) -> int:
         code = self._dtypes.get(t.dtype)

@@ -23,8 +23,8 @@
 //    O += P V (j - 1). One warp for both spent 3,350 cycles a key tile, most of them on
 //    its waits and commits one after another, for 1,400 cycles of products;
 //  * warps 4-7 / 8-11: the softmax of A / B, one thread per pair: a lazily moved
-//    reference m (2^8 of headroom), P as 16-bit values through shared memory, O in
-//    tensor memory, rescaled only when m moves;
+//    reference m (2^8 of headroom), P as 16-bit values over the scores it came from, the
+//    A operand of its product with V, O rescaled only when m moves;
 //  * 4 bits: warps 12-19 turn the codes into f16 tiles, (c - 8) d with one rounding,
 //    keys and values; the queries are then f16 too, scaled by a power of two per
 //    row.
@@ -46,7 +46,6 @@ namespace fmd {
 namespace {
 
 constexpr int kCkBox = 8192;       // 64 rows x 128 bytes
-constexpr int kCkPBytes = 16384;   // P: 128 pairs x 64 keys x 2 bytes
 constexpr int kCkMaxStages = 4;
 constexpr uint32_t kCkWait = 1u << 24;
 constexpr float kCkHeadroom = 8.f;
@@ -95,9 +94,62 @@ FMD_DEV uint64_t ck_desc_mn(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((kCkBox >> 4) & 0x3FFFu) << 16) |
          ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// N consecutive columns of this warp's 32 lanes, there when the statement ends. The
+// wait is part of it: between a load and a wait of their own the compiler could move or
+// spill registers that the load has not written yet.
+FMD_DEV void ck_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31"
+      "}, [%32];\n tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+FMD_DEV void ck_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, "
+      "%38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, "
+      "%56, %57, %58, %59, %60, %61, %62, %63"
+      "}, [%64];\n tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
+        "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+        "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] x B[smem], K = 16: A's rows are lanes, two 16-bit values a column.
+FMD_DEV void ck_umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
 FMD_DEV uint32_t ck_sub_mul(uint32_t a, uint32_t b, uint32_t d) {
   const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   const __half2 y = __hmul2(x, *reinterpret_cast<__half2*>(&d));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// What rounding a product of ck_sub_mul left out, (a - b) d - o: exact in f16, but for
+// what is below its subnormals.
+FMD_DEV uint32_t ck_sub_mul_rest(uint32_t a, uint32_t b, uint32_t d, uint32_t o) {
+  const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  const __half2 y = __hfma2(x, *reinterpret_cast<__half2*>(&d), __hneg2(*reinterpret_cast<__half2*>(&o)));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 
@@ -194,18 +246,22 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
   constexpr int TB = 64 * D * 2;                              // K or V of a page as an operand
   constexpr int NB = D / 32;
   constexpr int kMore = Q4 ? 152 : 208, kFew = Q4 ? 56 : 88;
+  // f16 outputs of a 4-bit cache: P and V go in as two f16 terms each (their roundings,
+  // 2^-11 each as the output's, would be two of the three that f16 operands cost;
+  // error against 64 bits 3.8e-4 without, 2.1e-4 for the output's rounding alone)
+  constexpr bool kFine = Q4 && !Act<T>::kIsBf16;
+  constexpr int CVB = (kFine ? 3 : 2) * TB;  // an operand buffer: K | V (| V's second term)
   constexpr float kPScale = Act<M>::kIsBf16 ? 0.f : 7.f;      // log2 factor of P (f16 subnormals start at 2^-14)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full[2], kv_full[kCkMaxStages], kv_empty[kCkMaxStages], cv_full[2][2], cv_empty[2][2],
-      s_full[2][2], s_empty[2][2], p_full[2], pv_done[2], o_final[2], o_empty[2], mma_done[2];
+      s_full[2][2], p_full[2][2], pv_done[2], o_final[2], o_empty[2], mma_done[2];
   __shared__ uint32_t tmem_s;
   __shared__ int abort_s, bad_s[kCkMaxStages], cbad_s[4], last_s;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t* qp = base;                      // Q_A | Q_B | P_A | P_B | stages | (4 bits) two operand tiles
-  uint8_t* pp = qp + 2 * QB;
-  uint8_t* kvp = pp + 2 * kCkPBytes;
+  uint8_t* qp = base;                      // Q_A | Q_B | stages | (4 bits) two operand tiles
+  uint8_t* kvp = qp + 2 * QB;
   uint8_t* cvp = kvp + p.stages * 2 * BLK;
   const int stages = p.stages, H = c.kv_heads;
   const int W = p.a.window, S = W ? p.a.sinks : 0;
@@ -227,9 +283,9 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
       mbar_init(&q_full[x], 4);
       for (int s = 0; s < 2; ++s) {
         mbar_init(&s_full[x][s], 1);
-        mbar_init(&s_empty[x][s], 4);
+        // one per buffer: a warp may be a tile ahead of its group, whose P(j) is not complete
+        mbar_init(&p_full[x][s], 4);
       }
-      mbar_init(&p_full[x], 4);
       mbar_init(&pv_done[x], 1);
       mbar_init(&o_final[x], 1);
       mbar_init(&o_empty[x], 4);
@@ -300,7 +356,9 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
     constexpr bool kBf = Act<M>::kIsBf16;
     constexpr uint32_t idesc_s = umma_idesc_f16(kBf, 128, 64);
     constexpr uint32_t idesc_o = umma_idesc_f16(kBf, 128, D) | (1u << 16);  // B (V) MN-major
-    int items = 0, sn = 0, pn = 0;
+    // scores and products issued; products known to be done: at most one is not, since
+    // the parity that pv_done is waited with tells one phase from the next, not from the one after
+    int items = 0, sn = 0, pn = 0, done = 0;
     int st = 0, ph = 0;  // operand tile of the next key tile: its stage (4 bits: buffer) and phase
     int prev_ph = 0;
     const int ring = Q4 ? 2 : stages;
@@ -311,7 +369,8 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
     const uint32_t s_tmem = tmem + x * 256, o_tmem = s_tmem + 128;
     // descriptors of the first operand tiles; addresses below 256 KB never carry out of
     // the address field, so the others are sums
-    const uint64_t dq = umma_desc_sw128(smem_u32(qp) + x * QB), dp = umma_desc_sw128(smem_u32(pp) + x * kCkPBytes);
+    const uint64_t dq = umma_desc_sw128(smem_u32(qp) + x * QB);
+    constexpr int SB = Q4 ? CVB : 2 * TB;  // bytes from tile to tile
     const uint64_t dk = umma_desc_sw128(smem_u32(tiles)), dv = ck_desc_mn(smem_u32(tiles) + TB);
     bool ok = true;
     CkWork w;
@@ -344,14 +403,18 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
                 __syncwarp();
               }
             }
+            const int sb = sn & 1;
             if (!got_q) {
               if (!(ok = ck_wait(&q_full[x], items & 1, abort_v))) break;
               got_q = true;
             }
-            const int sb = sn & 1;
-            if (sn >= 2 && !(ok = ck_wait(&s_empty[x][sb], ((sn >> 1) + 1) & 1, abort_v))) break;
+            // the buffer's last scores became a P whose product, the one two back, has to be done
+            if (done < sn - 1) {
+              if (!(ok = ck_wait(&pv_done[x], (pn - 1) & 1, abort_v))) break;
+              done = pn;
+            }
             tc_fence_after();
-            const uint64_t kd = dk + (uint64_t)(st * (2 * TB / 16));
+            const uint64_t kd = dk + (uint64_t)(st * (SB / 16));
             if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < D / 16; ++kk)
@@ -370,14 +433,25 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
           if (side.need(j - 1)) {
             // ---- O += P(j - 1) V
             if (!started && items >= 1 && !(ok = ck_wait(&o_empty[x], (items - 1) & 1, abort_v))) break;
-            if (!(ok = ck_wait(&p_full[x], pn & 1, abort_v))) break;
+            if (!(ok = ck_wait(&p_full[x][pn & 1], (pn >> 1) & 1, abort_v))) break;
             if (Q4 && !(ok = ck_wait(&cv_full[1][prev_st], prev_ph, abort_v))) break;
+            if (done < pn) {  // not in a row of needed tiles, where S(j) has waited for it
+              if (!(ok = ck_wait(&pv_done[x], (pn - 1) & 1, abort_v))) break;
+              done = pn;
+            }
             tc_fence_after();
-            const uint64_t vd = dv + (uint64_t)(prev_st * (2 * TB / 16));
+            const uint64_t vd = dv + (uint64_t)(prev_st * (SB / 16));
             if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk)
-                umma_f16(o_tmem, dp + kk * 32 / 16, vd + kk * 2048 / 16, idesc_o, started || kk != 0);
+                ck_umma_ts(o_tmem, s_tmem + (pn & 1) * 64 + kk * 8, vd + kk * 2048 / 16, idesc_o, started || kk != 0);
+              if constexpr (kFine) {
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                  ck_umma_ts(o_tmem, s_tmem + (pn & 1) * 64 + 32 + kk * 8, vd + kk * 2048 / 16, idesc_o, true);
+                  ck_umma_ts(o_tmem, s_tmem + (pn & 1) * 64 + kk * 8, vd + (TB + kk * 2048) / 16, idesc_o, true);
+                }
+              }
               umma_commit(&pv_done[x]);
               umma_commit(&empty[prev_st]);  // this warp's products have read the tile when it fires
             }
@@ -488,17 +562,12 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
         }
         tc_fence_after();
         float s[64];
+        {
+          uint32_t v[64];
+          ck_ld64(lane_addr + sb * 64, v);
 #pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2) {
-          uint32_t v[32];
-          tmem_ld32(lane_addr + sb * 64 + h2 * 32, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) s[h2 * 32 + i] = __uint_as_float(v[i]);
+          for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(v[i]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[x][sb]);
         ++sn;
         const bool bad = Q4 ? cbad_s[stage] : bad_s[stage];
         if (bad || k0 + 63 > pos || (W && k0 <= pos - W && k0 + 63 >= S)) {
@@ -528,8 +597,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
 #pragma unroll
           for (int h2 = 0; h2 < D / 32; ++h2) {
             uint32_t v[32];
-            tmem_ld32(o_addr + h2 * 32, v);
-            tmem_ld_wait();
+            ck_ld32(o_addr + h2 * 32, v);
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
             tmem_st32(o_addr + h2 * 32, v);
@@ -557,25 +625,24 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
           }
           l += ((a4[0].x + a4[0].y) + (a4[1].x + a4[1].y)) + ((a4[2].x + a4[2].y) + (a4[3].x + a4[3].y));
         }
-        // the P buffer was last read by the previous P V of this tile
-        if (pn >= 1 && !wwait(&pv_done[x], (pn - 1) & 1)) {
-          ok = false;
-          break;
-        }
-        uint8_t* prow = pp + x * kCkPBytes + row * 128;
+        {
+          uint32_t v[32];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint4 v;
-          v.x = Act<M>::pack2(s[8 * i + 0], s[8 * i + 1]);
-          v.y = Act<M>::pack2(s[8 * i + 2], s[8 * i + 3]);
-          v.z = Act<M>::pack2(s[8 * i + 4], s[8 * i + 5]);
-          v.w = Act<M>::pack2(s[8 * i + 6], s[8 * i + 7]);
-          *reinterpret_cast<uint4*>(prow + ((i ^ (row & 7)) << 4)) = v;
+          for (int i = 0; i < 32; ++i) v[i] = Act<M>::pack2(s[2 * i], s[2 * i + 1]);
+          tmem_st32(lane_addr + sb * 64, v);
+          if constexpr (kFine) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float2 f = Act<M>::unpack2(v[i]);
+              v[i] = Act<M>::pack2(s[2 * i] - f.x, s[2 * i + 1] - f.y);
+            }
+            tmem_st32(lane_addr + sb * 64 + 32, v);
+          }
+          tmem_st_wait();
         }
-        ck_fence_async();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
+        if (lane == 0) mbar_arrive(&p_full[x][sb]);
         ++pn;
         first = false;
       }
@@ -595,8 +662,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
 #pragma unroll
         for (int h2 = 0; h2 < D / 32; ++h2) {
           uint32_t v[32];
-          tmem_ld32(o_addr + h2 * 32, v);
-          tmem_ld_wait();
+          ck_ld32(o_addr + h2 * 32, v);
           if (!live) {
           } else if (pt) {
 #pragma unroll
@@ -687,7 +753,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
           break;
         }
         const uint8_t* src = kvp + s * 2 * BLK;
-        uint8_t* dst = cvp + b * 2 * TB;
+        uint8_t* dst = cvp + b * CVB;
         const bool bad = bad_s[s];
         if (tid == 12 * 32) cbad_s[(round_b * 2 + b) & 3] = bad;
         // 8 keys per warp; a lane takes chunk lane & 3 of a key, keys 4 apart in a
@@ -746,13 +812,18 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
         for (int g = 0; g < NB; ++g) {
           // nibbles 2 i, 2 i + 1 side by side: bytes of the even and the odd ones interleaved
           const uint32_t ev = (wd[g] << 4) & 0xf0f0f0f0u, od = wd[g] & 0xf0f0f0f0u;
-          uint4 o;
-          o.x = ck_sub_mul((__byte_perm(ev, od, 0x0400) & 0x00ff00ffu) | f64, k72, dv);
-          o.y = ck_sub_mul((__byte_perm(ev, od, 0x0501) & 0x00ff00ffu) | f64, k72, dv);
-          o.z = ck_sub_mul((__byte_perm(ev, od, 0x0602) & 0x00ff00ffu) | f64, k72, dv);
-          o.w = ck_sub_mul((__byte_perm(ev, od, 0x0703) & 0x00ff00ffu) | f64, k72, dv);
+          const uint32_t c4[4] = {__byte_perm(ev, od, 0x0400), __byte_perm(ev, od, 0x0501), __byte_perm(ev, od, 0x0602),
+                                  __byte_perm(ev, od, 0x0703)};
+          uint32_t o[4], rest[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            o[i] = ck_sub_mul((c4[i] & 0x00ff00ffu) | f64, k72, dv);
+            if constexpr (kFine) rest[i] = ck_sub_mul_rest((c4[i] & 0x00ff00ffu) | f64, k72, dv, o[i]);
+          }
           const int oc = NB * ch + g;
-          *reinterpret_cast<uint4*>(dst + TB + (oc >> 3) * kCkBox + key * 128 + (((oc & 7) ^ (key & 7)) << 4)) = o;
+          uint8_t* at = dst + TB + (oc >> 3) * kCkBox + key * 128 + (((oc & 7) ^ (key & 7)) << 4);
+          *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
+          if constexpr (kFine) *reinterpret_cast<uint4*>(at + TB) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
         }
         ck_fence_async();
         __syncwarp();
@@ -779,7 +850,7 @@ struct CkShape {
 };
 
 // Parts of an item: enough for every SM when there are fewer items than SMs.
-CkShape ck_shape(const CacheView& c, int n_heads, int n_seqs, int max_rows) {
+CkShape ck_shape(bool bf16, const CacheView& c, int n_heads, int n_seqs, int max_rows) {
   CkShape s;
   const long long pairs = (long long)max_rows * (n_heads / c.kv_heads);
   s.tiles = (int)((pairs + 255) / 256);
@@ -789,8 +860,8 @@ CkShape ck_shape(const CacheView& c, int n_heads, int n_seqs, int max_rows) {
   s.grid = (int)std::min<long long>(148, s.items * s.parts);
   const bool q4 = c.format == FMD_CACHE_Q4;
   const int tb = 64 * c.head_dim * 2, stage = 2 * (int)c.block_bytes();
-  s.stages = q4 ? 4 : 3;
-  s.smem = 1024 + 2 * 128 * c.head_dim * 2 + 2 * kCkPBytes + s.stages * stage + (q4 ? 2 * 2 * tb : 0);
+  s.stages = 4;
+  s.smem = 1024 + 2 * 128 * c.head_dim * 2 + s.stages * stage + (q4 ? 2 * (bf16 ? 2 : 3) * tb : 0);
   return s;
 }
 
@@ -798,7 +869,7 @@ CkShape ck_shape(const CacheView& c, int n_heads, int n_seqs, int max_rows) {
 
 // counters, then the parts
 size_t cache_chunk_workspace(const CacheView& c, int n_heads, int n_seqs, int max_rows) {
-  const CkShape s = ck_shape(c, n_heads, n_seqs, max_rows);
+  const CkShape s = ck_shape(true, c, n_heads, n_seqs, max_rows);
   if (s.parts == 1) return 0;
   return FMD_CACHE_WORKSPACE_ZERO + (size_t)s.items * s.parts * 256 * (c.head_dim + 2) * 4;
 }
@@ -806,7 +877,7 @@ size_t cache_chunk_workspace(const CacheView& c, int n_heads, int n_seqs, int ma
 cudaError_t launch_cache_chunk(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAttend& a,
                                void* workspace, int* status, cudaStream_t s) {
   const bool q4 = c.format == FMD_CACHE_Q4;
-  const CkShape sh = ck_shape(c, a.n_heads, r.n_seqs, a.max_rows);
+  const CkShape sh = ck_shape(bf16, c, a.n_heads, r.n_seqs, a.max_rows);
   CUtensorMap map{};
   if (!q4 && !cache_tensor_map(&map, c, layer)) return cudaErrorNotSupported;
   CkArgs p;

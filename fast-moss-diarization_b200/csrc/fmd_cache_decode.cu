@@ -583,7 +583,8 @@ __global__ void __launch_bounds__(kDc16Threads, 2)
 // which keeps what is 2^-24 of the row's largest.
 // Values: f16 pairs 64 + c by one shift and one and-or (mantissa bits 4-7), then
 // (c - 8) d in f16 (one rounding, 2^-11): the scale differs by key, which is
-// the sum's index there.
+// the sum's index there. With f16 outputs, whose own rounding is no larger, P goes in
+// as two terms (error against 64 bits 2.7e-4 instead of 3.4e-4; the output's 2.1e-4).
 
 constexpr int kDq4Threads = 128;
 
@@ -619,6 +620,7 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
   constexpr int CB = K * D / 2, SB = K * D / 16;  // its code and scale bytes
   constexpr int UB = 2 * (CB + SB);
   constexpr int U = 2;                        // 16-key steps
+  constexpr bool kHiLo = !Act<T>::kIsBf16;    // f16 outputs: P as two f16 terms (see below)
 
   extern __shared__ __align__(128) uint8_t smem[];
   float* red = reinterpret_cast<float*>(smem + p.red_off);
@@ -838,8 +840,8 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
             }
           }
         }
-        uint32_t pb[NT][U][2], pl[1][U][2], vis[U][2];
-        dc_softmax<__half, U, MT, NT, false>(sc, sl, m, l, o, pb, pl, vis, whole, k0, p0, p1, W, S, gs, 7.f);
+        uint32_t pb[NT][U][2], pl[kHiLo ? NT : 1][U][2], vis[U][2];
+        dc_softmax<__half, U, MT, NT, kHiLo>(sc, sl, m, l, o, pb, pl, vis, whole, k0, p0, p1, W, S, gs, 7.f);
         // O^T += V^T P^T; this thread's keys: kb, kb + 1, kb + 8, kb + 9
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -882,6 +884,10 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
               for (int n = 0; n < NT; ++n) {
                 mma16816<__half>(o[n][i * 4 + hf * 2], a0, pb[n][u][0], pb[n][u][1]);
                 mma16816<__half>(o[n][i * 4 + hf * 2 + 1], a1, pb[n][u][0], pb[n][u][1]);
+                if constexpr (kHiLo) {
+                  mma16816<__half>(o[n][i * 4 + hf * 2], a0, pl[n][u][0], pl[n][u][1]);
+                  mma16816<__half>(o[n][i * 4 + hf * 2 + 1], a1, pl[n][u][0], pl[n][u][1]);
+                }
               }
             }
         }

@@ -247,6 +247,31 @@ def test_attend_many_sequences(kind):
     _check_attend(c, held, kind, "bf16", [1] * 300, lengths, 2, 33, 2)
 
 
+@pytest.mark.parametrize("kind,dtype", [("bf16", "bf16"), ("f16", "f16"), ("q4", "bf16"), ("q4", "f16")])
+@pytest.mark.parametrize("dim,group", [(64, 2), (128, 1)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 3), (300, 70)])
+def test_attend_many_chunk_items_per_block(kind, dtype, dim, group, window, sinks):
+    """More (tile, sequence, head) items than blocks: every block goes through
+    several, of odd and even numbers of key tiles, some with one half empty."""
+    counts = [900, 130, 1, 640, 257, 700, 64, 513]
+    lengths = [n + 37 * i for i, n in enumerate(counts)]
+    c, held = _filled(kind, dtype, lengths, dim, 8, seed=21)
+    q = _rand(np.random.default_rng(5), sum(counts), 8 * group, dim, dtype=dtype)
+    rows = _seq_rows(c, list(range(8)), counts, lengths)
+    out = c.attend(0, rows, q, window=window, sinks=sinks)
+    c.check()
+    for _ in range(5):
+        assert torch.equal(out, c.attend(0, rows, q, window=window, sinks=sinks))
+    at = 0
+    for s, (n, end) in enumerate(zip(counts, lengths)):
+        for i in sorted({0, n // 2, max(0, n - 70), n - 1}):
+            want, mag = ref.attend(_np(q[at + i:at + i + 1]), *held[s], [end - n + i], window, sinks)
+            tol = ref.attend_tolerance(want, mag, _eps(dtype), kind == "q4")
+            assert (np.abs(_np(out[at + i:at + i + 1]) - want) <= tol).all(), (s, i)
+        at += n
+    c.check()
+
+
 @pytest.mark.parametrize("kind,dtype", [("bf16", "bf16"), ("f16", "f16"), ("q4", "bf16")])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("count", [1, 4])
