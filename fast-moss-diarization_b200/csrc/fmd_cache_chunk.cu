@@ -13,9 +13,11 @@
 // query heads of the kv head) of one sequence and kv head: each key tile (a page)
 // is read once for both. Its key tiles are those of the sinks, then those from
 // A's oldest window to B's newest row; a tile that one of A, B does not see is
-// skipped for it. With fewer items than SMs an item's key tiles are split into
-// parts, whose (m, l, o) go through the workspace; the last part to finish
-// merges them in order. Items go out latest rows first, dealt in turn.
+// skipped for it. Items are dealt in turn, or, where that would leave blocks idle for
+// longer (few items, or items of very different lengths), the items' key tiles form one
+// sequence, of which every block takes an equal range: an item cut by a range's end
+// leaves (m, l, o) partials in the workspace, and the last of its blocks to finish
+// merges them in order.
 //
 //  * warp 0: copies of the page tiles into a ring (16 bits: 2D TMA with the
 //    128-byte swizzle; 4 bits: bulk copies of the blocks);
@@ -59,10 +61,12 @@ template <int N> FMD_DEV void ck_fewer_regs() { asm volatile("setmaxnreg.dec.syn
 struct CkArgs {
   CacheRows r;
   CacheAttend a;
-  float* part;    // [items][parts][256][D + 2]
-  int* counters;  // [items], zero between calls
+  // partials of cut items: o as [2 x blocks][D / 4][256 pairs] of four dims, so that a warp's
+  // threads, a pair each, write and read runs; then [2 x blocks][256] (m, l)
+  float* part;
+  int* counters;  // [(sequence, tile)][kv heads], zero between calls
   int tiles;      // 256-pair tiles of the longest sequence
-  int parts, stages;
+  int split, stages;  // split: items may be cut
   uint32_t f64;   // f16 pair (64, 64)
 };
 
@@ -161,7 +165,9 @@ struct CkWork {
   int lo[2], hi[2];        // positions of their first and last row
   int sinks, w0;           // the item's key tiles: sinks, then from w0
   int lim, from[2], end[2];  // those A / B see: before lim, or from from[x] on, before end[x]
-  int j0, j1, item, part;
+  int j0, j1, item, units;
+  bool inside;      // the whole item is this work
+  long long start;  // else: the item's first unit, for its other blocks
   FMD_DEV int tile(int j) const { return j < sinks ? j : w0 + j - sinks; }
 };
 // What concerns one of A, B, in registers of its own (a run-time index into
@@ -190,19 +196,9 @@ FMD_DEV bool ck_wait(uint64_t* bar, uint32_t parity, volatile int* abort_v) {
   return __all_sync(0xffffffffu, ok);
 }
 
-// Work of round r of this CTA: 1 a work, 0 none (skip), -1 no more.
-FMD_DEV int ck_work(const CkArgs& p, const CacheView& c, int round, CkWork& w, int* status) {
-  const int H = c.kv_heads, G = gridDim.x;
-  const int ns = p.r.count();
-  const long long total = (long long)p.tiles * ns * H * p.parts;
-  const long long at = (long long)round * G + ((round & 1) ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);
-  if ((long long)round * G >= total) return -1;
-  if (at >= total) return 0;
-  w.part = (int)(at % p.parts);
-  const long long item = at / p.parts;
-  w.item = (int)item;
-  w.h = (int)(item % H);
-  const int seq = ns - 1 - (int)(item / H % ns), tile = p.tiles - 1 - (int)(item / H / ns);
+// Item (seq, tile) without its kv head and key range: its number of key tiles, 0 if
+// there is none.
+FMD_DEV int ck_item(const CkArgs& p, const CacheView& c, int seq, int tile, CkWork& w, int* status) {
   int n;
   p.r.get(seq, w.slot, w.p0, w.r0, n);
   if (n <= 0 || !cache_slot_ok(c, w.slot, status)) return 0;
@@ -210,7 +206,7 @@ FMD_DEV int ck_work(const CkArgs& p, const CacheView& c, int round, CkWork& w, i
     cache_report(status, n > p.a.max_rows ? FMD_EINVAL : FMD_EOVERFLOW);
     return 0;
   }
-  const int gs = __ffs(p.a.n_heads / H) - 1;
+  const int gs = __ffs(p.a.n_heads / c.kv_heads) - 1;
   const long long pairs = (long long)n << gs;
   const long long f = (long long)tile * 256;
   if (f >= pairs) return 0;
@@ -225,16 +221,90 @@ FMD_DEV int ck_work(const CkArgs& p, const CacheView& c, int round, CkWork& w, i
   const int oldest = W && w.lo[0] >= W ? w.lo[0] - W + 1 : 0;
   w.w0 = oldest / kPageTokens;
   w.sinks = (min(S, w.w0 * kPageTokens) + kPageTokens - 1) / kPageTokens;
-  const int T = w.sinks + (w.count[1] > 0 ? w.hi[1] : w.hi[0]) / kPageTokens - w.w0 + 1;
   w.lim = w.sinks + max(0, (min(S, w.hi[1]) + kPageTokens - 1) / kPageTokens - w.w0);
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     w.from[x] = w.sinks + (W && w.lo[x] >= W ? w.lo[x] - W + 1 : 0) / kPageTokens - w.w0;
     w.end[x] = w.count[x] > 0 ? w.sinks + w.hi[x] / kPageTokens - w.w0 + 1 : 0;
   }
-  w.j0 = (int)((long long)T * w.part / p.parts);
-  w.j1 = (int)((long long)T * (w.part + 1) / p.parts);
-  return 1;
+  return w.sinks + (w.count[1] > 0 ? w.hi[1] : w.hi[0]) / kPageTokens - w.w0 + 1;
+}
+
+constexpr int kCkEntries = 1024;  // (sequence, tile) pairs of a split launch at most
+// Units of an item beside its key tiles: what its queries, its first scores and its
+// output cost, about two tiles.
+constexpr int kCkSetup = 2;
+constexpr int kCkLeast = 6;       // units of a range at least
+// What cutting costs a block, in units of about 1.2 us: the partials' way through memory
+// and the merge. 256 items of 70 units (two rounds of 148 blocks, 17 % of them idle) took
+// 175 us whole and 173 cut, 64 items of 72 units 90 us whole and 68 cut, 128 items of 3 to
+// 35 units 49 us whole and 55 cut.
+constexpr int kCkCut = 24;
+
+// This block's range of units, and the units before each (sequence, tile).
+struct CkPlan {
+  int prefix[kCkEntries + 1];
+};
+struct CkRange {
+  long long x0, x1, total;  // of units; whole items: total counts them
+  int G;                    // blocks with a range
+  bool whole;
+};
+struct CkIter {
+  long long x;
+  int round = 0;
+};
+
+// The block's next work: 1 a work, 0 none (skip), -1 no more.
+FMD_DEV int ck_next(const CkArgs& p, const CacheView& c, const CkPlan& plan, const CkRange& g, CkIter& it, CkWork& w) {
+  const int H = c.kv_heads, ns = p.r.count();
+  if (p.split) {
+    if (g.whole) {
+      // the last pairs (the latest rows of a prompt) first, every other round the other way round
+      const long long G = gridDim.x;
+      if (it.round * G >= g.total) return -1;
+      it.x = g.total - 1 - (it.round * G + ((it.round & 1) ? G - 1 - blockIdx.x : blockIdx.x));
+      ++it.round;
+      if (it.x < 0) return 0;
+    } else if (it.x >= g.x1) {
+      return -1;
+    }
+    int lo = 0, hi = ns * p.tiles - 1;  // the last pair with units that starts at or before x
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((long long)H * plan.prefix[mid] <= it.x) lo = mid;
+      else hi = mid - 1;
+    }
+    w.units = plan.prefix[lo + 1] - plan.prefix[lo];
+    const int off = (int)(it.x - (long long)H * plan.prefix[lo]);
+    w.h = off / w.units;
+    w.item = lo * H + w.h;
+    if (g.whole) {
+      w.j0 = 0;
+      w.j1 = ck_item(p, c, lo / p.tiles, lo % p.tiles, w, nullptr);
+      w.inside = true;
+      return 1;
+    }
+    const int j = off - w.h * w.units, len = (int)min((long long)(w.units - j), g.x1 - it.x);
+    ck_item(p, c, lo / p.tiles, lo % p.tiles, w, nullptr);
+    w.j0 = max(j - kCkSetup, 0);
+    w.j1 = max(j + len - kCkSetup, 0);
+    w.inside = len == w.units;
+    w.start = it.x - j;
+    it.x += len;
+    return 1;
+  }
+  // latest rows first, every other round the other way round
+  const long long G = gridDim.x, total = (long long)p.tiles * ns * H;
+  const long long at = it.round * G + ((it.round & 1) ? G - 1 - blockIdx.x : blockIdx.x);
+  if (it.round * G >= total) return -1;
+  ++it.round;
+  if (at >= total) return 0;
+  w.h = (int)(at % H);
+  w.j0 = 0;
+  w.j1 = ck_item(p, c, ns - 1 - (int)(at / H % ns), p.tiles - 1 - (int)(at / H / ns), w, nullptr);
+  w.inside = true;
+  return w.j1 > 0;
 }
 
 template <typename T, int D, bool Q4>
@@ -257,6 +327,8 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
       s_full[2][2], p_full[2][2], pv_done[2], o_final[2], o_empty[2], mma_done[2];
   __shared__ uint32_t tmem_s;
   __shared__ int abort_s, bad_s[kCkMaxStages], cbad_s[4], last_s;
+  __shared__ CkPlan plan;
+  __shared__ CkRange range;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -297,9 +369,64 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
     tmem_alloc(&tmem_s, 512);
     tmem_relinquish();
   }
+  CkIter it;
+  const int entries = p.r.count() * p.tiles;
+  if (p.split) {
+    for (int e = tid; e < entries; e += ck_threads(Q4)) {
+      CkWork w;
+      const int n = ck_item(p, c, e / p.tiles, e % p.tiles, w, status);
+      plan.prefix[e] = n > 0 ? n + kCkSetup : 0;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      // each lane a run of pairs
+      const int per = (entries + 31) / 32, e0 = min(lane * per, entries), e1 = min(e0 + per, entries);
+      int sum = 0, have = 0, most = 0;
+      for (int e = e0; e < e1; ++e) {
+        const int v = plan.prefix[e];
+        sum += v;
+        have += v > 0;
+        most = max(most, v);
+      }
+      const long long units = (long long)H * __reduce_add_sync(0xffffffffu, (unsigned)sum);
+      const int items = H * (int)__reduce_add_sync(0xffffffffu, (unsigned)have), G = gridDim.x;
+      most = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
+      // whole items: the longest, or as many rounds of average ones; cut ones: an equal share
+      const bool whole = items > 0 && max((long long)most, (items + G - 1) / G * (units / items)) <= units / G + kCkCut;
+      if (whole) sum = have;
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      int run = incl - sum;
+      for (int e = e0; e < e1; ++e) {
+        const int v = whole ? plan.prefix[e] > 0 : plan.prefix[e];
+        plan.prefix[e] = run;
+        run += v;
+      }
+      if (lane == 31) {
+        plan.prefix[entries] = incl;
+        range.whole = whole;
+        range.total = (long long)H * incl;
+        range.G = (int)max(1LL, min((long long)G, range.total / kCkLeast));
+        const bool has = (int)blockIdx.x < range.G;
+        range.x0 = has ? (long long)blockIdx.x * range.total / range.G : 0;
+        range.x1 = has ? (long long)(blockIdx.x + 1) * range.total / range.G : 0;
+      }
+    }
+  } else if (blockIdx.x == 0) {
+    // bad slots and positions are reported once
+    for (int e = tid; e < entries; e += ck_threads(Q4)) {
+      CkWork w;
+      ck_item(p, c, e / p.tiles, e % p.tiles, w, status);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  it.x = p.split ? range.x0 : 0;
   const uint32_t tmem = tmem_s;
   volatile int* abort_v = &abort_s;
 
@@ -312,7 +439,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
       int issued = 0, s = 0, round_s = 0;
       bool ok = true;
       CkWork w;
-      for (int r = 0, k; ok && (k = ck_work(p, c, r, w, status)) >= 0; ++r) {
+      for (int k; ok && (k = ck_next(p, c, plan, range, it, w)) >= 0;) {
         if (k == 0) continue;
         const int* table = c.page_table + (size_t)w.slot * c.max_pages;
         for (int j = w.j0; j < w.j1; ++j) {
@@ -374,7 +501,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
     const uint64_t dk = umma_desc_sw128(smem_u32(tiles)), dv = ck_desc_mn(smem_u32(tiles) + TB);
     bool ok = true;
     CkWork w;
-    for (int r = 0, k; ok && (k = ck_work(p, c, r, w, nullptr)) >= 0; ++r) {
+    for (int k; ok && (k = ck_next(p, c, plan, range, it, w)) >= 0;) {
       if (k == 0) continue;
       const CkSide side(w, x);
       const int top = w.count[1] > 0 ? w.hi[1] : w.hi[0], low = w.lo[0];
@@ -497,8 +624,8 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
     int cb = 0;
     const int ring = Q4 ? 4 : stages;
     CkWork w;
-    // a warp whose wait gave up goes on without work: the parts' barriers below count every warp
-    for (int r = 0, kd; (ok || p.parts > 1) && (kd = ck_work(p, c, r, w, nullptr)) >= 0; ++r) {
+    // a warp whose wait gave up goes on without work: the merge's barriers below count every warp
+    for (int kd; (ok || p.split) && (kd = ck_next(p, c, plan, range, it, w)) >= 0;) {
       if (kd == 0) continue;
       const CkSide side(w, x);
       bool any = false;
@@ -654,7 +781,11 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
         any = false;
         *abort_v = 1;
       }
-      float* pt = p.parts > 1 ? p.part + (((size_t)w.item * p.parts + w.part) * 256 + x * 128 + row) * (D + 2) : nullptr;
+      // a cut item's partial: slot 2 c holds an item that began in an earlier block, 2 c + 1 one
+      // that goes on in a later one
+      float2* ml = reinterpret_cast<float2*>(p.part + (size_t)2 * gridDim.x * 256 * D);
+      const size_t pslot = 2 * blockIdx.x + (w.start < range.x0 ? 0 : 1);
+      float4* pt = w.inside ? nullptr : reinterpret_cast<float4*>(p.part) + pslot * (D / 4) * 256 + x * 128 + row;
       const float inv = 1.f / l;
       T* dst = (T*)p.a.out + (size_t)(w.r0 + (pr >> gs)) * p.a.out_row +
                (size_t)((w.h << gs) + (pr & ((1 << gs) - 1))) * p.a.out_head;
@@ -666,8 +797,9 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
           if (!live) {
           } else if (pt) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 2)
-              *reinterpret_cast<float2*>(pt + h2 * 32 + i) = make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(pt + (h2 * 8 + i) * 256) =
+                  make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -686,12 +818,14 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
         ++items;
       }
       if (pt) {
-        if (live) *reinterpret_cast<float2*>(pt + D) = make_float2(m_ref, l);
-        // the last part of the item merges all, one warp per pair
+        if (live) ml[pslot * 256 + x * 128 + row] = make_float2(m_ref, l);
+        // the last block of the item to get here merges all, a thread its pair
+        auto block_of = [&](long long u) { return (int)(((u + 1) * range.G - 1) / range.total); };
+        const int cf = block_of(w.start), np = block_of(w.start + w.units - 1) - cf + 1;
         named_sync(1, 256);
         if (tid == 128) {
           __threadfence();
-          last_s = atomicAdd(&p.counters[w.item], 1) == p.parts - 1;
+          last_s = atomicAdd(&p.counters[w.item], 1) == np - 1;
           if (last_s) {
             __threadfence();
             p.counters[w.item] = 0;
@@ -700,34 +834,46 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
         named_sync(1, 256);
         const bool last = last_s;
         if (last) {
-          const float* all = p.part + (size_t)w.item * p.parts * 256 * (D + 2);
-          for (int k = warp - 4; k < w.count[0] + w.count[1]; k += 8) {
-            auto at = [&](int sp) { return all + ((size_t)sp * 256 + k) * (D + 2); };
-            float Mx = -INFINITY;
-            for (int sp = 0; sp < p.parts; ++sp) Mx = fmaxf(Mx, __ldcg(at(sp) + D));
-            const float b = Mx == -INFINITY ? 0.f : Mx;
-            float L = 0.f;
-            float2 acc[D / 64];
+          auto at = [&](int sp) { return (size_t)(2 * (cf + sp) + (sp == 0 ? 1 : 0)); };
+          const int k = x * 128 + row;
+          float Mx = -INFINITY, L = 0.f;
+#pragma unroll 4
+          for (int sp = 0; sp < np; ++sp)
+            if (live) Mx = fmaxf(Mx, __ldcg(&ml[at(sp) * 256 + k]).x);
+          const float b = Mx == -INFINITY ? 0.f : Mx;
+          constexpr int C = Q4 ? 8 : 16;  // float4s at a time: their loads are in flight together
+          for (int c0 = 0; c0 < D / 4 && live; c0 += C) {
+            float4 acc[C];
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) acc[i] = make_float2(0.f, 0.f);
-            for (int sp = 0; sp < p.parts; ++sp) {
-              const float lw = __ldcg(at(sp) + D + 1);
-              if (lw == 0.f) continue;  // the part saw none of the pair's keys
-              const float f = ck_ex2(__ldcg(at(sp) + D) - b);
-              L = fmaf(lw, f, L);
+            for (int i = 0; i < C; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            L = 0.f;
+            for (int sp = 0; sp < np; ++sp) {
+              const float2 v = __ldcg(&ml[at(sp) * 256 + k]);
+              if (v.y == 0.f) continue;  // the part saw none of the pair's keys and left its row alone
+              const float4* src = reinterpret_cast<const float4*>(p.part) + (at(sp) * (D / 4) + c0) * 256 + k;
+              float4 u[C];
 #pragma unroll
-              for (int i = 0; i < D / 64; ++i) {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(at(sp) + i * 64 + lane * 2));
-                acc[i].x = fmaf(v.x, f, acc[i].x);
-                acc[i].y = fmaf(v.y, f, acc[i].y);
+              for (int i = 0; i < C; ++i) u[i] = __ldcg(src + i * 256);
+              const float f = ck_ex2(v.x - b);
+              L = fmaf(v.y, f, L);
+#pragma unroll
+              for (int i = 0; i < C; ++i) {
+                acc[i].x = fmaf(u[i].x, f, acc[i].x);
+                acc[i].y = fmaf(u[i].y, f, acc[i].y);
+                acc[i].z = fmaf(u[i].z, f, acc[i].z);
+                acc[i].w = fmaf(u[i].w, f, acc[i].w);
               }
             }
-            const int pk = w.first[0] + k;
-            T* o = (T*)p.a.out + (size_t)(w.r0 + (pk >> gs)) * p.a.out_row +
-                   (size_t)((w.h << gs) + (pk & ((1 << gs) - 1))) * p.a.out_head;
+            const float r = 1.f / L;
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i)
-              *reinterpret_cast<uint32_t*>(o + i * 64 + lane * 2) = Act<T>::pack2(acc[i].x / L, acc[i].y / L);
+            for (int i = 0; i < C; i += 2) {
+              uint4 y;
+              y.x = Act<T>::pack2(acc[i].x * r, acc[i].y * r);
+              y.y = Act<T>::pack2(acc[i].z * r, acc[i].w * r);
+              y.z = Act<T>::pack2(acc[i + 1].x * r, acc[i + 1].y * r);
+              y.w = Act<T>::pack2(acc[i + 1].z * r, acc[i + 1].w * r);
+              *reinterpret_cast<uint4*>(dst + (c0 + i) * 4) = y;
+            }
           }
         }
       }
@@ -742,7 +888,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
     bool ok = true;
     const uint32_t f64 = p.f64, k72 = 0x54805480u;  // f16 64, 72
     CkWork w;
-    for (int r = 0, k; ok && (k = ck_work(p, c, r, w, nullptr)) >= 0; ++r) {
+    for (int k; ok && (k = ck_next(p, c, plan, range, it, w)) >= 0;) {
       if (k == 0) continue;
       const int top = w.count[1] > 0 ? w.hi[1] : w.hi[0];
       for (int j = w.j0; j < w.j1; ++j) {
@@ -845,19 +991,15 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
 }
 
 struct CkShape {
-  int tiles, parts, stages, grid, smem;
-  long long items;
+  int tiles, split, stages, smem;
 };
 
-// Parts of an item: enough for every SM when there are fewer items than SMs.
 CkShape ck_shape(bool bf16, const CacheView& c, int n_heads, int n_seqs, int max_rows) {
   CkShape s;
   const long long pairs = (long long)max_rows * (n_heads / c.kv_heads);
   s.tiles = (int)((pairs + 255) / 256);
-  s.items = (long long)s.tiles * n_seqs * c.kv_heads;
-  s.parts = s.items >= 148 ? 1 : (int)(148 / s.items);
-  s.parts = std::min(s.parts, std::max(1, std::min(32, c.max_pages / 4)));
-  s.grid = (int)std::min<long long>(148, s.items * s.parts);
+  const long long entries = (long long)s.tiles * n_seqs;
+  s.split = entries <= kCkEntries && entries * c.kv_heads <= FMD_CACHE_WORKSPACE_ZERO / 4;
   const bool q4 = c.format == FMD_CACHE_Q4;
   const int tb = 64 * c.head_dim * 2, stage = 2 * (int)c.block_bytes();
   s.stages = 4;
@@ -865,13 +1007,14 @@ CkShape ck_shape(bool bf16, const CacheView& c, int n_heads, int n_seqs, int max
   return s;
 }
 
+constexpr int kCkGrid = 148;
+
 }  // namespace
 
-// counters, then the parts
+// counters, then the partials of cut items
 size_t cache_chunk_workspace(const CacheView& c, int n_heads, int n_seqs, int max_rows) {
-  const CkShape s = ck_shape(true, c, n_heads, n_seqs, max_rows);
-  if (s.parts == 1) return 0;
-  return FMD_CACHE_WORKSPACE_ZERO + (size_t)s.items * s.parts * 256 * (c.head_dim + 2) * 4;
+  if (!ck_shape(true, c, n_heads, n_seqs, max_rows).split) return 0;
+  return FMD_CACHE_WORKSPACE_ZERO + (size_t)2 * kCkGrid * 256 * (c.head_dim + 2) * 4;
 }
 
 cudaError_t launch_cache_chunk(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAttend& a,
@@ -886,7 +1029,7 @@ cudaError_t launch_cache_chunk(bool bf16, const CacheView& c, int layer, const C
   p.counters = (int*)workspace;
   p.part = (float*)((uint8_t*)workspace + FMD_CACHE_WORKSPACE_ZERO);
   p.tiles = sh.tiles;
-  p.parts = sh.parts;
+  p.split = sh.split;
   p.stages = sh.stages;
   p.f64 = 0x54005400u;
   auto go = [&](auto kern) -> cudaError_t {
@@ -896,7 +1039,7 @@ cudaError_t launch_cache_chunk(bool bf16, const CacheView& c, int layer, const C
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sh.grid);
+    cfg.gridDim = dim3(kCkGrid);
     cfg.blockDim = dim3(ck_threads(q4));
     cfg.dynamicSmemBytes = sh.smem;
     cfg.stream = s;

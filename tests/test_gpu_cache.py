@@ -241,6 +241,26 @@ def test_attend_one_long_sequence(kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "q4"])
+def test_attend_many_sequences_of_several_rows(kind):
+    """So many (sequence, tile) pairs that items are dealt out whole."""
+    counts = [40 - i % 9 for i in range(300)]
+    lengths = [n + (37 * i) % 150 for i, n in enumerate(counts)]
+    c, held = _filled(kind, "bf16", lengths, 64, 1, seed=4)
+    counts[17] = 0
+    q = _rand(np.random.default_rng(5), sum(counts), 16, 64)
+    out = c.attend(0, _seq_rows(c, list(range(300)), counts, lengths, max_rows=65), q, window=33, sinks=2)
+    c.check()
+    assert torch.equal(out, c.attend(0, _seq_rows(c, list(range(300)), counts, lengths, max_rows=65), q, window=33,
+                                     sinks=2))
+    at = 0
+    for s, (n, end) in enumerate(zip(counts, lengths)):
+        if s % 7 == 3 and n:
+            want, mag = ref.attend(_np(q[at:at + n]), *held[s], range(end - n, end), 33, 2)
+            assert (np.abs(_np(out[at:at + n]) - want) <= ref.attend_tolerance(want, mag, _eps("bf16"), kind == "q4")).all()
+        at += n
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
 def test_attend_many_sequences(kind):
     lengths = [1 + (37 * i) % 150 for i in range(300)]
     c, held = _filled(kind, "bf16", lengths, 64, 1, seed=4)
