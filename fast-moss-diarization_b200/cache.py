@@ -30,12 +30,6 @@ PAGE = 64
 _FORMATS = {"f16": _lib.CACHE_F16, "bf16": _lib.CACHE_BF16, "q4": _lib.CACHE_Q4}
 
 
-def _raw_stream(index: int) -> int:
-    import torch
-
-    return torch.cuda.current_stream(index).cuda_stream
-
-
 def _fail(message: str, status: int = _lib.FMD_EINVAL):
     raise _lib.FmdError(status, message)
 
@@ -104,6 +98,7 @@ class PagedCache:
                              max_slots, max_pages_per_slot, 0)
         self._ref = C.byref(self._c)
         self._index = pool.get_device()
+        self._cuda, self._f32 = torch.cuda, torch.float32
         self._dtypes = ({torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16} if kind == "q4" else
                         {{"f16": torch.float16, "bf16": torch.bfloat16}[kind]: self.format})
         self._status = torch.zeros(2, dtype=torch.int32, device=self.device)
@@ -163,9 +158,13 @@ class PagedCache:
             _fail("a slot is listed twice")
         for s in slots:
             self._open(s)
+        names, free = self._names, self._free
         for s in slots:
-            for p in self._pages[s]:
-                self._drop(p)
+            for p in self._pages[s]:  # _drop, in line: many slots of many pages
+                if p >= 0:
+                    names[p] -= 1
+                    if not names[p]:
+                        heapq.heappush(free, p)
             self._pages[s], self._length[s] = None, 0
 
     def _drop(self, page: int) -> None:
@@ -269,13 +268,12 @@ class PagedCache:
 
     # -- operators -------------------------------------------------------------------------
     def _call(self, fn, *args) -> None:
-        import torch
-
-        if torch.cuda.current_device() == self._index:
-            st = fn(self._ref, *args, _raw_stream(self._index))
+        cuda, index = self._cuda, self._index
+        if cuda.current_device() == index:
+            st = fn(self._ref, *args, cuda.current_stream(index).cuda_stream)
         else:
-            with torch.cuda.device(self._index):
-                st = fn(self._ref, *args, _raw_stream(self._index))
+            with cuda.device(index):
+                st = fn(self._ref, *args, cuda.current_stream(index).cuda_stream)
         if st != _lib.FMD_OK:
             raise _lib.FmdError(st, f"{fn.__name__}: {self.lib.fmd_status_string(st).decode()}")
 
@@ -295,17 +293,19 @@ class PagedCache:
 
     def _heads(self, t, name: str, heads: int, rows: int, dtype) -> tuple:
         """(address, row stride, head stride) of a [rows, heads, head_dim] tensor."""
-        shape = t.shape
-        if len(shape) != 3 or shape[2] != self.head_dim or (heads and shape[1] != heads):
-            _fail(f"{name} must be [rows, {heads or 'heads'}, {self.head_dim}], not {tuple(shape)}")
+        if t.dim() != 3:
+            _fail(f"{name} must be [rows, {heads or 'heads'}, {self.head_dim}], not {tuple(t.shape)}")
+        n, h, d = t.shape
+        if d != self.head_dim or (heads and h != heads):
+            _fail(f"{name} must be [rows, {heads or 'heads'}, {self.head_dim}], not {(n, h, d)}")
         if t.get_device() != self._index:
             _fail(f"{name} must be on {self.device}")
-        if shape[0] != rows or t.dtype != dtype:
+        if n != rows or t.dtype != dtype:
             _fail(f"{name} must have the rows and dtype of the others")
         row, head, dim = t.stride()
-        if rows <= 1:
+        if n <= 1:
             row = 0
-        if shape[1] <= 1:
+        if h <= 1:
             head = 0
         at = t.data_ptr()
         if (dim != 1 or (row | head) & 7 or at & 15) and t.numel():
@@ -353,28 +353,26 @@ class PagedCache:
         if (cos is None) != (sin is None):
             _fail("cos and sin go together")
         if cos is not None:
-            import torch
-
-            shape = cos.shape
-            for t in (cos, sin):
-                if (t.dtype != torch.float32 or len(shape) != 2 or t.shape != shape or not t.is_contiguous()
-                        or t.get_device() != self._index or t.data_ptr() & 15):
-                    _fail("cos and sin must be aligned contiguous f32 tables [positions, pairs]")
-            table, pairs = shape
+            cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+            if (cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != self._f32 or sin.dtype != self._f32
+                    or not cos.is_contiguous() or not sin.is_contiguous() or (cos_at | sin_at) & 15
+                    or cos.get_device() != self._index or sin.get_device() != self._index):
+                _fail("cos and sin must be aligned contiguous f32 tables [positions, pairs]")
+            table, pairs = cos.shape
             rot = 2 * pairs
             if table < 1 or pairs % 4 or not 0 < rot <= self.head_dim:
                 _fail("the rotated dims must be a multiple of 8, at most head_dim")
-            cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
         args = _lib.CacheAppendArgs(k_at, v_at, q_at, o_at, k_row, k_head, v_row, v_head, q_row, q_head, o_row, o_head,
                                     qn_at, kn_at, cos_at, sin_at, eps, code, heads, rot, table, bool(interleaved))
         self._call(self.lib.fmd_cache_append, layer, self._rows_c(rows, n), C.byref(args), self._status_at)
         return q_out
 
     def _weight(self, w, name: str, dtype) -> int:
-        if (w.dtype != dtype or w.dim() != 1 or w.shape[0] != self.head_dim or w.stride(0) != 1
-                or w.get_device() != self._index or w.data_ptr() & 15):
+        at = w.data_ptr()
+        if (w.dtype != dtype or w.dim() != 1 or w.numel() != self.head_dim or not w.is_contiguous()
+                or w.get_device() != self._index or at & 15):
             _fail(f"{name} must be an aligned contiguous [{self.head_dim}] tensor of the rows' dtype")
-        return w.data_ptr()
+        return at
 
     def read(self, layer: int, rows: CacheRows, k_out=None, v_out=None, n_rows: int | None = None):
         """The cached keys and values of the rows' positions, f32
@@ -415,15 +413,14 @@ class PagedCache:
         return w
 
     def _workspace(self, n_heads: int, rows: CacheRows):
-        import torch
-
+        cuda = self._cuda
         n = self.lib.fmd_cache_attend_workspace(self._ref, n_heads, rows.slot.shape[0], rows.max_rows)
         if n == 0:
             return None
-        if torch.cuda.is_current_stream_capturing():
+        if cuda.is_current_stream_capturing():
             # a graph's own: graphs replayed at the same time must not share one
             return self._fresh_workspace(n)
-        key = _raw_stream(self._index)
+        key = cuda.current_stream(self._index).cuda_stream
         w = self._workspaces.get(key)
         if w is None or w.numel() < n:
             w = self._workspaces[key] = self._fresh_workspace(n)
@@ -489,14 +486,14 @@ class PagedCache:
             _fail(f"slot {src}: its last page was evicted")
         if part and len(dsts) > len(self._free):
             _fail("the cache has too few free pages", _lib.FMD_ENOMEM)
+        m, shared, names = len(dsts), pages[:full], self._names
         fresh = [self._take() if part else -1 for _ in dsts]
         for d, p in zip(dsts, fresh):
-            self._pages[d] = pages[:full] + ([p] if part else [])
+            self._pages[d] = shared + [p] if part else shared.copy()
             self._length[d] = n
-            for s in pages[:full]:
-                if s >= 0:
-                    self._names[s] += 1
-        m = len(dsts)
+        for p in shared:
+            if p >= 0:
+                names[p] += m
         ia = C.c_int32 * m
         self._call(self.lib.fmd_cache_fork, m, ia(*[src] * m), ia(*dsts), ia(*[n] * m), ia(*fresh),
                    self._status_at)

@@ -46,11 +46,10 @@ constexpr float kDcHeadroom = 8.f;  // log2: how far a score may exceed the refe
 struct DcArgs {
   CacheRows r;
   CacheAttend a;
-  float* part;      // [2 x grid][rows][D + 2] partials of cut segments
+  float* part;      // [2 x grid][rows][D + 4] partials of cut segments
   int* counters;    // [sequences][kv heads], zero between calls
   int seq0, seqs;   // the sequences of this launch
   int tile_rows;    // (row, head) pairs of a segment at most
-  uint32_t f64;     // f16 pair (64, 64)
   int stages, red_off, red_row;  // ring stages, merge buffer: its offset, its floats per pair
 };
 
@@ -75,12 +74,13 @@ FMD_DEV float ex2(float x) {
 FMD_DEV int dc_cta(long long x, long long T, int G) { return (int)(((x + 1) * G - 1) / T); }
 
 // The keys of a sequence whose first row is at p0 as units of K: kSetup units
-// without keys, which stand for what a segment costs beside its keys (its queries,
-// its merge: about 2.5 us, as long as a CTA takes for so many units), so that
-// ranges over short segments are not the last to finish; then `sinks` units
-// from position 0, then units from unit `w0` on.
+// without keys, which stand for what a segment costs beside its keys (its queries
+// and its merge: a CTA's second piece took 5.5 us and more, a unit of 32 keys 0.7),
+// so that ranges over short segments are not the last to finish (64 streams of
+// 300 .. 16,384 positions in 4 bits: 89.5 us with 4 units, 84.5 with 7 or 10); then
+// `sinks` units from position 0, then units from unit `w0` on.
 template <int K> struct DcKeys {
-  static constexpr int kSetup = K == 32 ? 4 : 1;
+  static constexpr int kSetup = K == 32 ? 8 : 1;
   int sinks, w0;
   FMD_DEV DcKeys(const CacheAttend& a, int p0) {
     const int first = a.window && p0 >= a.window ? p0 - a.window + 1 : 0;
@@ -179,7 +179,8 @@ struct DcPiece {
 template <typename T, int D>
 FMD_DEV void dc_merge(float* red, DcSeqs& q, const DcArgs& p, const DcPiece& s, int H, int gs, bool aborted) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int rs = D + 2;
+  constexpr int rs = D + 4;     // floats of a partial's row: o, m, l and two to keep 16 bytes
+  constexpr int ls = D + 2;     // of a warp's row in `red`
   auto out_at = [&](int row, int d0) {
     return (T*)p.a.out + (size_t)(q.row[s.r] + (row >> gs)) * p.a.out_row +
            (size_t)((s.h << gs) + (row & ((1 << gs) - 1))) * p.a.out_head + d0;
@@ -190,12 +191,12 @@ FMD_DEV void dc_merge(float* red, DcSeqs& q, const DcArgs& p, const DcPiece& s, 
     const int row = i / (D / 2), d0 = (i % (D / 2)) * 2;
     float mm[4], Mx = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) Mx = fmaxf(Mx, mm[w] = red[(size_t)(w * p.tile_rows + row) * rs + D]);
+    for (int w = 0; w < 4; ++w) Mx = fmaxf(Mx, mm[w] = red[(size_t)(w * p.tile_rows + row) * ls + D]);
     const float base = Mx == -INFINITY ? 0.f : Mx;
     float L = 0.f, A0 = 0.f, A1 = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float* rw = red + (size_t)(w * p.tile_rows + row) * rs;
+      const float* rw = red + (size_t)(w * p.tile_rows + row) * ls;
       const float f = ex2(mm[w] - base);  // 0 for a warp that saw nothing
       L = fmaf(rw[D + 1], f, L);
       A0 = fmaf(rw[d0], f, A0);
@@ -227,36 +228,68 @@ FMD_DEV void dc_merge(float* red, DcSeqs& q, const DcArgs& p, const DcPiece& s, 
       };
       for (int row = warp; row < s.nq; row += 4) {
         float Mx = -INFINITY, L = 0.f;
-        for (int k = lane; k < np; k += 32) {
-          const float x = __ldcg(piece(k) + row * rs + D);
-          red[row * ws + k] = x;
-          Mx = fmaxf(Mx, x);
+        float2 ml[4];  // the first 128 pieces' (m, l), loaded together
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = lane + 32 * i;
+          ml[i] = k < np ? __ldcg(reinterpret_cast<const float2*>(piece(k) + row * rs + D)) : make_float2(-INFINITY, 0.f);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Mx = fmaxf(Mx, ml[i].x);
+        for (int k = lane + 128; k < np; k += 32) Mx = fmaxf(Mx, __ldcg(piece(k) + row * rs + D));
         Mx = warp_max(Mx);
         const float base = Mx == -INFINITY ? 0.f : Mx;
-        for (int k = lane; k < np; k += 32) {
-          const float f = ex2(red[row * ws + k] - base);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f = ex2(ml[i].x - base);
+          if (lane + 32 * i < np) red[row * ws + lane + 32 * i] = f;
+          L = fmaf(ml[i].y, f, L);
+        }
+        for (int k = lane + 128; k < np; k += 32) {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(piece(k) + row * rs + D));
+          const float f = ex2(v.x - base);
           red[row * ws + k] = f;
-          L = fmaf(__ldcg(piece(k) + row * rs + D + 1), f, L);
+          L = fmaf(v.y, f, L);
         }
         L = warp_sum(L);
         if (lane == 0) red[row * ws + np] = L;
       }
       named_sync(1, 128);
-      for (int i = tid; i < s.nq * (D / 2); i += 128) {
-        const int row = i / (D / 2), d0 = (i % (D / 2)) * 2;
+      // four dims a thread; where that leaves threads, groups of them share the pieces
+      // (one stream over 4,096 keys: 12.5 us, 13.5 without groups)
+      const int work = s.nq * (D / 4), groups = max(1, 128 / work);
+      float4* join = reinterpret_cast<float4*>(red + p.tile_rows * ws);
+      for (int i0 = 0; i0 < work; i0 += 128) {
+        const int grp = groups > 1 ? tid / work : 0, i = groups > 1 ? tid - grp * work : i0 + tid;
+        const int row = i / (D / 4), d0 = (i % (D / 4)) * 4;
         const float* w = red + row * ws;
-        float2 x = __ldcg(reinterpret_cast<const float2*>(piece(0) + row * rs + d0));
-        float A0 = x.x * w[0], A1 = x.y * w[0];
-        const float* pt = p.part + (size_t)2 * (cf + 1) * p.tile_rows * rs + row * rs + d0;
-        const size_t step = (size_t)2 * p.tile_rows * rs;
+        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (grp < groups && i < work) {
+          const size_t step = (size_t)2 * p.tile_rows * rs * groups;
+          const float* pt = p.part + (size_t)2 * (cf + grp) * p.tile_rows * rs + row * rs + d0;
 #pragma unroll 16
-        for (int k = 1; k < np; ++k, pt += step) {
-          x = __ldcg(reinterpret_cast<const float2*>(pt));
-          A0 = fmaf(x.x, w[k], A0);
-          A1 = fmaf(x.y, w[k], A1);
+          for (int k = grp; k < np; k += groups, pt += step) {
+            // the segment's first piece is its CTA's second slot
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(pt + (k == 0 ? p.tile_rows * rs : 0)));
+            const float f = w[k];
+            A.x = fmaf(x.x, f, A.x);
+            A.y = fmaf(x.y, f, A.y);
+            A.z = fmaf(x.z, f, A.z);
+            A.w = fmaf(x.w, f, A.w);
+          }
         }
-        if (!aborted) *reinterpret_cast<uint32_t*>(out_at(row, d0)) = Act<T>::pack2(A0 / w[np], A1 / w[np]);
+        if (groups > 1) {
+          join[tid] = A;
+          named_sync(1, 128);
+          for (int k = 1; grp == 0 && k < groups; ++k) {
+            const float4 x = join[tid + k * work];
+            A.x += x.x, A.y += x.y, A.z += x.z, A.w += x.w;
+          }
+        }
+        if (grp == 0 && i < work && !aborted) {
+          const float L = w[np];
+          *reinterpret_cast<uint2*>(out_at(row, d0)) = make_uint2(Act<T>::pack2(A.x / L, A.y / L), Act<T>::pack2(A.z / L, A.w / L));
+        }
       }
       if (tid == 0) *counter = 0;
     }
@@ -581,26 +614,29 @@ __global__ void __launch_bounds__(kDc16Threads, 2)
 // multiplies block b's f32 sum, exact up to f32 sums, and the second term is one
 // product of the scales with the queries' block sums. Queries are scaled by a power of two per row to [2^14, 2^15) at most,
 // which keeps what is 2^-24 of the row's largest.
-// Values: f16 pairs 64 + c by one shift and one and-or (mantissa bits 4-7), then
-// (c - 8) d in f16 (one rounding, 2^-11): the scale differs by key, which is
-// the sum's index there. With f16 outputs, whose own rounding is no larger, P goes in
+// Values: (c - 8) d in f16, one fused multiply-add on the same subnormals: with
+// D = d 2^(15 - k), c 2^-24 D - 2^-21 D = (c - 8) d 2^(-9 - k), rounded once (2^-11). The
+// scale differs by key, the sum's index here, so it cannot wait for the sum. k
+// is a running exponent of the block's scales, |d| < 2^k, moved with the sums and taken
+// out at the end: what the factor 2^-9 loses to subnormals is 2^-19 of the block's
+// largest value. With f16 outputs, whose own rounding is no larger, P goes in
 // as two terms (error against 64 bits 2.7e-4 instead of 3.4e-4; the output's 2.1e-4).
 
 constexpr int kDq4Threads = 128;
 
-FMD_DEV uint32_t h2sub(uint32_t a, uint32_t b) {
-  __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
 FMD_DEV uint32_t h2mul(uint32_t a, uint32_t b) {
   __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<uint32_t*>(&r);
 }
-// Nibble N of both 16-bit halves as the f16 pair 64 + c. f64 = 0x54005400 comes in
-// a register: with two literal operands the and-or became two instructions.
-template <int N> FMD_DEV uint32_t nibble64(uint32_t w, uint32_t f64) {
-  const uint32_t x = N == 0 ? w << 4 : N == 1 ? w : N == 2 ? w >> 4 : w >> 8;
-  return (x & 0x00f000f0u) | f64;
+FMD_DEV uint32_t h2fma(uint32_t a, uint32_t b, uint32_t c) {
+  __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b),
+                      *reinterpret_cast<__half2*>(&c));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+// 2^e as an f16 pair (e in -24 .. 15)
+FMD_DEV uint32_t h2pow(int e) {
+  const uint32_t h = e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);
+  return h | h << 16;
 }
 // d = a x b (m16n8k16, f16)
 FMD_DEV void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -686,7 +722,6 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
   for (int i = 0; i < stages && i < own; ++i) issue();
 
   bool aborted = false;
-  const uint32_t f64 = p.f64;
   const int gs = __ffs(p.a.n_heads / H) - 1;
   const int W = p.a.window, S = W ? p.a.sinks : 0;
   int cr, ch, cj;
@@ -698,6 +733,7 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
   // this warp's next unit of the CTA's range, its stage and the stage's phase
   int mine = warp, s = 0, phase = 0;
   for (int x = 0; x < ntl;) {
+    int ve = -24;  // k: the running exponent of this thread's value scales (-24: none yet)
     // a piece: units cj .. cj + len - 1 of segment (cr, ch)
     const int len = min(ctr - cj, ntl - x);
     const int nq = q.cnt[cr] << gs, p0 = q.pos[cr], p1 = p0 + q.cnt[cr] - 1;
@@ -842,23 +878,50 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
         }
         uint32_t pb[NT][U][2], pl[kHiLo ? NT : 1][U][2], vis[U][2];
         dc_softmax<__half, U, MT, NT, kHiLo>(sc, sl, m, l, o, pb, pl, vis, whole, k0, p0, p1, W, S, gs, 7.f);
-        // O^T += V^T P^T; this thread's keys: kb, kb + 1, kb + 8, kb + 9
+        // values: this thread's keys of a step are kb, kb + 1, kb + 8, kb + 9, its dims lie in one block
+        const uint8_t* vs = vt + CB;
+        const int blk = NB == 4 ? g >> 1 : g >> 2;
+        uint32_t d2[U][2], big = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int kb = u * 16 + 2 * t;
-          const uint8_t* vs = vt + CB;
-          const int blk = NB == 4 ? g >> 1 : g >> 2;  // this thread's dims lie in one block
-          uint32_t d2[2];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            const uint32_t lo = *reinterpret_cast<const uint16_t*>(vs + ((kb + b * 8) * NB + blk) * 2);
-            const uint32_t hi = *reinterpret_cast<const uint16_t*>(vs + ((kb + b * 8 + 1) * NB + blk) * 2);
-            d2[b] = __byte_perm(lo, hi, 0x5410) & vis[u][b];
+            const int kb = u * 16 + 2 * t + b * 8;
+            const uint32_t lo = *reinterpret_cast<const uint16_t*>(vs + (kb * NB + blk) * 2);
+            const uint32_t hi = *reinterpret_cast<const uint16_t*>(vs + ((kb + 1) * NB + blk) * 2);
+            d2[u][b] = __byte_perm(lo, hi, 0x5410) & vis[u][b];
+            big |= d2[u][b];
+          }
+        // an or of the scales is no smaller than their largest: |d| < 2^(field - 14)
+        const int e = min((int)((big | big >> 16) >> 10 & 31), 30) - 14;
+        if (__any_sync(0xffffffffu, e > ve)) {
+          int ne = max(ve, e);  // one for the four lanes of a row of O^T
+          ne = max(ne, __shfl_xor_sync(0xffffffffu, ne, 1));
+          ne = max(ne, __shfl_xor_sync(0xffffffffu, ne, 2));
+          const float f = __uint_as_float((uint32_t)(127 + ve - ne) << 23);
+          ve = ne;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) o[n][i][k] *= f;
+        }
+        const uint32_t up = h2pow(min(15 - ve, 15)), up2 = h2pow(max(-ve, 0));  // 2^(15 - k), in f16's range
+        // O^T += V^T P^T
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          uint32_t dl[2], dh[2], d8[2];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            dl[b] = h2mul(h2mul(d2[u][b], up2), up);  // for c 2^-24
+            dh[b] = h2mul(dl[b], 0x2c002c00u);        // 2^-4: for c 2^-20
+            d8[b] = h2mul(dl[b], 0x80088008u);        // -2^-21
           }
           uint32_t w[4][D / 64];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint8_t* src = vt + (kb + (e & 1) + (e >> 1) * 8) * (D / 2);
+            const uint8_t* src = vt + (u * 16 + 2 * t + (e & 1) + (e >> 1) * 8) * (D / 2);
             if constexpr (D == 128) {
               const uint2 y = *reinterpret_cast<const uint2*>(src + g * 8);
               w[e][0] = y.x, w[e][1] = y.y;
@@ -872,14 +935,13 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
               const uint32_t sel = hf ? 0x7632 : 0x5410;
+              constexpr uint32_t lo = 0x000f000fu, hi = 0x00f000f0u;
               const uint32_t y0 = __byte_perm(w[0][i], w[1][i], sel), y1 = __byte_perm(w[2][i], w[3][i], sel);
-              const uint32_t k72 = 0x54805480u;  // f16 72
-              const uint32_t a0[4] = {
-                  h2mul(h2sub(nibble64<0>(y0, f64), k72), d2[0]), h2mul(h2sub(nibble64<1>(y0, f64), k72), d2[0]),
-                  h2mul(h2sub(nibble64<0>(y1, f64), k72), d2[1]), h2mul(h2sub(nibble64<1>(y1, f64), k72), d2[1])};
-              const uint32_t a1[4] = {
-                  h2mul(h2sub(nibble64<2>(y0, f64), k72), d2[0]), h2mul(h2sub(nibble64<3>(y0, f64), k72), d2[0]),
-                  h2mul(h2sub(nibble64<2>(y1, f64), k72), d2[1]), h2mul(h2sub(nibble64<3>(y1, f64), k72), d2[1])};
+              const uint32_t z0 = y0 >> 8, z1 = y1 >> 8;
+              const uint32_t a0[4] = {h2fma(y0 & lo, dl[0], d8[0]), h2fma(y0 & hi, dh[0], d8[0]),
+                                      h2fma(y1 & lo, dl[1], d8[1]), h2fma(y1 & hi, dh[1], d8[1])};
+              const uint32_t a1[4] = {h2fma(z0 & lo, dl[0], d8[0]), h2fma(z0 & hi, dh[0], d8[0]),
+                                      h2fma(z1 & lo, dl[1], d8[1]), h2fma(z1 & hi, dh[1], d8[1])};
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 mma16816<__half>(o[n][i * 4 + hf * 2], a0, pb[n][u][0], pb[n][u][1]);
@@ -896,6 +958,13 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
       if (issued < own) issue();
       if (++s == stages) s = 0, phase ^= 1;
     }
+    const float vf = __uint_as_float((uint32_t)(127 + 9 + ve) << 23);  // the values' factor
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[n][i][k] *= vf;
     dc_store<D, NT>(red, p.tile_rows, nq, o, m, l, [&](int i, int e) {
       return (D / 8) * g + 8 * (i >> 2) + 4 * ((i >> 1) & 1) + 2 * (i & 1) + e;
     });
@@ -940,7 +1009,7 @@ DcShape dc_shape(const CacheView& c, int rows) {
     s.grid = 148 * s.per_sm;
     // merge buffer: four warps' rows, or a weight per piece of a segment (at most one a CTA) and the sum
     s.red_row = std::max(4 * (D + 2), s.grid + 4);
-    const int red = rows * s.red_row * 4;
+    const int red = (rows * s.red_row + 4 * 128) * 4;
     s.stages = std::min(q4 ? 4 : 8, (227 * 1024 / s.per_sm - fixed - red) / stage);
     if (s.stages >= 2 || s.per_sm == 1) {
       s.stages = std::max(s.stages, 2);
@@ -960,7 +1029,7 @@ bool cache_decode_fits(const CacheView& c, int n_heads, int max_rows) {
 // counters, then partials
 size_t cache_decode_workspace(const CacheView& c, int n_heads, int max_rows) {
   const int rows = max_rows * (n_heads / c.kv_heads);
-  return (kDcCounters + (size_t)2 * dc_shape(c, rows).grid * rows * (c.head_dim + 2)) * 4;
+  return (kDcCounters + (size_t)2 * dc_shape(c, rows).grid * rows * (c.head_dim + 4)) * 4;
 }
 
 bool cache_tensor_map(CUtensorMap* m, const CacheView& c, int layer) {
@@ -996,7 +1065,6 @@ cudaError_t launch_cache_decode(bool bf16, const CacheView& c, int layer, const 
   p.r = r;
   p.a = a;
   p.tile_rows = rows;
-  p.f64 = 0x54005400u;
   p.counters = (int*)workspace;
   p.part = (float*)workspace + kDcCounters;
   p.seqs = std::min(kDcSeqs, kDcCounters / c.kv_heads);
