@@ -282,6 +282,8 @@ class PagedCache:
         st = int(self._status[0].item())
         if st != 0:
             self._status.zero_()
+            if st == _lib.FMD_ETIMEDOUT:
+                self._workspaces.clear()  # their counters may be left in the middle
             raise _lib.FmdError(st, "a device-side wait gave up" if st == _lib.FMD_ETIMEDOUT else
                                 "a slot, position or page was out of range")
 
@@ -431,8 +433,8 @@ class PagedCache:
         """Attention of queries `[rows, heads, head_dim]` over their slots' cached
         positions j <= p (p: the row's own, already appended): all of them, or
         with `window` > 0 those with j > p - window or j < sinks. `scale` defaults
-        to head_dim ** -0.5. Returns `out` (rows of padding and behind the last
-        sequence are left as they were)."""
+        to head_dim ** -0.5. Returns `out` (not `q` itself; rows of padding and
+        behind the last sequence are left as they were)."""
         if not 0 <= layer < self.layers:
             _fail(f"layer {layer} is out of range")
         if not 0 <= window < 2**31 or not 0 <= sinks < 2**31:

@@ -3,6 +3,8 @@
 #include <algorithm>
 #include <climits>
 #include <cstring>
+#include <memory>
+#include <new>
 
 #include "fmd_cache.cuh"
 
@@ -620,6 +622,17 @@ CacheView view_of(const fmd_cache* c) {
 CacheRows rows_of(const fmd_cache_rows* r) {
   return CacheRows{r->slot, r->pos0, r->row0, nullptr, nullptr, r->n_seqs, r->n_rows};
 }
+// FMD_EINVAL if a value of dst occurs twice there, or in src.
+int check_moves(int n, const int32_t* src, const int32_t* dst) {
+  std::unique_ptr<int32_t[]> d(new (std::nothrow) int32_t[n]);
+  if (!d) return FMD_ENOMEM;
+  std::copy(dst, dst + n, d.get());
+  std::sort(d.get(), d.get() + n);
+  if (std::adjacent_find(d.get(), d.get() + n) != d.get() + n) return FMD_EINVAL;
+  for (int i = 0; src && i < n; ++i)
+    if (std::binary_search(d.get(), d.get() + n, src[i])) return FMD_EINVAL;
+  return FMD_OK;
+}
 int done(cudaError_t e) {
   if (e == cudaSuccess) return FMD_OK;
   cudaGetLastError();  // the call's own failure, returned here
@@ -696,14 +709,14 @@ int64_t fmd_cache_attend_workspace(const fmd_cache* c, int32_t n_heads, int32_t 
   if (check_cache(c) || n_heads < 1 || n_heads % c->kv_heads || n_seqs < 1 || max_rows < 1) return 0;
   const CacheView v = view_of(c);
   return (int64_t)(cache_decode_fits(v, n_heads, max_rows) ? cache_decode_workspace(v, n_heads, max_rows)
-                                                           : cache_chunk_workspace(v, n_heads, n_seqs, max_rows));
+                                                           : cache_chunk_workspace(v));
 }
 
 int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows, const fmd_cache_attend_args* a,
                      void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
   int rc = check_cache(c);
   if (rc || (rc = check_rows(c, layer, rows))) return rc;
-  if (!a || !a->q || !a->out || !aligned16(a->q) || !aligned16(a->out)) return FMD_EINVAL;
+  if (!a || !a->q || !a->out || a->out == a->q || !aligned16(a->q) || !aligned16(a->out)) return FMD_EINVAL;
   if (a->dtype != FMD_DT_F16 && a->dtype != FMD_DT_BF16) return FMD_EINVAL;
   if (c->format != FMD_CACHE_Q4 && c->format != a->dtype) return FMD_EINVAL;
   if (a->n_heads < 1 || a->n_heads % c->kv_heads) return FMD_EINVAL;
@@ -730,6 +743,7 @@ int fmd_cache_copy_pages(const fmd_cache* c, int32_t n, const int32_t* src, cons
   for (int i = 0; i < n; ++i)
     if (src[i] < 0 || src[i] >= c->n_pages || dst[i] < 0 || dst[i] >= c->n_pages) return FMD_EINVAL;
   if (n == 0) return FMD_OK;
+  if ((rc = check_moves(n, src, dst))) return rc;
   if (!on_current_device(c->pool)) return FMD_EINVAL;
   for (int i = 0; i < n; i += kCopyBatch) {
     CopyList l;
@@ -757,6 +771,15 @@ int fmd_cache_fork(const fmd_cache* c, int32_t n, const int32_t* src_slot, const
     if (len[i] % kPageTokens && (new_page[i] < 0 || new_page[i] >= c->n_pages)) return FMD_EINVAL;
   }
   if (n == 0) return FMD_OK;
+  if ((rc = check_moves(n, src_slot, dst_slot))) return rc;
+  {
+    std::unique_ptr<int32_t[]> pages(new (std::nothrow) int32_t[n]);
+    if (!pages) return FMD_ENOMEM;
+    int m = 0;
+    for (int i = 0; i < n; ++i)
+      if (len[i] % kPageTokens) pages[m++] = new_page[i];
+    if ((rc = check_moves(m, nullptr, pages.get()))) return rc;
+  }
   if (!on_current_device(c->pool)) return FMD_EINVAL;
   for (int i = 0; i < n; i += kCopyBatch) {
     ForkList l;

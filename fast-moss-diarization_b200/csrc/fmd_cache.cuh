@@ -123,7 +123,7 @@ cudaError_t launch_cache_decode(bool bf16, const CacheView& c, int layer, const 
 // the TMA map of a 16-bit cache's layer as [rows][head_dim], 64 x 64 boxes, 128-byte swizzle
 bool cache_tensor_map(CUtensorMap* m, const CacheView& c, int layer);
 // fmd_cache_chunk.cu: the others
-size_t cache_chunk_workspace(const CacheView& c, int n_heads, int n_seqs, int max_rows);
+size_t cache_chunk_workspace(const CacheView& c);
 cudaError_t launch_cache_chunk(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAttend& a,
                                void* workspace, int* status, cudaStream_t s);
 

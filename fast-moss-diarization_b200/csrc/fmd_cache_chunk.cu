@@ -1011,9 +1011,8 @@ constexpr int kCkGrid = 148;
 
 }  // namespace
 
-// counters, then the partials of cut items
-size_t cache_chunk_workspace(const CacheView& c, int n_heads, int n_seqs, int max_rows) {
-  if (!ck_shape(true, c, n_heads, n_seqs, max_rows).split) return 0;
+// counters, then the partials of cut items (of smaller calls, where this size is not split)
+size_t cache_chunk_workspace(const CacheView& c) {
   return FMD_CACHE_WORKSPACE_ZERO + (size_t)2 * kCkGrid * 256 * (c.head_dim + 2) * 4;
 }
 

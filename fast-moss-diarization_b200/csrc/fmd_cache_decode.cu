@@ -50,6 +50,7 @@ struct DcArgs {
   int* counters;    // [sequences][kv heads], zero between calls
   int seq0, seqs;   // the sequences of this launch
   int tile_rows;    // (row, head) pairs of a segment at most
+  uint32_t f64;     // f16 pair (64, 64)
   int stages, red_off, red_row;  // ring stages, merge buffer: its offset, its floats per pair
 };
 
@@ -614,29 +615,26 @@ __global__ void __launch_bounds__(kDc16Threads, 2)
 // multiplies block b's f32 sum, exact up to f32 sums, and the second term is one
 // product of the scales with the queries' block sums. Queries are scaled by a power of two per row to [2^14, 2^15) at most,
 // which keeps what is 2^-24 of the row's largest.
-// Values: (c - 8) d in f16, one fused multiply-add on the same subnormals: with
-// D = d 2^(15 - k), c 2^-24 D - 2^-21 D = (c - 8) d 2^(-9 - k), rounded once (2^-11). The
-// scale differs by key, the sum's index here, so it cannot wait for the sum. k
-// is a running exponent of the block's scales, |d| < 2^k, moved with the sums and taken
-// out at the end: what the factor 2^-9 loses to subnormals is 2^-19 of the block's
-// largest value. With f16 outputs, whose own rounding is no larger, P goes in
+// Values: f16 pairs 64 + c by one shift and one and-or (mantissa bits 4-7), then
+// (c - 8) d in f16 (one rounding, 2^-11): the scale differs by key, which is
+// the sum's index there. With f16 outputs, whose own rounding is no larger, P goes in
 // as two terms (error against 64 bits 2.7e-4 instead of 3.4e-4; the output's 2.1e-4).
 
 constexpr int kDq4Threads = 128;
 
+FMD_DEV uint32_t h2sub(uint32_t a, uint32_t b) {
+  __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
 FMD_DEV uint32_t h2mul(uint32_t a, uint32_t b) {
   __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<uint32_t*>(&r);
 }
-FMD_DEV uint32_t h2fma(uint32_t a, uint32_t b, uint32_t c) {
-  __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b),
-                      *reinterpret_cast<__half2*>(&c));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-// 2^e as an f16 pair (e in -24 .. 15)
-FMD_DEV uint32_t h2pow(int e) {
-  const uint32_t h = e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);
-  return h | h << 16;
+// Nibble N of both 16-bit halves as the f16 pair 64 + c. f64 = 0x54005400 comes in
+// a register: with two literal operands the and-or became two instructions.
+template <int N> FMD_DEV uint32_t nibble64(uint32_t w, uint32_t f64) {
+  const uint32_t x = N == 0 ? w << 4 : N == 1 ? w : N == 2 ? w >> 4 : w >> 8;
+  return (x & 0x00f000f0u) | f64;
 }
 // d = a x b (m16n8k16, f16)
 FMD_DEV void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -722,6 +720,7 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
   for (int i = 0; i < stages && i < own; ++i) issue();
 
   bool aborted = false;
+  const uint32_t f64 = p.f64;
   const int gs = __ffs(p.a.n_heads / H) - 1;
   const int W = p.a.window, S = W ? p.a.sinks : 0;
   int cr, ch, cj;
@@ -733,7 +732,6 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
   // this warp's next unit of the CTA's range, its stage and the stage's phase
   int mine = warp, s = 0, phase = 0;
   for (int x = 0; x < ntl;) {
-    int ve = -24;  // k: the running exponent of this thread's value scales (-24: none yet)
     // a piece: units cj .. cj + len - 1 of segment (cr, ch)
     const int len = min(ctr - cj, ntl - x);
     const int nq = q.cnt[cr] << gs, p0 = q.pos[cr], p1 = p0 + q.cnt[cr] - 1;
@@ -878,50 +876,23 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
         }
         uint32_t pb[NT][U][2], pl[kHiLo ? NT : 1][U][2], vis[U][2];
         dc_softmax<__half, U, MT, NT, kHiLo>(sc, sl, m, l, o, pb, pl, vis, whole, k0, p0, p1, W, S, gs, 7.f);
-        // values: this thread's keys of a step are kb, kb + 1, kb + 8, kb + 9, its dims lie in one block
-        const uint8_t* vs = vt + CB;
-        const int blk = NB == 4 ? g >> 1 : g >> 2;
-        uint32_t d2[U][2], big = 0;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int kb = u * 16 + 2 * t + b * 8;
-            const uint32_t lo = *reinterpret_cast<const uint16_t*>(vs + (kb * NB + blk) * 2);
-            const uint32_t hi = *reinterpret_cast<const uint16_t*>(vs + ((kb + 1) * NB + blk) * 2);
-            d2[u][b] = __byte_perm(lo, hi, 0x5410) & vis[u][b];
-            big |= d2[u][b];
-          }
-        // an or of the scales is no smaller than their largest: |d| < 2^(field - 14)
-        const int e = min((int)((big | big >> 16) >> 10 & 31), 30) - 14;
-        if (__any_sync(0xffffffffu, e > ve)) {
-          int ne = max(ve, e);  // one for the four lanes of a row of O^T
-          ne = max(ne, __shfl_xor_sync(0xffffffffu, ne, 1));
-          ne = max(ne, __shfl_xor_sync(0xffffffffu, ne, 2));
-          const float f = __uint_as_float((uint32_t)(127 + ve - ne) << 23);
-          ve = ne;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) o[n][i][k] *= f;
-        }
-        const uint32_t up = h2pow(min(15 - ve, 15)), up2 = h2pow(max(-ve, 0));  // 2^(15 - k), in f16's range
-        // O^T += V^T P^T
+        // O^T += V^T P^T; this thread's keys: kb, kb + 1, kb + 8, kb + 9
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          uint32_t dl[2], dh[2], d8[2];
+          const int kb = u * 16 + 2 * t;
+          const uint8_t* vs = vt + CB;
+          const int blk = NB == 4 ? g >> 1 : g >> 2;  // this thread's dims lie in one block
+          uint32_t d2[2];
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            dl[b] = h2mul(h2mul(d2[u][b], up2), up);  // for c 2^-24
-            dh[b] = h2mul(dl[b], 0x2c002c00u);        // 2^-4: for c 2^-20
-            d8[b] = h2mul(dl[b], 0x80088008u);        // -2^-21
+            const uint32_t lo = *reinterpret_cast<const uint16_t*>(vs + ((kb + b * 8) * NB + blk) * 2);
+            const uint32_t hi = *reinterpret_cast<const uint16_t*>(vs + ((kb + b * 8 + 1) * NB + blk) * 2);
+            d2[b] = __byte_perm(lo, hi, 0x5410) & vis[u][b];
           }
           uint32_t w[4][D / 64];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint8_t* src = vt + (u * 16 + 2 * t + (e & 1) + (e >> 1) * 8) * (D / 2);
+            const uint8_t* src = vt + (kb + (e & 1) + (e >> 1) * 8) * (D / 2);
             if constexpr (D == 128) {
               const uint2 y = *reinterpret_cast<const uint2*>(src + g * 8);
               w[e][0] = y.x, w[e][1] = y.y;
@@ -935,13 +906,14 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
               const uint32_t sel = hf ? 0x7632 : 0x5410;
-              constexpr uint32_t lo = 0x000f000fu, hi = 0x00f000f0u;
               const uint32_t y0 = __byte_perm(w[0][i], w[1][i], sel), y1 = __byte_perm(w[2][i], w[3][i], sel);
-              const uint32_t z0 = y0 >> 8, z1 = y1 >> 8;
-              const uint32_t a0[4] = {h2fma(y0 & lo, dl[0], d8[0]), h2fma(y0 & hi, dh[0], d8[0]),
-                                      h2fma(y1 & lo, dl[1], d8[1]), h2fma(y1 & hi, dh[1], d8[1])};
-              const uint32_t a1[4] = {h2fma(z0 & lo, dl[0], d8[0]), h2fma(z0 & hi, dh[0], d8[0]),
-                                      h2fma(z1 & lo, dl[1], d8[1]), h2fma(z1 & hi, dh[1], d8[1])};
+              const uint32_t k72 = 0x54805480u;  // f16 72
+              const uint32_t a0[4] = {
+                  h2mul(h2sub(nibble64<0>(y0, f64), k72), d2[0]), h2mul(h2sub(nibble64<1>(y0, f64), k72), d2[0]),
+                  h2mul(h2sub(nibble64<0>(y1, f64), k72), d2[1]), h2mul(h2sub(nibble64<1>(y1, f64), k72), d2[1])};
+              const uint32_t a1[4] = {
+                  h2mul(h2sub(nibble64<2>(y0, f64), k72), d2[0]), h2mul(h2sub(nibble64<3>(y0, f64), k72), d2[0]),
+                  h2mul(h2sub(nibble64<2>(y1, f64), k72), d2[1]), h2mul(h2sub(nibble64<3>(y1, f64), k72), d2[1])};
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 mma16816<__half>(o[n][i * 4 + hf * 2], a0, pb[n][u][0], pb[n][u][1]);
@@ -958,13 +930,6 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
       if (issued < own) issue();
       if (++s == stages) s = 0, phase ^= 1;
     }
-    const float vf = __uint_as_float((uint32_t)(127 + 9 + ve) << 23);  // the values' factor
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[n][i][k] *= vf;
     dc_store<D, NT>(red, p.tile_rows, nq, o, m, l, [&](int i, int e) {
       return (D / 8) * g + 8 * (i >> 2) + 4 * ((i >> 1) & 1) + 2 * (i & 1) + e;
     });
@@ -1026,10 +991,10 @@ bool cache_decode_fits(const CacheView& c, int n_heads, int max_rows) {
   return (long long)max_rows * (n_heads / c.kv_heads) <= 16;
 }
 
-// counters, then partials
+// counters, then partials, of the largest grid: fewer rows may run on a larger one
 size_t cache_decode_workspace(const CacheView& c, int n_heads, int max_rows) {
   const int rows = max_rows * (n_heads / c.kv_heads);
-  return (kDcCounters + (size_t)2 * dc_shape(c, rows).grid * rows * (c.head_dim + 4)) * 4;
+  return (kDcCounters + (size_t)2 * dc_shape(c, 1).grid * rows * (c.head_dim + 4)) * 4;
 }
 
 bool cache_tensor_map(CUtensorMap* m, const CacheView& c, int layer) {
@@ -1071,6 +1036,7 @@ cudaError_t launch_cache_decode(bool bf16, const CacheView& c, int layer, const 
   p.stages = sh.stages;
   p.red_off = sh.red_off;
   p.red_row = sh.red_row;
+  p.f64 = 0x54005400u;
   auto each = [&](auto kern, auto&&... head) -> cudaError_t {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.smem);
     for (int s0 = 0; e == cudaSuccess && s0 < r.n_seqs; s0 += p.seqs) {

@@ -926,6 +926,7 @@ int sync_check(fmd_handle* h) {
     if (e != cudaSuccess) return fail(h, FMD_EIO, std::string("status read: ") + cudaGetErrorString(e));
     if (st[0] != 0) {
       cudaMemset(h->d_status, 0, 2 * sizeof(int));
+      if (h->cache_ws) cudaMemset(h->cache_ws, 0, FMD_CACHE_WORKSPACE_ZERO);
       static const char* const kSites[] = {"?", "k_gemv", "k_lm_head", "k_attn_decode_tma", "k_attn_prefill_tc",
                                            "k_gemm_tc", "k_layer_tail", "k_wait_probe", "k_proj_tc", "k_cache_decode", "k_cache_chunk"};
       constexpr int kNumSites = (int)(sizeof(kSites) / sizeof(kSites[0]));
@@ -1327,7 +1328,7 @@ int fmd_kv_reserve(fmd_handle* h, int32_t max_slots, int64_t max_tokens_total, i
   h->d_status = (int*)p;
   if (h->cache_ops()) {
     const size_t n = std::max(cache_decode_workspace(h->cache, h->Hq(), 1),
-                              cache_chunk_workspace(h->cache, h->Hq(), h->pb_max, 2 * kRowsPerPBlock));
+                              cache_chunk_workspace(h->cache));
     if ((rc = A(n, &p))) return rc;
     CK(cudaMemset(p, 0, n));
     h->cache_ws = p;

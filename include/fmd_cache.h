@@ -140,7 +140,8 @@ int64_t fmd_cache_attend_workspace(const fmd_cache* c, int32_t n_heads, int32_t 
  * sums are f32. What a cached position that no row of the call sees holds, NaN
  * included, has no influence. `workspace` is 16-byte aligned; its first
  * FMD_CACHE_WORKSPACE_ZERO bytes are zero before its first use, and every call
- * leaves them zero, so calls of any shape and cache may take turns with it. */
+ * leaves them zero, so calls of any shape and cache may take turns with it (after
+ * a FMD_ETIMEDOUT in `status` they must be zeroed again). `out` may not be q. */
 int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows,
                      const fmd_cache_attend_args* args, void* workspace, int64_t workspace_bytes, int32_t* status,
                      void* stream);
@@ -148,14 +149,14 @@ int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
 /* ---- pages --------------------------------------------------------------------- */
 
 /* Copies pages src[i] -> dst[i] (host arrays) of every layer. No dst may occur
- * twice or as a src. */
+ * twice or as a src (FMD_EINVAL). */
 int fmd_cache_copy_pages(const fmd_cache* c, int32_t n, const int32_t* src, const int32_t* dst, void* stream);
 
 /* Forks slots (host arrays): dst_slot[i] gets the first len[i] positions of
  * src_slot[i]: its page table row names the same full pages, and the len[i] % 64
  * rows behind them are copied, in every layer, to page new_page[i] (ignored when
  * there are none). No dst_slot may occur twice or as a src_slot, no new_page
- * twice or in a src_slot's row. */
+ * twice (FMD_EINVAL), and none in a src_slot's row. */
 int fmd_cache_fork(const fmd_cache* c, int32_t n, const int32_t* src_slot, const int32_t* dst_slot,
                    const int32_t* len, const int32_t* new_page, int32_t* status, void* stream);
 

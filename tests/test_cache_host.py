@@ -311,3 +311,33 @@ def test_reference_attention_of_one_key_is_its_value():
     wide, _ = ref.attend(q, k, v, [6, 7, 8], window=9)
     sunk, _ = ref.attend(q, k, v, [6, 7, 8], window=1, sinks=9)
     assert np.allclose(full, wide) and np.allclose(full, sunk)
+
+
+@pytest.mark.parametrize("fmt", [L.CACHE_BF16, L.CACHE_Q4])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_workspace_serves_smaller_calls(fmt, dim):
+    """The workspace for up to n_seqs sequences of up to max_rows rows is large
+    enough for every smaller call."""
+    lib = PKG.load_library()
+    c = C.byref(_c_cache(format=fmt, head_dim=dim))
+    for heads in (2, 16, 32):
+        sizes = [lib.fmd_cache_attend_workspace(c, heads, n, m) for n in (1, 64, 5000) for m in range(1, 40)]
+        sizes += [lib.fmd_cache_attend_workspace(c, heads, 5000, m) for m in (512, 4096, 100000)]
+        for n in range(3):
+            part = sizes[n * 39:(n + 1) * 39]
+            assert part == sorted(part) and part[0] > 0
+        assert sizes[-1] >= max(sizes)
+
+
+def test_c_entry_points_refuse_the_same_index_twice():
+    lib = PKG.load_library()
+    ia = lambda *v: (C.c_int32 * len(v))(*v)
+    cc = C.byref(_c_cache(n_pages=16, max_slots=8))
+    for src, dst in (((0, 1), (2, 2)), ((0, 1), (1, 2)), ((0, 1), (2, 1)), ((3,), (3,))):
+        assert lib.fmd_cache_copy_pages(cc, len(src), ia(*src), ia(*dst), None) == L.FMD_EINVAL
+    for src, dst, page in (((0, 0), (2, 2), (3, 4)), ((0, 1), (1, 2), (3, 4)), ((0, 1), (2, 0), (3, 4)),
+                           ((0, 0), (1, 2), (3, 3))):
+        assert lib.fmd_cache_fork(cc, 2, ia(*src), ia(*dst), ia(5, 70), ia(*page), None, None) == L.FMD_EINVAL
+    # queries are read until the last output is written
+    assert lib.fmd_cache_attend(cc, 0, C.byref(_c_rows()), C.byref(_c_attend(out=_c_attend().q)), 4096, 1 << 40, None,
+                                None) == L.FMD_EINVAL

@@ -731,6 +731,56 @@ def test_two_streams_and_two_graphs_at_the_same_time(kind):
     assert all(torch.equal(o, want[i]) for i in range(2) for o in outs[i])
 
 
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
+def test_one_workspace_for_calls_of_many_shapes(kind):
+    """A workspace made for the largest call serves the smaller ones, in any order."""
+    c, held = _filled(kind, "bf16", [700, 400, 90], seed=17)
+    for heads, most in ((4, 5), (4, 8), (4, 9), (4, 300), (2, 16)):
+        ws = c.workspace(heads, 3, most)
+        for counts in ([1, 1, 1], [most, 2, 1], [3, 1, 4], [min(most, 90)] * 3, [1, 1, 1]):
+            _check_attend(c, held, kind, "bf16", counts, [700, 400, 90], heads, workspace=ws)
+        assert not bool(ws[:PKG._lib.CACHE_WORKSPACE_ZERO].any())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
+def test_a_hidden_weight_of_a_large_value_leaves_the_small_ones_alone(kind):
+    """Values that differ by 2^24 between positions, the large ones with weights
+    that are nearly 0: the small ones keep their digits."""
+    rng = np.random.default_rng(18)
+    n, dim, heads = 200, 64, 2
+    c = _cache(kind, dim, 1, max_slots=1)
+    c.open(0)
+    rows = c.step([0], [n])
+    k, v = _rand(rng, n, 1, dim, scale=0.1), _rand(rng, n, 1, dim, scale=2.0 ** -10)
+    q = torch.ones(n, heads, dim, dtype=torch.bfloat16, device="cuda")
+    v[::7] *= 2.0**24
+    k[::7] = -4.0  # scores of -32 and about 0
+    c.append(0, rows, k, v)
+    kk, vv = (ref.quantise(_np(k))[0], ref.quantise(_np(v))[0]) if kind == "q4" else (_np(k), _np(v))
+    _check_attend(c, [(kk, vv)], kind, "bf16", [1], [n], heads, q=q[:1])
+    _check_attend(c, [(kk, vv)], kind, "bf16", [n - 20], [n], heads, q=q[:n - 20])
+
+
+def test_calls_that_would_race_are_refused():
+    import ctypes as C
+
+    c = _cache("bf16", 64, 1, n_pages=8, max_slots=4, max_pages=2)
+    ia = lambda *v: (C.c_int32 * len(v))(*v)
+    before = c.pool.clone()
+    lib, at = PKG.load_library(), C.byref(c._c)
+    for src, dst in (((0, 1), (2, 2)), ((0, 1), (1, 2))):
+        assert lib.fmd_cache_copy_pages(at, 2, ia(*src), ia(*dst), None) == PKG._lib.FMD_EINVAL
+    for src, dst, page in (((0, 0), (2, 2), (3, 4)), ((0, 1), (1, 2), (3, 4)), ((0, 0), (1, 2), (3, 3))):
+        assert lib.fmd_cache_fork(at, 2, ia(*src), ia(*dst), ia(5, 70), ia(*page), None, None) == PKG._lib.FMD_EINVAL
+    c.open(0)
+    rows = c.step([0], [1])
+    q = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(PKG.FmdError):
+        c.attend(0, rows, q, out=q)
+    torch.cuda.synchronize()
+    assert torch.equal(c.pool, before)
+
+
 def test_large_offsets_in_a_long_pool():
     """A pool above 4 GB: pages whose byte and element offsets pass 32 bits."""
     heads, dim, n_pages = 8, 128, 20000
