@@ -235,11 +235,12 @@ constexpr int kCkEntries = 1024;  // (sequence, tile) pairs of a split launch at
 // output cost, about two tiles.
 constexpr int kCkSetup = 2;
 constexpr int kCkLeast = 6;       // units of a range at least
-// What cutting costs a block, in units of about 1.2 us: the partials' way through memory
-// and the merge. 256 items of 70 units (two rounds of 148 blocks, 17 % of them idle) took
-// 175 us whole and 173 cut, 64 items of 72 units 90 us whole and 68 cut, 128 items of 3 to
-// 35 units 49 us whole and 55 cut.
-constexpr int kCkCut = 24;
+// What cutting costs a block, in units (1.2 us; 4 bits 1.5 us): the partials' way through
+// memory and the merge. 16 bits: 256 items of 70 units (two rounds of 148 blocks, 17 % of
+// them idle) take 173 us whole and 169 cut, 64 items of 72 units 88 and 65, 128 items of
+// 35 to 66 units 48 either way. 4 bits: the last 62 and 73, 128 items of 143 to 174 units
+// 267 and 242.
+constexpr int ck_cut(bool q4) { return q4 ? 24 : 16; }
 
 // This block's range of units, and the units before each (sequence, tile).
 struct CkPlan {
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
       const int items = H * (int)__reduce_add_sync(0xffffffffu, (unsigned)have), G = gridDim.x;
       most = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
       // whole items: the longest, or as many rounds of average ones; cut ones: an equal share
-      const bool whole = items > 0 && max((long long)most, (items + G - 1) / G * (units / items)) <= units / G + kCkCut;
+      const bool whole = items > 0 && max((long long)most, (items + G - 1) / G * (units / items)) <= units / G + ck_cut(Q4);
       if (whole) sum = have;
       int incl = sum;
 #pragma unroll
@@ -631,22 +632,43 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
       bool any = false;
       for (int j = w.j0; j < w.j1 && !any && ok; ++j) any = side.need(j);
       float m_ref = -INFINITY, l = 0.f, scale = p.a.scale * 1.4426950408889634f;
-      const int pr = side.first + row;
       const bool live = row < side.count;
-      const int pos = w.p0 + (pr >> gs);
+      const int pos = w.p0 + ((side.first + row) >> gs);
+      // queries come and outputs go through the query operand's rows, which the warp has to
+      // itself, with D / 8 lanes a row (a row a lane: 177 us instead of 172, two chunks of 2,048 rows
+      // over a window of 4,096)
+      constexpr int LR = D / 8, RL = 32 / LR;
+      const int ch = lane & (LR - 1);
+      auto row_of = [&](int i) { return q4 * 32 + i * RL + lane / LR; };  // step i's row of this lane
+      auto pair_at = [&](int r, long long row_stride, long long head_stride) {
+        const int pr = side.first + r;
+        return (size_t)(w.r0 + (pr >> gs)) * row_stride + (size_t)((w.h << gs) + (pr & ((1 << gs) - 1))) * head_stride;
+      };
+      auto chunk_at = [&](int r, int c8) {  // 16-byte chunk c8 of row r of the query operand
+        return reinterpret_cast<uint4*>(qp + x * QB + (c8 >> 3) * 2 * kCkBox + r * 128 + (((c8 & 7) ^ (r & 7)) << 4));
+      };
+      auto flush = [&]() {
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < LR; ++i)
+          if (row_of(i) < side.count)
+            *reinterpret_cast<uint4*>((T*)p.a.out + pair_at(row_of(i), p.a.out_row, p.a.out_head) + ch * 8) =
+                *chunk_at(row_of(i), ch);
+        __syncwarp();
+      };
       if (any) {
-        // ---- the query row into the operand tile. The last part's scores are complete (their
+        // ---- queries into the operand tile. The last part's scores are complete (their
         // s_full was waited for), so its queries are no longer read
-        const T* src = (const T*)p.a.q + (size_t)(w.r0 + (pr >> gs)) * p.a.q_row +
-                       (size_t)((w.h << gs) + (pr & ((1 << gs) - 1))) * p.a.q_head;
-        uint4 u[D / 8];
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          u[i] = live ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
+        uint4 u[LR];
         if constexpr (Q4) {
+          // a row a lane, for the row's scale
+          const T* src = (const T*)p.a.q + pair_at(row, p.a.q_row, p.a.q_head);
+#pragma unroll
+          for (int i = 0; i < LR; ++i)
+            u[i] = live ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
           float amax = 0.f;
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
+          for (int i = 0; i < LR; ++i) {
             const uint32_t v[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -659,20 +681,24 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
           const float up = __uint_as_float((uint32_t)(127 + e2) << 23);
           scale *= __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
+          for (int i = 0; i < LR; ++i) {
             uint32_t v[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float2 f = Act<T>::unpack2(v[e]);
               v[e] = Act<__half>::pack2(f.x * up, f.y * up);
             }
-            u[i] = make_uint4(v[0], v[1], v[2], v[3]);
+            *chunk_at(row, i) = make_uint4(v[0], v[1], v[2], v[3]);
           }
-        }
-        uint8_t* dst = qp + x * QB + row * 128;
+        } else {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          *reinterpret_cast<uint4*>(dst + (i >> 3) * 2 * kCkBox + (((i & 7) ^ (row & 7)) << 4)) = u[i];
+          for (int i = 0; i < LR; ++i)
+            u[i] = row_of(i) < side.count ? *reinterpret_cast<const uint4*>(
+                                                (const T*)p.a.q + pair_at(row_of(i), p.a.q_row, p.a.q_head) + ch * 8)
+                                          : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < LR; ++i) *chunk_at(row_of(i), ch) = u[i];
+        }
         ck_fence_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[x]);
@@ -787,8 +813,6 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
       const size_t pslot = 2 * blockIdx.x + (w.start < range.x0 ? 0 : 1);
       float4* pt = w.inside ? nullptr : reinterpret_cast<float4*>(p.part) + pslot * (D / 4) * 256 + x * 128 + row;
       const float inv = 1.f / l;
-      T* dst = (T*)p.a.out + (size_t)(w.r0 + (pr >> gs)) * p.a.out_row +
-               (size_t)((w.h << gs) + (pr & ((1 << gs) - 1))) * p.a.out_head;
       if (any) {
 #pragma unroll
         for (int h2 = 0; h2 < D / 32; ++h2) {
@@ -808,7 +832,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
               y.y = Act<T>::pack2(__uint_as_float(v[8 * i + 2]) * inv, __uint_as_float(v[8 * i + 3]) * inv);
               y.z = Act<T>::pack2(__uint_as_float(v[8 * i + 4]) * inv, __uint_as_float(v[8 * i + 5]) * inv);
               y.w = Act<T>::pack2(__uint_as_float(v[8 * i + 6]) * inv, __uint_as_float(v[8 * i + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + h2 * 32 + 8 * i) = y;
+              *chunk_at(row, h2 * 4 + i) = y;
             }
           }
         }
@@ -816,6 +840,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_empty[x]);
         ++items;
+        if (!pt) flush();
       }
       if (pt) {
         if (live) ml[pslot * 256 + x * 128 + row] = make_float2(m_ref, l);
@@ -872,9 +897,10 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
               y.y = Act<T>::pack2(acc[i].z * r, acc[i].w * r);
               y.z = Act<T>::pack2(acc[i + 1].x * r, acc[i + 1].y * r);
               y.w = Act<T>::pack2(acc[i + 1].z * r, acc[i + 1].w * r);
-              *reinterpret_cast<uint4*>(dst + (c0 + i) * 4) = y;
+              *chunk_at(k - x * 128, (c0 + i) / 2) = y;
             }
           }
+          flush();
         }
       }
     }
