@@ -158,14 +158,28 @@ class PagedCache:
             _fail("a slot is listed twice")
         for s in slots:
             self._open(s)
-        names, free = self._names, self._free
-        for s in slots:
-            for p in self._pages[s]:  # _drop, in line: many slots of many pages
+        names, free, common, m = self._names, self._free, [], 0
+
+        def drop(pages, n):
+            for p in pages:
                 if p >= 0:
-                    names[p] -= 1
+                    names[p] -= n
                     if not names[p]:
                         heapq.heappush(free, p)
+
+        for s in slots:
+            # slots that differ from the one before in their last page only, as forks do, give
+            # the others up together
+            pages = self._pages[s]
             self._pages[s], self._length[s] = None, 0
+            n = len(common)
+            if not n or pages[:n] != common:
+                drop(common, m)
+                common, m = pages[:-1], 0
+                n = len(common)
+            m += 1
+            drop(pages[n:], 1)
+        drop(common, m)
 
     def _drop(self, page: int) -> None:
         if page >= 0:
@@ -464,7 +478,7 @@ class PagedCache:
         src, dst = list(src), list(dst)
         if len(src) != len(dst):
             _fail("src and dst must be as long")
-        if any(not 0 <= p < self.n_pages for p in src + dst):
+        if src and not 0 <= min(min(src), min(dst)) <= max(max(src), max(dst)) < self.n_pages:
             _fail("page out of range")
         if len(set(dst)) != len(dst) or set(dst) & set(src):
             _fail("a page is written twice, or read and written")
@@ -489,7 +503,9 @@ class PagedCache:
         if part and len(dsts) > len(self._free):
             _fail("the cache has too few free pages", _lib.FMD_ENOMEM)
         m, shared, names = len(dsts), pages[:full], self._names
-        fresh = [self._take() if part else -1 for _ in dsts]
+        fresh = [heapq.heappop(self._free) for _ in dsts] if part else [-1] * m
+        for p in fresh if part else ():
+            names[p] = 1
         for d, p in zip(dsts, fresh):
             self._pages[d] = shared + [p] if part else shared.copy()
             self._length[d] = n

@@ -33,6 +33,15 @@
 // Registers go where they are needed: the softmax groups take what the others give.
 // Values of positions that no pair of the item sees are cleared in shared memory
 // before the product, so that what they hold (NaN x 0) has no influence.
+// Measured (16 query heads to 8 kv heads of 128): 2,048 rows behind 8,192 positions
+// 138 us, 870 TFLOP/s; two such chunks over a window of 4,096 168.5 us, 817 TFLOP/s;
+// 2,001 f16 rows behind 9,001 positions in 4 bits 241 us, 543 TFLOP/s of the 4 x head_dim a
+// key (twice the products of P V are issued there). A key tile of A and B takes 2,000
+// cycles (4 bits: 4,000), an item's queries and outputs 8,000 more. Of the 2,000, a
+// softmax warp spends 900 on its exponentials, the special-function unit half busy with
+// those of A and B; no pipe is full (tensor 44 %, issue 37 %). A quarter of the
+// exponentials as polynomials took 177 us instead of 173, half of them 183; one score
+// buffer beside a P of its own, which lets S(j + 1) start before P V (j - 1), 185.
 // Every wait is bounded; a timeout sets the status word, stops issuing work,
 // waits (bounded) for copies and MMAs in flight and frees tensor memory.
 #include <cuda.h>
