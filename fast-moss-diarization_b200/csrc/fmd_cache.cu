@@ -15,18 +15,18 @@ namespace {
 // ---- rows ---------------------------------------------------------------------------
 //
 // append and read are bound by the bytes they move, as long as their instructions
-// stay few. A block of two warps takes one row (with few rows, some of its heads);
-// L = D / 8 lanes take a head, 8 dims (16 bytes) each, so that every access is a
+// stay few. A block of one warp (read: two) takes one row, with few rows some of its
+// heads; L = D / 8 lanes take a head, 8 dims (16 bytes) each, so that every access is a
 // full sector, and each lane has HPG heads' loads in flight before it looks up the
-// row's sequence, position and page, which they do not need. Two warps, not eight:
-// that lookup and the addresses cost about 400 instructions a warp, as much as
-// four heads.
+// row's sequence, position and page, which they do not need. One warp, not eight: that
+// lookup and the addresses cost about 400 instructions a warp, as much as four heads.
 
-constexpr int kRowThreads = 64;
-constexpr int kRowHeads = 2;  // heads a lane has in flight, with many rows
-// Blocks of an SM: 64 registers a thread, a few spilled for 4 bits. 10,007 and 16,384 (4 bits)
-// rows of 32 heads took 41.5 and 79 us so, 42.5 and 80 with 14 blocks, 51 and 92 with 10.
-constexpr int kRowBlocks = 16;
+constexpr int kRowThreads = 32;
+// Heads a lane has in flight, with many rows, and the blocks of an SM (80 registers a
+// thread). 10,007 rows of 32 heads with norms and rotation, 16 bits, and 16,384 of 16 heads
+// into 4 bits: 34.7 and 35.7 us; 39.9 and 38.0 with 2 heads and 32 blocks, 44.9 and 46.1 with
+// 8 and 16, 38.5 and 40.3 with two warps, 2 heads and 16 blocks.
+constexpr int kRowHeads = 4, kRowBlocks = 24;
 
 // What a row is stored as: its position's place in a page, and the page's first
 // block in the layer. False where the row takes no part.
@@ -161,8 +161,8 @@ FMD_DEV uint32_t quantise8(float (&x)[8], bool key, __half& scale) {
 // about 10 flop a byte at most, far below the memory's. The queries', keys' and
 // values' heads are passed over one after the other, so that what is done with a
 // head is the same for the whole block. 10,007 rows of 16 + 8 + 8 heads with norms and
-// rotation, 16 bits: 41.5 us, 4.1 TB/s, two thirds of the issue slots used; 16,384 rows
-// into 4 bits: 79 us, 79 % of them. One row: 2.6 us, 64 rows 2.9.
+// rotation, 16 bits: 34.7 us, 4.9 TB/s; 16,384 rows of 8 + 8 heads into 4 bits 35.7 us, 2.4
+// TB/s, the quantiser's instructions. One row: 2.6 us, 64 rows 2.9.
 template <typename T, int D, bool Q4, int HPG>
 __global__ void __launch_bounds__(kRowThreads, kRowBlocks)
     k_cache_append(CacheView c, int layer, CacheRows r, CacheAppend a, int* status) {
@@ -321,10 +321,13 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks)
 // ---- read ---------------------------------------------------------------------------
 //
 // 32,768 rows of 8 heads of 128 to f32: 74.5 us from 16 bits, 5.4 TB/s, 68 us from 4.
+// Two warps a row: 24.3 us for 10,007 rows in 16 bits, 26.6 with one.
+constexpr int kReadThreads = 64;
+
 template <int D, int FORMAT>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kReadThreads)
     k_cache_read(CacheView c, int layer, CacheRows r, float* k, float* v, int* status) {
-  constexpr int L = D / 8, GROUPS = kRowThreads / L, HPG = 4;
+  constexpr int L = D / 8, GROUPS = kReadThreads / L, HPG = 4;
   constexpr bool Q4 = FORMAT == FMD_CACHE_Q4;
   constexpr int BB = Q4 ? kPageTokens * (D / 2 + D / 16) : kPageTokens * D * 2;
   griddep_wait();
@@ -570,7 +573,7 @@ cudaError_t launch_dep(void (*kern)(KArgs...), dim3 grid, dim3 block, cudaStream
 cudaError_t launch_cache_append(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAppend& a,
                                 int* status, cudaStream_t s) {
   // With few rows a lane takes one head and a row as many blocks as its heads fill:
-  // one row of 32 heads 2.6 us so, 4.75 as one block with two heads a lane.
+  // one row of 32 heads 2.6 us so, 4.75 as one block of two warps with two heads a lane.
   const bool few = r.n_rows < 148 * 4;
   const int g = kRowThreads / (c.head_dim / 8);
   const int passes = (a.n_heads + g - 1) / g + 2 * ((c.kv_heads + g - 1) / g);
@@ -736,14 +739,14 @@ int fmd_cache_read(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows
   if (rows->n_seqs == 0 || rows->n_rows == 0) return FMD_OK;
   if (!on_current_device(c->pool) || !on_current_device(k)) return FMD_EINVAL;
   // blocks of a row: as in append
-  const int per_block = kRowThreads / (c->head_dim / 8) * 4, most = (2 * c->kv_heads + per_block - 1) / per_block;
+  const int per_block = kReadThreads / (c->head_dim / 8) * 4, most = (2 * c->kv_heads + per_block - 1) / per_block;
   const dim3 grid(rows->n_rows, rows->n_rows < 148 * 4 ? most : 1);
   auto go = [&](auto d) {
     constexpr int D = decltype(d)::value;
     return launch_dep(c->format == FMD_CACHE_Q4     ? k_cache_read<D, FMD_CACHE_Q4>
                       : c->format == FMD_CACHE_BF16 ? k_cache_read<D, FMD_CACHE_BF16>
                                                     : k_cache_read<D, FMD_CACHE_F16>,
-                      grid, dim3(kRowThreads), (cudaStream_t)stream, view_of(c), layer, rows_of(rows), k, v, status);
+                      grid, dim3(kReadThreads), (cudaStream_t)stream, view_of(c), layer, rows_of(rows), k, v, status);
   };
   return done(c->head_dim == 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 64>{}));
 }
