@@ -660,6 +660,10 @@ int check_rows(const fmd_cache* c, int32_t layer, const fmd_cache_rows* r) {
 }
 
 bool bad_stride(int64_t s) { return s < 0 || (s & 7); }
+// Output rows or heads on top of one another.
+bool overlaps(int64_t row, int64_t head, int n_rows, int n_heads) {
+  return (row == 0 && n_rows > 1) || (head == 0 && n_heads > 1);
+}
 
 CacheView view_of(const fmd_cache* c) {
   return CacheView{(uint8_t*)c->pool, c->page_table, c->format,    c->n_pages,
@@ -722,6 +726,7 @@ int fmd_cache_append(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
   if (a->q)
     for (int64_t s : {a->q_row, a->q_head, a->q_out_row, a->q_out_head})
       if (bad_stride(s)) return FMD_EINVAL;
+  if (a->q && overlaps(a->q_out_row, a->q_out_head, rows->n_rows, a->n_heads)) return FMD_EINVAL;
   if (rows->n_seqs == 0 || rows->n_rows == 0) return FMD_OK;
   if (!on_current_device(c->pool) || !on_current_device(a->k)) return FMD_EINVAL;
   CacheAppend p{a->q,      a->k,      a->v,     a->q_out,     a->q_row,     a->q_head, a->k_row,
@@ -771,6 +776,7 @@ int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
   if (a->window < 0 || a->sinks < 0 || !(a->scale > 0.f) || !(a->scale <= 3.4e38f)) return FMD_EINVAL;
   for (int64_t s : {a->q_row, a->q_head, a->out_row, a->out_head})
     if (bad_stride(s)) return FMD_EINVAL;
+  if (overlaps(a->out_row, a->out_head, rows->n_rows, a->n_heads)) return FMD_EINVAL;
   if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return FMD_OK;
   const int64_t need = fmd_cache_attend_workspace(c, a->n_heads, rows->n_seqs, rows->max_rows);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return FMD_EINVAL;

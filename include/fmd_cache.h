@@ -19,7 +19,8 @@
  *    range is skipped, never accessed, and `status` (2 x int32, may be NULL)
  *    receives FMD_EINVAL (slot or page number) or FMD_EOVERFLOW (position).
  *  - Row pointers are 16-byte aligned and row and head strides are multiples
- *    of 8 elements; the dims of a head are contiguous.
+ *    of 8 elements; the dims of a head are contiguous. Inputs may repeat a row or
+ *    a head with a stride of 0, outputs may not.
  */
 #ifndef FMD_CACHE_H
 #define FMD_CACHE_H

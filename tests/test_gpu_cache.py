@@ -777,8 +777,23 @@ def test_calls_that_would_race_are_refused():
     q = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(PKG.FmdError):
         c.attend(0, rows, q, out=q)
+    # one row or one head for all of an output, but not of an input
+    c.open(1)
+    rows = c.step([0, 1], [1, 1])
+    q, kv = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros_like(before[:256]).view(torch.bfloat16)
+    kv = kv[:64].expand(2, 1, 64)
+    for out in (q[:1].clone().expand(2, 2, 64), q[:, :1].clone().expand(2, 2, 64)):
+        with pytest.raises(PKG.FmdError):
+            c.attend(0, rows, q, out=out)
+        with pytest.raises(PKG.FmdError):
+            c.append(0, rows, kv, kv, q=q, q_out=out)
     torch.cuda.synchronize()
     assert torch.equal(c.pool, before)
+    kv = _rand(np.random.default_rng(0), 64).expand(2, 1, 64)
+    assert torch.equal(c.append(0, rows, kv, kv, q=kv.expand(2, 2, 64)), kv.expand(2, 2, 64))
+    c.check()
+    for s in (0, 1):
+        assert torch.equal(_values(c, s, 0)[0].to(torch.bfloat16)[-1], kv[0])
 
 
 def test_large_offsets_in_a_long_pool():
