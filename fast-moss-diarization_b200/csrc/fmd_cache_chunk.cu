@@ -27,7 +27,7 @@
 //  * warps 4-7 / 8-11: the softmax of A / B, one thread per pair: a lazily moved
 //    reference m (2^8 of headroom), P as 16-bit values over the scores it came from, the
 //    A operand of its product with V, O rescaled only when m moves;
-//  * 4 bits: warps 12-19 turn the codes into f16 tiles, (c - 8) d with one rounding,
+//  * 4 bits: warps 12-15 turn the codes into f16 tiles, (c - 8) d with one rounding,
 //    keys and values; the queries are then f16 too, scaled by a power of two per
 //    row.
 // Registers go where they are needed: the softmax groups take what the others give.
@@ -35,9 +35,9 @@
 // before the product, so that what they hold (NaN x 0) has no influence.
 // Measured (16 query heads to 8 kv heads of 128): 2,048 rows behind 8,192 positions
 // 138 us, 870 TFLOP/s; two such chunks over a window of 4,096 168.5 us, 817 TFLOP/s;
-// 2,001 f16 rows behind 9,001 positions in 4 bits 241 us, 543 TFLOP/s of the 4 x head_dim a
+// 2,001 f16 rows behind 9,001 positions in 4 bits 234 us, 560 TFLOP/s of the 4 x head_dim a
 // key (twice the products of P V are issued there). A key tile of A and B takes 2,000
-// cycles (4 bits: 4,000), an item's queries and outputs 8,000 more. Of the 2,000, a
+// cycles (4 bits: 3,900), an item's queries and outputs 8,000 more. Of the 2,000, a
 // softmax warp spends 900 on its exponentials, the special-function unit half busy with
 // those of A and B; no pipe is full (tensor 44 %, issue 37 %). A quarter of the
 // exponentials as polynomials took 177 us instead of 173, half of them 183; one score
@@ -61,9 +61,12 @@ constexpr int kCkMaxStages = 4;
 constexpr uint32_t kCkWait = 1u << 24;
 constexpr float kCkHeadroom = 8.f;
 
-constexpr int ck_threads(bool q4) { return q4 ? 640 : 384; }
+constexpr int kCkConv = 4;  // converter warps (4 bits)
+constexpr int ck_threads(bool q4) { return 384 + (q4 ? kCkConv * 32 : 0); }
 // Registers of a thread at launch, of a softmax thread, of any other; the sums fit.
-//   16 bits: 384 x 168 = 256 x 208 + 128 x 88; 4 bits: 640 x 96 > 256 x 152 + 384 x 56
+//   16 bits: 384 x 168 = 256 x 208 + 128 x 88; 4 bits: 512 x 128 = 256 x 192 + 256 x 64.
+// Eight converter warps leave 152 to a softmax thread, which then spills: 2,048 rows over 2,048
+// to 4,096 keys 62 us instead of 55.5, the f16 chunk above 241 instead of 234.
 template <int N> FMD_DEV void ck_more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
 template <int N> FMD_DEV void ck_fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
 
@@ -247,8 +250,8 @@ constexpr int kCkLeast = 6;       // units of a range at least
 // What cutting costs a block, in units (1.2 us; 4 bits 1.5 us): the partials' way through
 // memory and the merge. 16 bits: 256 items of 70 units (two rounds of 148 blocks, 17 % of
 // them idle) take 173 us whole and 169 cut, 64 items of 72 units 88 and 65, 128 items of
-// 35 to 66 units 48 either way. 4 bits: the last 62 and 73, 128 items of 143 to 174 units
-// 267 and 242.
+// 35 to 66 units 48 either way. 4 bits: the last 56 and 60, 128 items of 143 to 174 units
+// 261 and 234.
 constexpr int ck_cut(bool q4) { return q4 ? 24 : 16; }
 
 // This block's range of units, and the units before each (sequence, tile).
@@ -325,7 +328,7 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
   constexpr int BLK = Q4 ? 64 * (D / 2 + D / 16) : 64 * D * 2;  // K or V of a page as stored
   constexpr int TB = 64 * D * 2;                              // K or V of a page as an operand
   constexpr int NB = D / 32;
-  constexpr int kMore = Q4 ? 152 : 208, kFew = Q4 ? 56 : 88;
+  constexpr int kMore = Q4 ? 192 : 208, kFew = Q4 ? 64 : 88;
   // f16 outputs of a 4-bit cache: P and V go in as two f16 terms each (their roundings,
   // 2^-11 each as the output's, would be two of the three that f16 operands cost;
   // error against 64 bits 3.8e-4 without, 2.1e-4 for the output's rounding alone)
@@ -354,11 +357,11 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], Q4 ? 8 : 2);
+      mbar_init(&kv_empty[s], Q4 ? kCkConv : 2);
     }
     for (int x = 0; x < 2; ++x) {
       for (int b = 0; b < 2; ++b) {
-        mbar_init(&cv_full[x][b], 8);
+        mbar_init(&cv_full[x][b], kCkConv);
         mbar_init(&cv_empty[x][b], 2);
       }
       mbar_init(&mma_done[x], 1);
@@ -937,11 +940,15 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
         uint8_t* dst = cvp + b * CVB;
         const bool bad = bad_s[s];
         if (tid == 12 * 32) cbad_s[(round_b * 2 + b) & 3] = bad;
-        // 8 keys per warp; a lane takes chunk lane & 3 of a key, keys 4 apart in a
+        // 8 keys a pass of a warp; a lane takes chunk lane & 3 of a key, keys 4 apart in a
         // quarter-warp, whose swizzled rows share no banks
-        const int kk = lane >> 2, key = cw * 8 + (kk & 1) * 4 + (kk >> 1), ch = lane & 3;
+        constexpr int PASS = 8 / kCkConv;
+        const int kk = lane >> 2, ch = lane & 3;
+        auto key_of = [&](int ps) { return (cw + ps * kCkConv) * 8 + (kk & 1) * 4 + (kk >> 1); };
         constexpr int CB = 64 * D / 2;  // code bytes of a block
-        {
+#pragma unroll
+        for (int ps = 0; ps < PASS; ++ps) {
+          const int key = key_of(ps);
           // a key chunk: word g holds dims 32 g + 8 ch .. + 7
           uint32_t wd[NB], d2[NB];
           if constexpr (NB == 4) {
@@ -971,40 +978,48 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&cv_full[0][b]);
         // a value chunk: its words are dims in order
-        uint32_t wd[NB];
-        if constexpr (NB == 4) {
-          const uint4 u = *reinterpret_cast<const uint4*>(src + BLK + key * 64 + ch * 16);
-          wd[0] = u.x, wd[1] = u.y, wd[2] = u.z, wd[3] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(src + BLK + key * 32 + ch * 8);
-          wd[0] = u.x, wd[1] = u.y;
+        uint32_t wd[PASS][NB], dv[PASS];
+#pragma unroll
+        for (int ps = 0; ps < PASS; ++ps) {
+          const int key = key_of(ps);
+          if constexpr (NB == 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(src + BLK + key * 64 + ch * 16);
+            wd[ps][0] = u.x, wd[ps][1] = u.y, wd[ps][2] = u.z, wd[ps][3] = u.w;
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(src + BLK + key * 32 + ch * 8);
+            wd[ps][0] = u.x, wd[ps][1] = u.y;
+          }
+          dv[ps] = *reinterpret_cast<const uint16_t*>(src + BLK + CB + key * NB * 2 + (NB == 4 ? ch : ch >> 1) * 2);
+          const int kp = k0 + key;
+          const bool hide = bad || kp > top || (W && kp <= w.lo[0] - W && kp >= S);
+          dv[ps] = hide ? 0u : dv[ps] | dv[ps] << 16;
         }
-        uint32_t dv = *reinterpret_cast<const uint16_t*>(src + BLK + CB + key * NB * 2 + (NB == 4 ? ch : ch >> 1) * 2);
         __syncwarp();
         if (lane == 0) mbar_arrive(&kv_empty[s]);  // this warp has read its part of the stage
-        const int kp = k0 + key;
-        const bool hide = bad || kp > top || (W && kp <= w.lo[0] - W && kp >= S);
-        dv = hide ? 0u : dv | dv << 16;
         if (round_b > 0 && !ck_wait(&cv_empty[1][b], (round_b - 1) & 1, abort_v)) {
           ok = false;
           break;
         }
 #pragma unroll
-        for (int g = 0; g < NB; ++g) {
-          // nibbles 2 i, 2 i + 1 side by side: bytes of the even and the odd ones interleaved
-          const uint32_t ev = (wd[g] << 4) & 0xf0f0f0f0u, od = wd[g] & 0xf0f0f0f0u;
-          const uint32_t c4[4] = {__byte_perm(ev, od, 0x0400), __byte_perm(ev, od, 0x0501), __byte_perm(ev, od, 0x0602),
-                                  __byte_perm(ev, od, 0x0703)};
-          uint32_t o[4], rest[4];
+        for (int ps = 0; ps < PASS; ++ps) {
+          const int key = key_of(ps);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            o[i] = ck_sub_mul((c4[i] & 0x00ff00ffu) | f64, k72, dv);
-            if constexpr (kFine) rest[i] = ck_sub_mul_rest((c4[i] & 0x00ff00ffu) | f64, k72, dv, o[i]);
+          for (int g = 0; g < NB; ++g) {
+            // nibbles 2 i, 2 i + 1 side by side: bytes of the even and the odd ones interleaved
+            const uint32_t ev = (wd[ps][g] << 4) & 0xf0f0f0f0u, od = wd[ps][g] & 0xf0f0f0f0u;
+            const uint32_t c4[4] = {__byte_perm(ev, od, 0x0400), __byte_perm(ev, od, 0x0501), __byte_perm(ev, od, 0x0602),
+                                    __byte_perm(ev, od, 0x0703)};
+            uint32_t o[4], rest[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              o[i] = ck_sub_mul((c4[i] & 0x00ff00ffu) | f64, k72, dv[ps]);
+              if constexpr (kFine) rest[i] = ck_sub_mul_rest((c4[i] & 0x00ff00ffu) | f64, k72, dv[ps], o[i]);
+            }
+            const int oc = NB * ch + g;
+            uint8_t* at = dst + TB + (oc >> 3) * kCkBox + key * 128 + (((oc & 7) ^ (key & 7)) << 4);
+            *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
+            if constexpr (kFine) *reinterpret_cast<uint4*>(at + TB) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
           }
-          const int oc = NB * ch + g;
-          uint8_t* at = dst + TB + (oc >> 3) * kCkBox + key * 128 + (((oc & 7) ^ (key & 7)) << 4);
-          *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
-          if constexpr (kFine) *reinterpret_cast<uint4*>(at + TB) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
         }
         ck_fence_async();
         __syncwarp();
