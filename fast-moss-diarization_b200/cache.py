@@ -59,7 +59,10 @@ class PagedCache:
     `64 * max_pages_per_slot` positions. `kind`: "f16" or "bf16" (rows of that
     dtype) or "q4" (rows of either). `pool` and `page_table` may be the caller's
     (uint8 of `pool_bytes`, int32 `[max_slots, max_pages_per_slot]`), with
-    `slots` as `(slot, its pages, its length)` for what they hold already."""
+    `slots` as `(slot, its pages, its length)` for what they hold already. One host
+    thread at a time may change the bookkeeping (open, step, fork, evict, release,
+    compact); the operators may run on several streams, as long as no call writes
+    what another reads."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, n_pages: int, max_slots: int,
                  max_pages_per_slot: int, kind: str = "bf16", device="cuda", pool=None, page_table=None, slots=()):

@@ -241,6 +241,16 @@ def test_attend_one_long_sequence(kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "q4"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads", [1, 2, 16])
+def test_attend_one_segment_over_the_whole_grid(kind, dim, heads):
+    """One kv head: every block has a piece of the same segment."""
+    c, held = _filled(kind, "bf16", [20011], dim, 1, seed=3)
+    for count in (1, 3):
+        _check_attend(c, held, kind, "bf16", [count], [20011], heads)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
 def test_attend_many_sequences_of_several_rows(kind):
     """So many (sequence, tile) pairs that items are dealt out whole."""
     counts = [40 - i % 9 for i in range(300)]
