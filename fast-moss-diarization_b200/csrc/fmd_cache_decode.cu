@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kDc16Threads, 2)
       const int cnt = min(32, ntl - b0);
       for (int i = 0; i < cnt; ++i) {
         const int h = __shfl_sync(0xffffffffu, lh, i), page = __shfl_sync(0xffffffffu, lpage, i);
-        if (round > 0 && !mbar_wait_bounded(&empty[s], (round - 1) & 1, kDcWait)) {
+        if (round > 0 && !mbar_wait_warp(&empty[s], (round - 1) & 1, kDcWait)) {
           ok = false;
           break;
         }
@@ -554,7 +554,8 @@ __global__ void __launch_bounds__(kDc16Threads, 2)
           qf[n][ks][b] = pr < nq ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + b * 8 + 2 * t) : 0u;
     }
     for (int j = cj; j < cj + len; ++j) {
-      if (!aborted && !mbar_wait_bounded(&full[s], phase, kDcWait)) aborted = true;
+      // one outcome for the warp: what follows is warp-wide
+      if (!aborted && !mbar_wait_warp(&full[s], phase, kDcWait)) aborted = true;
       // keys k0 .. k0 + 15 of this warp
       const int k0 = keys.unit(j) * 64 + warp * 16;
       const bool whole = k0 + 15 <= p0 && (W == 0 || k0 > p1 - W || k0 + 15 < S);
