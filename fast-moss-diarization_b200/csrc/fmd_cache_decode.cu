@@ -1001,6 +1001,16 @@ DcShape dc_shape(const CacheView& c, int rows) {
   }
 }
 
+// The shared memory of the largest call of the kernel that takes segments of `rows`
+// pairs. The limit belongs to the function, not to a call: every call sets this one
+// value, so that calls of other shapes, from other host threads, do not lower it
+// between another's setting and its launch.
+int dc_limit(const CacheView& c, int rows) {
+  int most = 0;
+  for (int r = rows <= 8 ? 1 : 9; r <= (rows <= 8 ? 8 : 16); ++r) most = std::max(most, dc_shape(c, r).smem);
+  return most;
+}
+
 }  // namespace
 
 bool cache_decode_fits(const CacheView& c, int n_heads, int max_rows) {
@@ -1040,6 +1050,7 @@ cudaError_t launch_cache_decode(bool bf16, const CacheView& c, int layer, const 
   const bool q4 = c.format == FMD_CACHE_Q4;
   const int rows = a.max_rows * (a.n_heads / c.kv_heads), D = c.head_dim;
   const DcShape sh = dc_shape(c, rows);
+  const int limit = dc_limit(c, rows);
   CUtensorMap map{};
   if (!q4 && !cache_tensor_map(&map, c, layer)) return cudaErrorNotSupported;
   DcArgs p;
@@ -1054,7 +1065,7 @@ cudaError_t launch_cache_decode(bool bf16, const CacheView& c, int layer, const 
   p.red_row = sh.red_row;
   p.f64 = 0x54005400u;
   auto each = [&](auto kern, auto&&... head) -> cudaError_t {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.smem);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
     for (int s0 = 0; e == cudaSuccess && s0 < r.n_seqs; s0 += p.seqs) {
       p.seq0 = s0;
       cudaLaunchAttribute attr;

@@ -1,0 +1,80 @@
+"""Calls of the paged-cache operators as programs make them: from several host
+threads, in graphs of several shapes, with empty batches and odd outputs."""
+
+from __future__ import annotations
+
+import ctypes as C
+import threading
+
+import numpy as np
+import pytest
+
+from conftest import PKG
+from test_gpu_cache import _filled, _rand, _seq_rows
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind,dim", [("bf16", 128), ("q4", 128), ("f16", 64)])
+def test_two_host_threads_with_different_shapes(kind, dim):
+    """Each thread has a cache and a stream of its own; their calls differ in the
+    query heads of a kv head, and so in the shared memory that they ask for."""
+    dtype = "f16" if kind == "f16" else "bf16"
+    jobs, failed = [], []
+    for i, group in enumerate((1, 2, 4, 8)):
+        c, _ = _filled(kind, dtype, [40 + i], dim=dim, seed=i)
+        q = _rand(np.random.default_rng(i), 1, 2 * group, dim, dtype=dtype)
+        rows = _seq_rows(c, [0], [1], [40 + i])
+        out = torch.zeros_like(q)
+        # the C entry with its arguments at hand, so that the threads are in it most of the time
+        args = PKG._lib.CacheAttendArgs(q.data_ptr(), out.data_ptr(), *q.stride()[:2], *out.stride()[:2], dim ** -0.5,
+                                        c._dtype(q, "q"), q.shape[1], 0, 0)
+        ws = c.workspace(q.shape[1], 1)
+        call = (c._ref, 0, c._rows_c(rows, 1), C.byref(args), ws.data_ptr(), ws.numel(), c._status_at)
+        jobs.append((c, call, out, c.attend(0, rows, q).clone(), (q, args, ws, rows)))
+    torch.cuda.synchronize()
+    start = threading.Barrier(len(jobs))
+
+    def work(c, call, out, want, keep):
+        stream = torch.cuda.Stream()
+        torch.cuda.set_device(0)
+        start.wait()
+        codes = {c.lib.fmd_cache_attend(*call, stream.cuda_stream) for _ in range(10000)}
+        stream.synchronize()
+        if codes != {PKG._lib.FMD_OK} or not torch.equal(out, want):
+            failed.append((codes, keep[0].shape))
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for c, *_ in jobs:
+        c.check()
+    assert not failed, failed
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_graph_of_calls_of_many_shapes(kind, dim):
+    """Calls that ask for different amounts of shared memory, captured into one
+    graph, with others made before it is replayed."""
+    lengths = [200, 90]
+    c, _ = _filled(kind, "bf16", lengths, dim=dim)
+    shapes = [(heads, n) for heads in (2, 8, 16, 32) for n in (1, 2, 40)]
+    calls = [(_seq_rows(c, [0, 1], [n, n], lengths),
+              _rand(np.random.default_rng(heads + n), 2 * n, heads, dim)) for heads, n in shapes]
+    want = [c.attend(0, rows, q).clone() for rows, q in calls]
+    outs = [torch.zeros_like(q) for _, q in calls]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for (rows, q), out in zip(calls, outs):
+            c.attend(0, rows, q, out=out)
+    for rows, q in reversed(calls):
+        c.attend(0, rows, q)
+    for _ in range(2):
+        g.replay()
+    c.check()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
