@@ -48,8 +48,9 @@ class CacheRows:
     max_rows: int
 
     def advance(self, n: int = 1) -> None:
-        """Move every sequence on by `n` positions, on the device (the pages
-        must be there: `PagedCache.reserve`)."""
+        """Move every sequence on by `n` positions, on the device, for launches
+        whose positions no `step` gave out (a captured graph's). The cache's books
+        follow by `PagedCache.advance`, called before those launches."""
         self.pos0.add_(n)
 
 
@@ -223,6 +224,29 @@ class PagedCache:
         import torch
 
         slots, counts = list(slots), list(counts)
+        pos0 = self._extend(slots, counts)
+        row0 = None
+        if any(n != 1 for n in counts):
+            row0 = [0]
+            for n in counts:
+                row0.append(row0[-1] + n)
+        dev = self.device
+        return CacheRows(torch.tensor(slots, dtype=torch.int32).to(dev), torch.tensor(pos0, dtype=torch.int32).to(dev),
+                         None if row0 is None else torch.tensor(row0, dtype=torch.int32).to(dev), sum(counts),
+                         max(counts, default=0))
+
+    def advance(self, slots, n: int = 1) -> None:
+        """The books of `n` new positions of each slot, as `step` keeps them, for
+        rows that move on by themselves (`CacheRows.advance`, a replayed graph): call
+        it before the launches that write the positions, so that their pages are
+        there and the slot's own, and `length`, `step`, `fork` and `evict` know of
+        them."""
+        slots = list(slots)
+        self._extend(slots, [n] * len(slots))
+
+    def _extend(self, slots, counts) -> list:
+        """Make `counts[i]` new positions part of each slot, with pages of its own
+        for them; returns the slots' lengths before."""
         if len(slots) != len(counts) or any(n < 0 for n in counts):
             _fail("one count >= 0 per slot")
         if len(set(slots)) != len(slots):
@@ -255,15 +279,7 @@ class PagedCache:
         pos0 = [self._length[s] for s in slots]
         for s, n in zip(slots, counts):
             self._length[s] += n
-        row0 = None
-        if any(n != 1 for n in counts):
-            row0 = [0]
-            for n in counts:
-                row0.append(row0[-1] + n)
-        dev = self.device
-        return CacheRows(torch.tensor(slots, dtype=torch.int32).to(dev), torch.tensor(pos0, dtype=torch.int32).to(dev),
-                         None if row0 is None else torch.tensor(row0, dtype=torch.int32).to(dev), sum(counts),
-                         max(counts, default=0))
+        return pos0
 
     def rows(self, slot, pos0, row0=None, max_rows: int = 1, n_rows: int | None = None) -> CacheRows:
         """Rows from device tensors of the caller (a device-side scheduler, a

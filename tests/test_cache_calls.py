@@ -1,0 +1,42 @@
+"""The paged cache's books and argument checks, on the CPU: calls beside those
+of test_cache_host."""
+
+from __future__ import annotations
+
+import pytest
+
+from conftest import PKG
+from test_cache_host import HostCache, _consistent
+
+torch = pytest.importorskip("torch")
+L = PKG._lib
+
+
+def test_books_follow_rows_that_move_on_by_themselves():
+    c = HostCache(n_pages=12)
+    c.open(0, 130), c.open(1)
+    c.step([0, 1], [126, 64])
+    for _ in range(4):
+        c.advance([0, 1])
+    assert c.length(0) == 130 and c.length(1) == 68 and len(c.pages(1)) == 2
+    _consistent(c)
+    c.fork(0, [2])
+    assert c.length(2) == 130 and c.pages(2)[:2] == c.pages(0)[:2] and c.pages(2)[2] != c.pages(0)[2]
+    r = c.step([0, 1], [1, 1])
+    assert r.pos0.tolist() == [130, 68]
+    # pages that are shared become the slot's own before they are written; full ones stay shared
+    c.calls.clear()
+    c.release(2)
+    shared = HostCache(n_pages=8, slots=[(0, [3], 10), (1, [3], 10)])
+    shared._upload(0, 0), shared._upload(1, 0)
+    shared.advance([1], 5)
+    assert shared.calls == ["fmd_cache_copy_pages"] and shared.pages(0) == [3] and shared.pages(1) == [0]
+    assert shared.length(1) == 15
+    _consistent(c), _consistent(shared)
+    for slots, n, status in (([0, 0], 1, L.FMD_EINVAL), ([3], 1, L.FMD_EINVAL), ([0], -1, L.FMD_EINVAL),
+                             ([0], 400, L.FMD_EOVERFLOW)):
+        with pytest.raises(PKG.FmdError) as e:
+            c.advance(slots, n)
+        assert e.value.status == status
+    assert c.length(0) == 131
+    _consistent(c)

@@ -9,8 +9,9 @@ import threading
 import numpy as np
 import pytest
 
+import cache_ref as ref
 from conftest import PKG
-from test_gpu_cache import _filled, _rand, _seq_rows
+from test_gpu_cache import _eps, _filled, _np, _rand, _seq_rows
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -78,3 +79,57 @@ def test_a_graph_of_calls_of_many_shapes(kind, dim):
         g.replay()
     c.check()
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
+def test_steps_and_forks_after_replayed_steps(kind):
+    """A captured step is replayed; the cache's books, told by `advance`, then serve
+    a fork and further steps, and nothing that was written is lost."""
+    c = PKG.PagedCache(1, 2, 128, 12, 3, 4, kind=kind)
+    c.open(0)
+    rng = np.random.default_rng(3)
+    held = [np.zeros((0, 2, 128)), np.zeros((0, 2, 128))]
+
+    def keep(k, v):
+        for i, x in enumerate((k, v)):
+            x = _np(x)
+            held[i] = np.concatenate([held[i], ref.quantise(x)[0] if kind == "q4" else x])
+
+    def check(slot, n=1):
+        end = c.length(slot)
+        q = _rand(rng, n, 4, 128)
+        out = c.attend(0, _seq_rows(c, [slot], [n], [end]), q)
+        c.check()
+        want, mag = ref.attend(_np(q), held[0][:end], held[1][:end], range(end - n, end))
+        assert (np.abs(_np(out) - want) <= ref.attend_tolerance(want, mag, _eps("bf16"), kind == "q4")).all()
+
+    rows = c.step([0], [60])
+    k, v = _rand(rng, 60, 2, 128), _rand(rng, 60, 2, 128)
+    c.append(0, rows, k, v)
+    keep(k, v)
+    k, v = _rand(rng, 1, 2, 128), _rand(rng, 1, 2, 128)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    moving = c.rows(t([0]), t([60]))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.append(0, moving, k, v)
+        moving.advance()
+    for _ in range(9):  # over the end of the first page
+        k.copy_(_rand(rng, 1, 2, 128))
+        v.copy_(_rand(rng, 1, 2, 128))
+        c.advance([0])
+        g.replay()
+        keep(k, v)
+    assert c.length(0) == 69
+    check(0)
+    check(0, 30)
+    c.fork(0, [1])
+    assert c.length(1) == 69
+    check(1)
+    rows = c.step([0], [2])
+    assert rows.pos0.tolist() == [69]
+    k, v = _rand(rng, 2, 2, 128), _rand(rng, 2, 2, 128)
+    c.append(0, rows, k, v)
+    keep(k, v)
+    check(0)
+    check(1)
