@@ -7,6 +7,7 @@
 #include <new>
 
 #include "fmd_cache.cuh"
+#include "fmd_views.h"
 
 namespace fmd {
 
@@ -672,10 +673,11 @@ int check_rows(const fmd_cache* c, int32_t layer, const fmd_cache_rows* r) {
 }
 
 bool bad_stride(int64_t s) { return s < 0 || (s & 7); }
-// Output rows or heads on top of one another.
-bool overlaps(int64_t row, int64_t head, int n_rows, int n_heads) {
-  return (row == 0 && n_rows > 1) || (head == 0 && n_heads > 1);
+HeadRows rows_at(const void* at, int64_t row, int64_t head, int n_rows, int n_heads, int dim) {
+  return HeadRows{(uint64_t)reinterpret_cast<uintptr_t>(at), n_rows > 1 ? row : 0, n_heads > 1 ? head : 0,
+                  n_rows, n_heads, dim};
 }
+bool same(const HeadRows& a, const HeadRows& b) { return a.at == b.at && a.row == b.row && a.head == b.head; }
 
 CacheView view_of(const fmd_cache* c) {
   return CacheView{(uint8_t*)c->pool, c->page_table, c->format,    c->n_pages,
@@ -738,8 +740,17 @@ int fmd_cache_append(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
   if (a->q)
     for (int64_t s : {a->q_row, a->q_head, a->q_out_row, a->q_out_head})
       if (bad_stride(s)) return FMD_EINVAL;
-  if (a->q && overlaps(a->q_out_row, a->q_out_head, rows->n_rows, a->n_heads)) return FMD_EINVAL;
   if (rows->n_seqs == 0 || rows->n_rows == 0) return FMD_OK;
+  if (a->q) {
+    // queries are written while others, keys and values are still read: in place, or nowhere near
+    const int n = rows->n_rows, d = c->head_dim;
+    const HeadRows out = rows_at(a->q_out, a->q_out_row, a->q_out_head, n, a->n_heads, d);
+    const HeadRows q = rows_at(a->q, a->q_row, a->q_head, n, a->n_heads, d);
+    if (out.overlaps() || (!same(out, q) && meet(out, q)) ||
+        meet(out, rows_at(a->k, a->k_row, a->k_head, n, c->kv_heads, d)) ||
+        meet(out, rows_at(a->v, a->v_row, a->v_head, n, c->kv_heads, d)))
+      return FMD_EINVAL;
+  }
   if (!on_current_device(c->pool) || !on_current_device(a->k)) return FMD_EINVAL;
   CacheAppend p{a->q,      a->k,      a->v,     a->q_out,     a->q_row,     a->q_head, a->k_row,
                 a->k_head, a->v_row,  a->v_head, a->q_out_row, a->q_out_head, a->q_norm, a->k_norm,
@@ -788,8 +799,10 @@ int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
   if (a->window < 0 || a->sinks < 0 || !(a->scale > 0.f) || !(a->scale <= 3.4e38f)) return FMD_EINVAL;
   for (int64_t s : {a->q_row, a->q_head, a->out_row, a->out_head})
     if (bad_stride(s)) return FMD_EINVAL;
-  if (overlaps(a->out_row, a->out_head, rows->n_rows, a->n_heads)) return FMD_EINVAL;
   if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return FMD_OK;
+  const HeadRows out = rows_at(a->out, a->out_row, a->out_head, rows->n_rows, a->n_heads, c->head_dim);
+  if (out.overlaps() || meet(out, rows_at(a->q, a->q_row, a->q_head, rows->n_rows, a->n_heads, c->head_dim)))
+    return FMD_EINVAL;
   const int64_t need = fmd_cache_attend_workspace(c, a->n_heads, rows->n_seqs, rows->max_rows);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return FMD_EINVAL;
   if (!on_current_device(c->pool) || !on_current_device(a->q)) return FMD_EINVAL;

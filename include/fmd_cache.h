@@ -20,7 +20,10 @@
  *    receives FMD_EINVAL (slot or page number) or FMD_EOVERFLOW (position).
  *  - Row pointers are 16-byte aligned and row and head strides are multiples
  *    of 8 elements; the dims of a head are contiguous. Inputs may repeat a row or
- *    a head with a stride of 0, outputs may not.
+ *    a head with a stride of 0, and overlap. No two heads of an output may share an
+ *    element, nor an output and an input but where q_out is q itself, strides
+ *    included (FMD_EINVAL). Outputs whose addresses lie among an input's have the
+ *    input's row stride, as views of one buffer have; with another they are refused.
  */
 #ifndef FMD_CACHE_H
 #define FMD_CACHE_H

@@ -133,3 +133,40 @@ def test_steps_and_forks_after_replayed_steps(kind):
     keep(k, v)
     check(0)
     check(1)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
+@pytest.mark.parametrize("count", [1, 20])
+def test_outputs_that_share_elements_are_refused_and_views_of_one_buffer_are_not(kind, count):
+    lengths = [100, 60]
+    c, held = _filled(kind, "bf16", lengths, kv_heads=2)
+    n, d = 2 * count, 128
+    rows = _seq_rows(c, [0, 1], [count] * 2, lengths)
+    x = _rand(np.random.default_rng(0), n + 1, 16, d)
+    q, k, v, out = x[:n, :4], x[:n, 4:6], x[:n, 6:8], x[:n, 8:12]
+    big = torch.zeros(64 * n * d, dtype=torch.bfloat16, device="cuda")
+    before, pool = x.clone(), c.pool.clone()
+    bad = [x[:n, 2:6], x[:n, 3:7], big.as_strided((n, 4, d), (8 * d, d // 2, 1)), big.as_strided((n, 4, d), (8 * d, 8, 1)),
+           x.flatten()[8:8 + n * 16 * d].view(n, 16, d)[:, :4]]
+    if n > 2:
+        bad += [big.as_strided((n, 4, d), (2 * d, d, 1)), big.as_strided((n, 4, d), (8, n * d, 1)), x[1:, :4]]
+    for o in bad:
+        with pytest.raises(PKG.FmdError) as e:
+            c.append(0, rows, k, v, q=q, q_out=o)
+        assert e.value.status == PKG._lib.FMD_EINVAL
+    for o in bad + [q]:
+        with pytest.raises(PKG.FmdError) as e:
+            c.attend(0, rows, q, out=o)
+        assert e.value.status == PKG._lib.FMD_EINVAL
+    torch.cuda.synchronize()
+    assert torch.equal(x, before) and torch.equal(c.pool, pool) and not bool(big.any())
+    # views of one buffer beside one another, and heads outermost
+    want = c.attend(0, rows, q.clone())
+    c.attend(0, rows, q, out=out)
+    turned = torch.zeros(4, n, d, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    c.attend(0, rows, q, out=turned)
+    assert torch.equal(out, want) and torch.equal(turned, want)
+    c.append(0, rows, k, v, q=q, q_out=out)
+    c.append(0, rows, k, v, q=q, q_out=q)
+    c.check()
+    assert torch.equal(out, before[:n, :4]) and torch.equal(q, before[:n, :4])
