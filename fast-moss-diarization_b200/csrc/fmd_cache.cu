@@ -672,6 +672,8 @@ int check_rows(const fmd_cache* c, int32_t layer, const fmd_cache_rows* r) {
   return FMD_OK;
 }
 
+// No rows at all: the row buffers are not looked at (an empty one has no address).
+bool empty(const fmd_cache_rows* r) { return r->n_seqs == 0 || r->n_rows == 0; }
 bool bad_stride(int64_t s) { return s < 0 || (s & 7); }
 HeadRows rows_at(const void* at, int64_t row, int64_t head, int n_rows, int n_heads, int dim) {
   return HeadRows{(uint64_t)reinterpret_cast<uintptr_t>(at), n_rows > 1 ? row : 0, n_heads > 1 ? head : 0,
@@ -723,12 +725,14 @@ int fmd_cache_append(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
                      int32_t* status, void* stream) {
   int rc = check_cache(c);
   if (rc || (rc = check_rows(c, layer, rows))) return rc;
-  if (!a || !a->k || !a->v || !aligned16(a->k) || !aligned16(a->v)) return FMD_EINVAL;
-  if (a->dtype != FMD_DT_F16 && a->dtype != FMD_DT_BF16) return FMD_EINVAL;
+  if (!a || (a->dtype != FMD_DT_F16 && a->dtype != FMD_DT_BF16)) return FMD_EINVAL;
   if (c->format != FMD_CACHE_Q4 && c->format != a->dtype) return FMD_EINVAL;
-  if (a->n_heads < 0 || a->n_heads > 16384 || (a->n_heads > 0) != (a->q != nullptr) || (a->q && !a->q_out))
-    return FMD_EINVAL;
-  if (a->q && (!aligned16(a->q) || !aligned16(a->q_out))) return FMD_EINVAL;
+  if (a->n_heads < 0 || a->n_heads > 16384) return FMD_EINVAL;
+  if (!empty(rows)) {
+    if (!a->k || !a->v || !aligned16(a->k) || !aligned16(a->v)) return FMD_EINVAL;
+    if ((a->n_heads > 0) != (a->q != nullptr) || (a->q && !a->q_out)) return FMD_EINVAL;
+    if (a->q && (!aligned16(a->q) || !aligned16(a->q_out))) return FMD_EINVAL;
+  }
   if (a->rot_dim < 0 || a->rot_dim > c->head_dim || a->rot_dim % 8) return FMD_EINVAL;
   if (a->rot_dim > 0 && (!a->cos_table || !a->sin_table || a->table_rows < 1 || !aligned16(a->cos_table) ||
                          !aligned16(a->sin_table)))
@@ -740,7 +744,7 @@ int fmd_cache_append(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
   if (a->q)
     for (int64_t s : {a->q_row, a->q_head, a->q_out_row, a->q_out_head})
       if (bad_stride(s)) return FMD_EINVAL;
-  if (rows->n_seqs == 0 || rows->n_rows == 0) return FMD_OK;
+  if (empty(rows)) return FMD_OK;
   if (a->q) {
     // queries are written while others, keys and values are still read: in place, or nowhere near
     const int n = rows->n_rows, d = c->head_dim;
@@ -763,8 +767,8 @@ int fmd_cache_read(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows
                    void* stream) {
   int rc = check_cache(c);
   if (rc || (rc = check_rows(c, layer, rows))) return rc;
+  if (empty(rows)) return FMD_OK;
   if (!k || !v || !aligned16(k) || !aligned16(v)) return FMD_EINVAL;
-  if (rows->n_seqs == 0 || rows->n_rows == 0) return FMD_OK;
   if (!on_current_device(c->pool) || !on_current_device(k)) return FMD_EINVAL;
   // blocks of a row: as in append
   const int per_block = kReadThreads / (c->head_dim / 8) * 4, most = (2 * c->kv_heads + per_block - 1) / per_block;
@@ -790,7 +794,8 @@ int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
                      void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
   int rc = check_cache(c);
   if (rc || (rc = check_rows(c, layer, rows))) return rc;
-  if (!a || !a->q || !a->out || a->out == a->q || !aligned16(a->q) || !aligned16(a->out)) return FMD_EINVAL;
+  if (!a || (!empty(rows) && (!a->q || !a->out || a->out == a->q || !aligned16(a->q) || !aligned16(a->out))))
+    return FMD_EINVAL;
   if (a->dtype != FMD_DT_F16 && a->dtype != FMD_DT_BF16) return FMD_EINVAL;
   if (c->format != FMD_CACHE_Q4 && c->format != a->dtype) return FMD_EINVAL;
   if (a->n_heads < 1 || a->n_heads % c->kv_heads) return FMD_EINVAL;
@@ -799,7 +804,7 @@ int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
   if (a->window < 0 || a->sinks < 0 || !(a->scale > 0.f) || !(a->scale <= 3.4e38f)) return FMD_EINVAL;
   for (int64_t s : {a->q_row, a->q_head, a->out_row, a->out_head})
     if (bad_stride(s)) return FMD_EINVAL;
-  if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return FMD_OK;
+  if (empty(rows) || rows->max_rows == 0) return FMD_OK;
   const HeadRows out = rows_at(a->out, a->out_row, a->out_head, rows->n_rows, a->n_heads, c->head_dim);
   if (out.overlaps() || meet(out, rows_at(a->q, a->q_row, a->q_head, rows->n_rows, a->n_heads, c->head_dim)))
     return FMD_EINVAL;

@@ -40,3 +40,31 @@ def test_books_follow_rows_that_move_on_by_themselves():
         assert e.value.status == status
     assert c.length(0) == 131
     _consistent(c)
+
+
+def test_calls_without_rows_do_nothing():
+    """An empty tensor's address is 0: calls that have no rows do not look at it."""
+    import ctypes as C
+
+    lib = PKG.load_library()
+    cache = C.byref(L.Cache(4096, 4096, L.CACHE_BF16, 1, 4, 2, 128, 2, 4, 0))
+    app = C.byref(L.CacheAppendArgs(k_row=256, k_head=128, v_row=256, v_head=128, dtype=L.DT_BF16))
+    both = C.byref(L.CacheAppendArgs(k_row=256, k_head=128, v_row=256, v_head=128, q_row=512, q_head=128, q_out_row=512,
+                                     q_out_head=128, dtype=L.DT_BF16, n_heads=4))
+    att = C.byref(L.CacheAttendArgs(q_row=512, q_head=128, out_row=512, out_head=128, scale=0.1, dtype=L.DT_BF16,
+                                    n_heads=4))
+    for rows in (L.CacheRows(None, None, None, 0, 0, 0), L.CacheRows(4096, 4096, 4096, 3, 0, 0),
+                 L.CacheRows(4096, 4096, 4096, 3, 0, 5)):
+        r = C.byref(rows)
+        assert lib.fmd_cache_append(cache, 0, r, app, None, None) == L.FMD_OK
+        assert lib.fmd_cache_append(cache, 0, r, both, None, None) == L.FMD_OK
+        assert lib.fmd_cache_read(cache, 0, r, None, None, None, None) == L.FMD_OK
+        assert lib.fmd_cache_attend(cache, 0, r, att, None, 0, None, None) == L.FMD_OK
+    # with rows they are looked at, and what does not depend on them is checked either way
+    r, none = C.byref(L.CacheRows(4096, 4096, None, 1, 1, 1)), C.byref(L.CacheRows(4096, 4096, 4096, 3, 0, 0))
+    assert lib.fmd_cache_append(cache, 0, r, app, None, None) == L.FMD_EINVAL
+    assert lib.fmd_cache_read(cache, 0, r, None, None, None, None) == L.FMD_EINVAL
+    assert lib.fmd_cache_attend(cache, 0, r, att, 4096, 1 << 40, None, None) == L.FMD_EINVAL
+    assert lib.fmd_cache_append(cache, 1, none, app, None, None) == L.FMD_EINVAL
+    assert lib.fmd_cache_attend(cache, 0, none, C.byref(L.CacheAttendArgs(dtype=9, n_heads=4, scale=0.1)), None, 0, None,
+                                None) == L.FMD_EINVAL

@@ -170,3 +170,17 @@ def test_outputs_that_share_elements_are_refused_and_views_of_one_buffer_are_not
     c.append(0, rows, k, v, q=q, q_out=q)
     c.check()
     assert torch.equal(out, before[:n, :4]) and torch.equal(q, before[:n, :4])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
+def test_calls_without_rows_do_nothing(kind):
+    c, _ = _filled(kind, "bf16", [70, 5])
+    pool = c.pool.clone()
+    for rows in (c.step([0, 1], [0, 0]), c.step([], [])):
+        k, q = _rand(np.random.default_rng(0), 0, 2, 128), _rand(np.random.default_rng(0), 0, 4, 128)
+        assert c.append(0, rows, k, k) is None
+        assert c.append(0, rows, k, k, q=q).shape == q.shape
+        assert c.attend(0, rows, q).shape == q.shape and c.attend(0, rows, q, window=3, out=q).shape == q.shape
+        assert [t.shape for t in c.read(0, rows)] == [k.shape, k.shape]
+    c.check()
+    assert torch.equal(c.pool, pool) and c.length(0) == 70
