@@ -251,29 +251,34 @@ class PagedCache:
             _fail("one count >= 0 per slot")
         if len(set(slots)) != len(slots):
             _fail("a slot is listed twice")
-        fresh = 0
-        for s, n in zip(slots, counts):
+        # entries that need a page of their own (shared with a slot that keeps it, or evicted)
+        fresh, given, own = 0, {}, [[] for _ in slots]
+        for s, n, mine in zip(slots, counts, own):
             pages, at = self._open(s), self._length[s]
             need = -(-(at + n) // PAGE)
             if need > self.max_pages_per_slot:
                 _fail(f"slot {s}: {at + n} positions exceed {self.max_pages_per_slot} pages", _lib.FMD_EOVERFLOW)
             fresh += max(0, need - len(pages))
-            fresh += sum(p < 0 or self._names[p] > 1 for p in pages[at // PAGE:need])
+            for k in range(at // PAGE, min(need, len(pages))):
+                p = pages[k]
+                if p < 0:
+                    mine.append(k)
+                elif self._names[p] - given.get(p, 0) > 1:  # the last to write a page keeps it
+                    given[p] = given.get(p, 0) + 1
+                    mine.append(k)
+            fresh += len(mine)
         if fresh > len(self._free):
             _fail("the cache has too few free pages", _lib.FMD_ENOMEM)
         moves = []
-        for s, n in zip(slots, counts):
-            at = self._length[s]
-            need = -(-(at + n) // PAGE)
-            for k in range(at // PAGE, min(need, len(self._pages[s]))):
+        for s, n, mine in zip(slots, counts, own):
+            for k in mine:
                 p = self._pages[s][k]
-                if p < 0 or self._names[p] > 1:
-                    self._pages[s][k] = self._take()
-                    if p >= 0:
-                        moves.append((p, self._pages[s][k]))
-                        self._drop(p)
-                    self._upload(s, k)
-            self.reserve(s, at + n)
+                self._pages[s][k] = self._take()
+                if p >= 0:
+                    moves.append((p, self._pages[s][k]))
+                    self._drop(p)
+                self._upload(s, k)
+            self.reserve(s, self._length[s] + n)
         if moves:
             self.copy_pages([a for a, _ in moves], [b for _, b in moves])
         pos0 = [self._length[s] for s in slots]

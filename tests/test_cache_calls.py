@@ -68,3 +68,31 @@ def test_calls_without_rows_do_nothing():
     assert lib.fmd_cache_append(cache, 1, none, app, None, None) == L.FMD_EINVAL
     assert lib.fmd_cache_attend(cache, 0, none, C.byref(L.CacheAttendArgs(dtype=9, n_heads=4, scale=0.1)), None, 0, None,
                                 None) == L.FMD_EINVAL
+
+
+def _sharing(n_pages=4, names=2, **kw):
+    """Slots 0 .. names - 1 name one partial page."""
+    c = HostCache(n_pages=n_pages, slots=[(i, [0], 10) for i in range(names)], **kw)
+    for i in range(names):
+        c._upload(i, 0)
+    return c
+
+
+def test_sharers_of_a_page_need_one_page_less_than_they_are():
+    """The last of them keeps the page itself."""
+    c = _sharing(n_pages=2)
+    c.step([0, 1], [1, 1])
+    assert c.pages(0) == [1] and c.pages(1) == [0] and c.free_pages == 0 and c.calls == ["fmd_cache_copy_pages"]
+    _consistent(c)
+    c = _sharing(n_pages=3, names=3)
+    c.step([2, 0, 1], [3, 2, 1])
+    assert sorted(c.pages(i)[0] for i in range(3)) == [0, 1, 2] and c._names == [1, 1, 1]
+    _consistent(c)
+    c = _sharing(n_pages=3, names=3)  # not all of them: each needs its copy
+    c.step([0, 1], [1, 1])
+    assert c.pages(2) == [0] and c.free_pages == 0
+    c = _sharing(n_pages=2, names=3)
+    with pytest.raises(PKG.FmdError) as e:
+        c.step([0, 1], [1, 1])
+    assert e.value.status == L.FMD_ENOMEM and c._names == [3, 0]
+    _consistent(c)
