@@ -259,7 +259,7 @@ class PagedCache:
             if need > self.max_pages_per_slot:
                 _fail(f"slot {s}: {at + n} positions exceed {self.max_pages_per_slot} pages", _lib.FMD_EOVERFLOW)
             fresh += max(0, need - len(pages))
-            for k in range(at // PAGE, min(need, len(pages))):
+            for k in range(at // PAGE, min(need, len(pages)) if n else 0):  # the pages that are written
                 p = pages[k]
                 if p < 0:
                     mine.append(k)

@@ -96,3 +96,15 @@ def test_sharers_of_a_page_need_one_page_less_than_they_are():
         c.step([0, 1], [1, 1])
     assert e.value.status == L.FMD_ENOMEM and c._names == [3, 0]
     _consistent(c)
+
+
+def test_a_slot_without_new_positions_is_left_alone():
+    c = _sharing(n_pages=1)  # no page for a copy
+    r = c.step([0, 1], [0, 0])
+    assert r.n_rows == 0 and c.pages(0) == c.pages(1) == [0] and c.calls == []
+    c.advance([1], 0)
+    _consistent(c)
+    c = _sharing(n_pages=2)
+    c.step([0, 1], [0, 1])
+    assert c.pages(0) == [0] and c.pages(1) == [1] and (c.length(0), c.length(1)) == (10, 11)
+    _consistent(c)
