@@ -60,7 +60,8 @@ class PagedCache:
     `64 * max_pages_per_slot` positions. `kind`: "f16" or "bf16" (rows of that
     dtype) or "q4" (rows of either). `pool` and `page_table` may be the caller's
     (uint8 of `pool_bytes`, int32 `[max_slots, max_pages_per_slot]`), with
-    `slots` as `(slot, its pages, its length)` for what they hold already. One host
+    `slots` as `(slot, its pages, its length)` for what they hold already (a table
+    that the cache makes gets their pages). One host
     thread at a time may change the bookkeeping (open, step, fork, evict, release,
     compact); the operators may run on several streams, as long as no call writes
     what another reads."""
@@ -88,7 +89,8 @@ class PagedCache:
             self.device = torch.device("cuda", torch.cuda.current_device())
         if pool is None:
             pool = torch.zeros(self.pool_bytes, dtype=torch.uint8, device=self.device)
-        if page_table is None:
+        own_table = page_table is None
+        if own_table:
             page_table = torch.full((max_slots, max_pages_per_slot), -1, dtype=torch.int32, device=self.device)
         if pool.dtype != torch.uint8 or pool.numel() != self.pool_bytes or not pool.is_contiguous():
             _fail(f"pool must be a contiguous uint8 tensor of {self.pool_bytes} bytes")
@@ -123,6 +125,8 @@ class PagedCache:
             for p in pages:
                 if p >= 0:
                     self._names[p] += 1
+            if own_table:
+                self._upload(slot, 0)
         self._free = [p for p in range(n_pages) if self._names[p] == 0]  # a heap: the lowest page goes first
 
     # -- bookkeeping ---------------------------------------------------------------------

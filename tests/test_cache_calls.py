@@ -108,3 +108,13 @@ def test_a_slot_without_new_positions_is_left_alone():
     c.step([0, 1], [0, 1])
     assert c.pages(0) == [0] and c.pages(1) == [1] and (c.length(0), c.length(1)) == (10, 11)
     _consistent(c)
+
+
+def test_slots_given_to_the_constructor_are_in_its_own_table():
+    """Without the caller's page table the cache's own holds what `slots` names."""
+    c = HostCache(slots=[(2, [3, 1], 100), (0, [5, -1, 3], 150)])
+    assert c.page_table.tolist() == [[5, -1, 3, -1], [-1] * 4, [3, 1, -1, -1], [-1] * 4]
+    _consistent(c)
+    table = torch.tensor([[5, 6, 7, 0]] * 4, dtype=torch.int32)
+    HostCache(page_table=table, slots=[(2, [5, 6], 100)])  # the caller's holds it already
+    assert table.tolist() == [[5, 6, 7, 0]] * 4
