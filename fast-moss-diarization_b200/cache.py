@@ -200,10 +200,10 @@ class PagedCache:
         self._names[p] = 1
         return p
 
-    def _upload(self, slot: int, first: int) -> None:
+    def _upload(self, slot: int, first: int, pages=None) -> None:
         import torch
 
-        row = self._pages[slot][first:]
+        row = (self._pages[slot] if pages is None else pages)[first:]
         if row:
             self.page_table[slot, first:first + len(row)].copy_(torch.tensor(row, dtype=torch.int32))
 
@@ -273,18 +273,34 @@ class PagedCache:
             fresh += len(mine)
         if fresh > len(self._free):
             _fail("the cache has too few free pages", _lib.FMD_ENOMEM)
-        moves = []
+        taken = [heapq.heappop(self._free) for _ in range(fresh)]
+        moves, changed, new = [], [], iter(taken)
         for s, n, mine in zip(slots, counts, own):
-            for k in mine:
-                p = self._pages[s][k]
-                self._pages[s][k] = self._take()
-                if p >= 0:
-                    moves.append((p, self._pages[s][k]))
-                    self._drop(p)
-                self._upload(s, k)
-            self.reserve(s, self._length[s] + n)
-        if moves:
-            self.copy_pages([a for a, _ in moves], [b for _, b in moves])
+            more = -(-(self._length[s] + n) // PAGE) - len(self._pages[s])
+            if mine or more > 0:
+                pages = list(self._pages[s])
+                for k in mine:
+                    p, pages[k] = pages[k], next(new)
+                    if p >= 0:
+                        moves.append((p, pages[k]))
+                first = mine[0] if mine else len(pages)
+                pages += [next(new) for _ in range(more)]
+                changed.append((s, pages, first))
+        try:
+            if moves:
+                self.copy_pages([a for a, _ in moves], [b for _, b in moves])
+            for s, pages, first in changed:
+                self._upload(s, first, pages)
+        except BaseException:
+            self._free += taken  # nothing else has changed
+            heapq.heapify(self._free)
+            raise
+        for p in taken:
+            self._names[p] = 1
+        for p, _ in moves:
+            self._drop(p)
+        for s, pages, _ in changed:
+            self._pages[s] = pages
         pos0 = [self._length[s] for s in slots]
         for s, n in zip(slots, counts):
             self._length[s] += n
@@ -532,6 +548,15 @@ class PagedCache:
             _fail("the cache has too few free pages", _lib.FMD_ENOMEM)
         m, shared, names = len(dsts), pages[:full], self._names
         fresh = [heapq.heappop(self._free) for _ in dsts] if part else [-1] * m
+        ia = C.c_int32 * m
+        try:
+            self._call(self.lib.fmd_cache_fork, m, ia(*[src] * m), ia(*dsts), ia(*[n] * m), ia(*fresh),
+                       self._status_at)
+        except BaseException:
+            if part:
+                self._free += fresh  # nothing else has changed
+                heapq.heapify(self._free)
+            raise
         for p in fresh if part else ():
             names[p] = 1
         for d, p in zip(dsts, fresh):
@@ -540,9 +565,6 @@ class PagedCache:
         for p in shared:
             if p >= 0:
                 names[p] += m
-        ia = C.c_int32 * m
-        self._call(self.lib.fmd_cache_fork, m, ia(*[src] * m), ia(*dsts), ia(*[n] * m), ia(*fresh),
-                   self._status_at)
 
     def evict(self, slot: int, window: int, sinks: int = 0) -> int:
         """Free the slot's pages that no later row sees with this window and

@@ -118,3 +118,24 @@ def test_slots_given_to_the_constructor_are_in_its_own_table():
     table = torch.tensor([[5, 6, 7, 0]] * 4, dtype=torch.int32)
     HostCache(page_table=table, slots=[(2, [5, 6], 100)])  # the caller's holds it already
     assert table.tolist() == [[5, 6, 7, 0]] * 4
+
+
+def test_a_launch_that_fails_leaves_the_books_alone(monkeypatch):
+    def refuse(fn, *args):
+        raise PKG.FmdError(L.FMD_EIO, fn.__name__)
+
+    def books(c):
+        return [list(p) if p is not None else None for p in c._pages], list(c._length), list(c._names), sorted(c._free)
+
+    c = _sharing(n_pages=6)
+    c.open(2, 0)
+    table, before, call = c.page_table.clone(), books(c), c._call
+    monkeypatch.setattr(c, "_call", refuse)
+    for f in (lambda: c.step([0, 2], [60, 5]), lambda: c.advance([1], 1), lambda: c.fork(0, [3])):
+        with pytest.raises(PKG.FmdError):
+            f()
+        assert books(c) == before and torch.equal(c.page_table, table)
+    monkeypatch.setattr(c, "_call", call)
+    c.fork(0, [3])
+    c.step([0, 2], [60, 5])
+    assert c.length(0) == 70 and c.length(3) == 10 and c.pages(0) == [2, 3] and c.pages(2) == [4]
