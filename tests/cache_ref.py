@@ -72,3 +72,15 @@ def attend_tolerance(want, mag, eps, q4):
     hardware exponential by less: 2^-14 of the magnitude in all."""
     terms = 2 * 2.0 ** -11 if q4 else eps / 2
     return eps / 2 * np.abs(want) + (terms + 2.0 ** -14) * mag + 2.0 ** -25
+
+
+def finite(check):
+    """`check` (a comparison that returns the tensor it looked at), which a NaN or
+    an infinity does not pass: |NaN - x| > tol is false."""
+    def strict(*args, **kw):
+        out = check(*args, **kw)
+        values = out.detach().double().cpu().numpy()
+        assert np.isfinite(values).all(), np.argwhere(~np.isfinite(values))[:4].tolist()
+        return out
+
+    return strict

@@ -3,8 +3,10 @@ of test_cache_host."""
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 
+import cache_ref as ref
 from conftest import PKG
 from test_cache_host import HostCache, _consistent
 
@@ -139,3 +141,29 @@ def test_a_launch_that_fails_leaves_the_books_alone(monkeypatch):
     c.fork(0, [3])
     c.step([0, 2], [60, 5])
     assert c.length(0) == 70 and c.length(3) == 10 and c.pages(0) == [2, 3] and c.pages(2) == [4]
+
+
+def test_the_strict_comparison_refuses_a_nan(monkeypatch):
+    import test_gpu_cache as base
+
+    held = [(np.ones((5, 1, 64)), np.ones((5, 1, 64)))]
+
+    class Fake:
+        head_dim = 64
+
+        def attend(self, layer, rows, q, **kw):
+            return self.out
+
+        def check(self):
+            pass
+
+    monkeypatch.setattr(base, "_seq_rows", lambda *a: None)
+    c, q = Fake(), torch.ones(2, 1, 64)
+    call = lambda f: f(c, held, "bf16", "bf16", [2], [5], 1, q=q)
+    c.out = torch.ones(2, 1, 64)
+    call(base._check_attend), call(ref.finite(base._check_attend))
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        c.out = torch.ones(2, 1, 64)
+        c.out[1, 0, 3] = bad
+        with pytest.raises(AssertionError):
+            call(ref.finite(base._check_attend))
