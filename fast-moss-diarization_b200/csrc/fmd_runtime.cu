@@ -20,6 +20,7 @@
 #include "fmd_cache.cuh"
 #include "fmd_kernels.cuh"
 #include "fmd_scheduler.cuh"
+#include "fmd_status.h"
 #include "fmd_watch.h"
 
 namespace fmd {
@@ -157,7 +158,8 @@ struct fmd_handle {
   int chain_clusters = 0;
   int* chain_sync = nullptr;        // [layers][kChainSyncInts], cleared by each decode step's first kernel
   int* d_status = nullptr;          // device-side error status (bounded waits)
-  bool launch_refused = false;      // a decode projection could not be launched
+  bool launch_refused = false;      // a decode projection or cache operator could not be launched
+  std::string cache_refused;        // what CUDA said to the cache operator's launch
   int* d_page_table = nullptr;
   std::vector<int> h_page_table;
   std::vector<int> free_pages;           // host allocator (operator mode)
@@ -604,7 +606,11 @@ void cache_layer(fmd_handle* h, int l, int max_rows, const int* n_rows_ptr, bool
     if (e == cudaSuccess) e = launch_cache_chunk(bf, h->cache, l, blocks, a, h->cache_ws, h->d_status, s);
     trace(h, "cache_chunk", l);
   }
-  if (e != cudaSuccess) h->launch_refused = true;
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // reported as this refusal, not by a later call
+    h->launch_refused = true;
+    h->cache_refused = cudaGetErrorString(e);
+  }
 }
 
 // The layer loop of a decode-only pass over the rows of `v` on stream `s`.
@@ -914,7 +920,9 @@ int check_ready(fmd_handle* h) {
 int sync_check(fmd_handle* h) {
   if (h->launch_refused) {
     h->launch_refused = false;
-    return fail(h, FMD_EIO, "a decode projection was not launched (no packed weight tiles or no valid K split)");
+    const std::string why = refusal_text(h->cache_refused);
+    h->cache_refused.clear();
+    return fail(h, FMD_EIO, why);
   }
   cudaError_t e = cudaStreamSynchronize(h->stream);
   if (e != cudaSuccess) return fail(h, FMD_EIO, std::string("device error: ") + cudaGetErrorString(e));
@@ -927,13 +935,7 @@ int sync_check(fmd_handle* h) {
     if (st[0] != 0) {
       cudaMemset(h->d_status, 0, 2 * sizeof(int));
       if (h->cache_ws) cudaMemset(h->cache_ws, 0, FMD_CACHE_WORKSPACE_ZERO);
-      static const char* const kSites[] = {"?", "k_gemv", "k_lm_head", "k_attn_decode_tma", "k_attn_prefill_tc",
-                                           "k_gemm_tc", "k_layer_tail", "k_wait_probe", "k_proj_tc", "k_cache_decode", "k_cache_chunk"};
-      constexpr int kNumSites = (int)(sizeof(kSites) / sizeof(kSites[0]));
-      const char* site = st[1] >= 1 && st[1] < kNumSites ? kSites[st[1]] : "?";
-      return fail(h, st[0], st[0] == FMD_EIO ? std::string("a greedy pick found no finite logit (non-finite activations)")
-                                             : "a bounded device-side wait gave up in " + std::string(site) +
-                                                   " (status " + std::to_string(st[0]) + ")");
+      return fail(h, st[0], device_status_text(st[0], st[1]));
     }
   }
   return FMD_OK;
