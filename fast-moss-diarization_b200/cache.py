@@ -336,7 +336,10 @@ class PagedCache:
             raise _lib.FmdError(st, f"{fn.__name__}: {self.lib.fmd_status_string(st).decode()}")
 
     def check(self) -> None:
-        """Wait for the operators and raise if a row or page was out of range."""
+        """Wait for the operators, on every stream of the device, and raise if a row
+        or page was out of range."""
+        if self.device.type == "cuda":
+            self._cuda.synchronize(self.device)
         st = int(self._status[0].item())
         if st != 0:
             self._status.zero_()

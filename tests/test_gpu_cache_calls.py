@@ -184,3 +184,26 @@ def test_calls_without_rows_do_nothing(kind):
         assert [t.shape for t in c.read(0, rows)] == [k.shape, k.shape]
     c.check()
     assert torch.equal(c.pool, pool) and c.length(0) == 70
+
+
+def test_check_waits_for_every_stream():
+    c, _ = _filled("bf16", "bf16", [100])
+    q = _rand(np.random.default_rng(0), 1, 4, 128)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    bad = c.rows(t([17]), t([99]))
+    out = torch.zeros_like(q)
+    busy = torch.ones(8192, 8192, device="cuda")
+    side, then = torch.cuda.Stream(), torch.zeros_like(busy)
+    with torch.cuda.stream(side):  # what these allocate is there before the stream is busy
+        torch.mm(busy, busy, out=then)
+        c.attend(0, _seq_rows(c, [0], [1], [100]), q, out=out)
+    c.check()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            torch.mm(busy, busy, out=then)
+        c.attend(0, bad, q, out=out)
+    with pytest.raises(PKG.FmdError) as e:
+        c.check()
+    assert e.value.status == PKG._lib.FMD_EINVAL
+    c.check()
