@@ -480,7 +480,12 @@ class PagedCache:
         n = self.lib.fmd_cache_attend_workspace(self._ref, n_heads, rows.slot.shape[0], rows.max_rows)
         if n == 0:
             return None
-        if cuda.is_current_stream_capturing():
+        if cuda.current_device() == self._index:
+            capturing = cuda.is_current_stream_capturing()
+        else:
+            with cuda.device(self._index):
+                capturing = cuda.is_current_stream_capturing()
+        if capturing:
             # a graph's own: graphs replayed at the same time must not share one
             return self._fresh_workspace(n)
         key = cuda.current_stream(self._index).cuda_stream

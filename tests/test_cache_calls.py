@@ -167,3 +167,43 @@ def test_the_strict_comparison_refuses_a_nan(monkeypatch):
         c.out[1, 0, 3] = bad
         with pytest.raises(AssertionError):
             call(ref.finite(base._check_attend))
+
+
+def test_a_capture_on_the_caches_device_is_seen_from_another(monkeypatch):
+    """Whether a stream is capturing is asked of the current device, which need not be
+    the cache's: a graph's workspace is its own either way."""
+    class Cuda:
+        at, capturing = 1, {0}
+
+        def current_device(self):
+            return self.at
+
+        def device(self, index):
+            cuda = self
+
+            class Within:
+                def __enter__(self):
+                    self.was, cuda.at = cuda.at, index
+
+                def __exit__(self, *a):
+                    cuda.at = self.was
+
+            return Within()
+
+        def is_current_stream_capturing(self):
+            return self.at in self.capturing
+
+        def current_stream(self, index):
+            return type("Stream", (), {"cuda_stream": 7 + index})
+
+    c = HostCache(kv_heads=2)
+    c.open(0)
+    rows = c.step([0], [1])
+    c._cuda, c._index = Cuda(), 0
+    a, b = c._workspace(4, rows), c._workspace(4, rows)
+    assert a is not b and not c._workspaces and c._cuda.at == 1
+    c._cuda.capturing = {1}  # the other device's capture is none of the cache's
+    a, b = c._workspace(4, rows), c._workspace(4, rows)
+    assert a is b and list(c._workspaces) == [7]
+    c._cuda.at = 0
+    assert c._workspace(4, rows) is a
