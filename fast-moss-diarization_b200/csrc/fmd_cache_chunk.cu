@@ -688,8 +688,8 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
               amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
             }
           }
-          // 2^e brings the largest magnitude to [1, 2)
-          const int e2 = min(126, amax > 0.f && amax <= FLT_MAX ? 127 - (int)(__float_as_uint(amax) >> 23) : 0);
+          // 2^e brings the largest magnitude to [1, 2), or to [2, 4) where 2^e would not be normal
+          const int e2 = max(-126, min(126, amax > 0.f && amax <= FLT_MAX ? 127 - (int)(__float_as_uint(amax) >> 23) : 0));
           const float up = __uint_as_float((uint32_t)(127 + e2) << 23);
           scale *= __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll

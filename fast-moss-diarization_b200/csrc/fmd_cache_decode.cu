@@ -814,10 +814,13 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? 4 : 3)
         pick[k] = t < 2 ? hi : v - hi;
       }
       qb[n] = Act<__half>::pack2(pick[0], pick[1]);
-      // accumulators hold columns 2 t, 2 t + 1: their scales
+      // accumulators hold columns 2 t, 2 t + 1: their scales. Queries from 2^120 on can take
+      // one past f32, where a score of 0 would become a NaN; the largest f32 in its place keeps
+      // the order of the others
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        sl[n][k] = p.a.scale * (16777216.f * 1.4426950408889634f) * __shfl_sync(0xffffffffu, down, (2 * t + k) * 4);
+        sl[n][k] = fminf(p.a.scale * (16777216.f * 1.4426950408889634f) *
+                             __shfl_sync(0xffffffffu, down, (2 * t + k) * 4), FLT_MAX);
     }
     for (; mine < x + len; mine += 4) {
       if (aborted || !mbar_wait_warp(&full[warp][s], phase, kDcWait)) {

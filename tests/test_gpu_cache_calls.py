@@ -207,3 +207,24 @@ def test_check_waits_for_every_stream():
         c.check()
     assert e.value.status == PKG._lib.FMD_EINVAL
     c.check()
+
+
+@pytest.mark.parametrize("e", [-133, -126, 110, 121, 125, 126, 127])
+@pytest.mark.parametrize("count", [1, 40])
+def test_queries_at_the_ends_of_bf16_over_4_bits(e, count):
+    """Queries of up to 1.5 x 2^127 whose scores are finite: their scaling to f16 stays
+    within f32 as well. One key meets them; the rest scores 0."""
+    dim, n = 128, 100
+    c = PKG.PagedCache(1, 1, dim, 3, 1, 2, kind="q4")
+    c.open(0)
+    rng = np.random.default_rng(4)
+    k, v = torch.zeros(n, 1, dim, dtype=torch.bfloat16, device="cuda"), _rand(rng, n, 1, dim)
+    k[20, 0, 0] = 2.0 ** -10
+    c.append(0, c.step([0], [n]), k, v)
+    q = torch.zeros(count, 2, dim, dtype=torch.bfloat16, device="cuda")
+    q[:, :, 0] = 1.5 * 2.0 ** e
+    out = c.attend(0, _seq_rows(c, [0], [count], [n]), q)
+    c.check()
+    kk, vv = ref.quantise(_np(k))[0], ref.quantise(_np(v))[0]
+    want, mag = ref.attend(_np(q), kk, vv, range(n - count, n))
+    assert (np.abs(_np(out) - want) <= ref.attend_tolerance(want, mag, _eps("bf16"), True)).all()
