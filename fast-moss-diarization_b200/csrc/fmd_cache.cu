@@ -804,7 +804,8 @@ int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
   if (a->window < 0 || a->sinks < 0 || !(a->scale > 0.f) || !(a->scale <= 3.4e38f)) return FMD_EINVAL;
   for (int64_t s : {a->q_row, a->q_head, a->out_row, a->out_head})
     if (bad_stride(s)) return FMD_EINVAL;
-  if (empty(rows) || rows->max_rows == 0) return FMD_OK;
+  if (empty(rows)) return FMD_OK;
+  if (rows->max_rows == 0) return rows->row0 ? FMD_OK : FMD_EINVAL;  // without row0 each sequence has a row
   const HeadRows out = rows_at(a->out, a->out_row, a->out_head, rows->n_rows, a->n_heads, c->head_dim);
   if (out.overlaps() || meet(out, rows_at(a->q, a->q_row, a->q_head, rows->n_rows, a->n_heads, c->head_dim)))
     return FMD_EINVAL;

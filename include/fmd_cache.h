@@ -80,7 +80,8 @@ typedef struct fmd_cache_rows {
   const int32_t* row0;  /* [n_seqs + 1], ascending, or NULL                        */
   int32_t n_seqs;
   int32_t n_rows;       /* rows of the row buffers (>= row0[n_seqs])               */
-  int32_t max_rows;     /* rows of the longest sequence at most                    */
+  int32_t max_rows;     /* attention: rows of the longest sequence at most; >= 1
+                         * without row0                                            */
   int32_t reserved;
 } fmd_cache_rows;
 

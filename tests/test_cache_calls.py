@@ -207,3 +207,19 @@ def test_a_capture_on_the_caches_device_is_seen_from_another(monkeypatch):
     assert a is b and list(c._workspaces) == [7]
     c._cuda.at = 0
     assert c._workspace(4, rows) is a
+
+
+def test_sequences_of_one_row_need_max_rows_of_one():
+    """Without row offsets every sequence has a row, so a `max_rows` of 0 cannot be
+    right; attention would return without its outputs."""
+    import ctypes as C
+
+    lib = PKG.load_library()
+    calls = []
+    att = L.CacheAttendArgs(q=4096, out=8192, q_row=512, q_head=128, out_row=512, out_head=128, scale=0.1,
+                            dtype=L.DT_BF16, n_heads=4)
+    cache = L.Cache(4096, 4096, L.CACHE_BF16, 1, 4, 2, 128, 2, 4, 0)
+    for row0, n_rows, max_rows in ((None, 1, 0), (4096, 0, 0), (4096, 1, 0)):
+        r = L.CacheRows(4096, 4096, row0, 1, n_rows, max_rows)
+        calls.append(lib.fmd_cache_attend(C.byref(cache), 0, C.byref(r), C.byref(att), 4096, 1 << 40, None, None))
+    assert calls == [L.FMD_EINVAL, L.FMD_OK, L.FMD_OK]
