@@ -1069,7 +1069,8 @@ size_t cache_chunk_workspace(const CacheView& c) {
 cudaError_t launch_cache_chunk(bool bf16, const CacheView& c, int layer, const CacheRows& r, const CacheAttend& a,
                                void* workspace, int* status, cudaStream_t s) {
   const bool q4 = c.format == FMD_CACHE_Q4;
-  const CkShape sh = ck_shape(bf16, c, a.n_heads, r.n_seqs, a.max_rows);
+  // no sequence has more rows than the buffers, and every (sequence, tile) is looked at
+  const CkShape sh = ck_shape(bf16, c, a.n_heads, r.n_seqs, std::min(a.max_rows, r.n_rows));
   CUtensorMap map{};
   if (!q4 && !cache_tensor_map(&map, c, layer)) return cudaErrorNotSupported;
   CkArgs p;

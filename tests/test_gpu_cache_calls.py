@@ -228,3 +228,16 @@ def test_queries_at_the_ends_of_bf16_over_4_bits(e, count):
     kk, vv = ref.quantise(_np(k))[0], ref.quantise(_np(v))[0]
     want, mag = ref.attend(_np(q), kk, vv, range(n - count, n))
     assert (np.abs(_np(out) - want) <= ref.attend_tolerance(want, mag, _eps("bf16"), True)).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
+def test_max_rows_is_only_a_bound(kind):
+    """A caller that does not know the longest sequence may say the largest number."""
+    lengths = [90, 70, 300, 40] * 8
+    c, held = _filled(kind, "bf16", lengths)
+    counts = [40, 1, 33, 0] * 8
+    q = _rand(np.random.default_rng(0), sum(counts), 4, 128)
+    want = c.attend(0, _seq_rows(c, range(32), counts, lengths), q)
+    for most in (1000, 2**31 - 1):
+        assert torch.equal(c.attend(0, _seq_rows(c, range(32), counts, lengths, max_rows=most), q), want)
+    c.check()
