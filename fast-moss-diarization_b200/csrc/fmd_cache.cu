@@ -769,6 +769,9 @@ int fmd_cache_read(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows
   if (rc || (rc = check_rows(c, layer, rows))) return rc;
   if (empty(rows)) return FMD_OK;
   if (!k || !v || !aligned16(k) || !aligned16(v)) return FMD_EINVAL;
+  const int64_t elems = (int64_t)rows->n_rows * c->kv_heads * c->head_dim;
+  const uintptr_t ka = (uintptr_t)k, va = (uintptr_t)v;
+  if (std::max(ka, va) - std::min(ka, va) < (uint64_t)elems * sizeof(float)) return FMD_EINVAL;  // on one another
   if (!on_current_device(c->pool) || !on_current_device(k)) return FMD_EINVAL;
   // blocks of a row: as in append
   const int per_block = kReadThreads / (c->head_dim / 8) * 4, most = (2 * c->kv_heads + per_block - 1) / per_block;

@@ -116,7 +116,8 @@ typedef struct fmd_cache_append_args {
 int fmd_cache_append(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows,
                      const fmd_cache_append_args* args, int32_t* status, void* stream);
 
-/* The cached values of the rows' positions as f32, [n_rows][kv_heads][head_dim]. */
+/* The cached values of the rows' positions as f32, [n_rows][kv_heads][head_dim];
+ * k and v may not overlap (FMD_EINVAL). */
 int fmd_cache_read(const fmd_cache* c, int32_t layer, const fmd_cache_rows* rows, float* k, float* v,
                    int32_t* status, void* stream);
 

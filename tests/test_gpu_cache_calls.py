@@ -241,3 +241,19 @@ def test_max_rows_is_only_a_bound(kind):
     for most in (1000, 2**31 - 1):
         assert torch.equal(c.attend(0, _seq_rows(c, range(32), counts, lengths, max_rows=most), q), want)
     c.check()
+
+
+def test_read_outputs_that_overlap_are_refused():
+    c, _ = _filled("bf16", "bf16", [30])
+    rows = _seq_rows(c, [0], [30], [30])
+    want = c.read(0, rows)
+    n = 30 * 2 * 128
+    both = torch.zeros(2 * n, device="cuda")
+    view = lambda at: both[at:at + n].view(30, 2, 128)
+    for a, b in ((view(0), view(0)), (view(0), view(4)), (view(n - 4), view(0))):
+        with pytest.raises(PKG.FmdError) as e:
+            c.read(0, rows, k_out=a, v_out=b)
+        assert e.value.status == PKG._lib.FMD_EINVAL
+    assert not bool(both.any())
+    got = c.read(0, rows, k_out=view(n), v_out=view(0))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
