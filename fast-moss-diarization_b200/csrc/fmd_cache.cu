@@ -814,6 +814,7 @@ int fmd_cache_attend(const fmd_cache* c, int32_t layer, const fmd_cache_rows* ro
     return FMD_EINVAL;
   const int64_t need = fmd_cache_attend_workspace(c, a->n_heads, rows->n_seqs, rows->max_rows);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return FMD_EINVAL;
+  if (cache_units(view_of(c)) * c->kv_heads > INT32_MAX) return FMD_ENOTSUP;
   if (!on_current_device(c->pool) || !on_current_device(a->q)) return FMD_EINVAL;
   CacheAttend p{a->q,     a->out,     a->q_row,  a->q_head, a->out_row, a->out_head,
                 a->scale, a->n_heads, a->window, a->sinks,  rows->max_rows};

@@ -114,6 +114,9 @@ struct CacheAttend {
   float scale;
   int n_heads, window, sinks, max_rows;
 };
+// Units of a sequence in either form at most (32 keys each, and what stands for its fixed cost);
+// the units of all kv heads are numbered in 32 bits.
+inline long long cache_units(const CacheView& c) { return 2LL * c.max_pages + 16; }
 // fmd_cache_decode.cu: at most 16 (row, head) pairs per kv head and sequence
 bool cache_decode_fits(const CacheView& c, int n_heads, int max_rows);
 size_t cache_decode_workspace(const CacheView& c, int n_heads, int max_rows);

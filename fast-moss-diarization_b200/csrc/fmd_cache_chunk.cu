@@ -46,6 +46,7 @@
 // waits (bounded) for copies and MMAs in flight and frees tensor memory.
 #include <cuda.h>
 #include <float.h>
+#include <limits.h>
 
 #include <algorithm>
 
@@ -1049,7 +1050,8 @@ CkShape ck_shape(bool bf16, const CacheView& c, int n_heads, int n_seqs, int max
   const long long pairs = (long long)max_rows * (n_heads / c.kv_heads);
   s.tiles = (int)((pairs + 255) / 256);
   const long long entries = (long long)s.tiles * n_seqs;
-  s.split = entries <= kCkEntries && entries * c.kv_heads <= FMD_CACHE_WORKSPACE_ZERO / 4;
+  s.split = entries <= kCkEntries && entries * c.kv_heads <= FMD_CACHE_WORKSPACE_ZERO / 4 &&
+            entries * cache_units(c) <= INT_MAX;
   const bool q4 = c.format == FMD_CACHE_Q4;
   const int tb = 64 * c.head_dim * 2, stage = 2 * (int)c.block_bytes();
   s.stages = 4;

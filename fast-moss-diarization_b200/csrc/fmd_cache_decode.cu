@@ -31,6 +31,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <float.h>
+#include <limits.h>
 
 #include <algorithm>
 
@@ -1063,6 +1064,7 @@ cudaError_t launch_cache_decode(bool bf16, const CacheView& c, int layer, const 
   p.counters = (int*)workspace;
   p.part = (float*)workspace + kDcCounters;
   p.seqs = std::min(kDcSeqs, kDcCounters / c.kv_heads);
+  p.seqs = (int)std::min<long long>(p.seqs, INT_MAX / (cache_units(c) * c.kv_heads));  // >= 1, as the caller has seen to
   p.stages = sh.stages;
   p.red_off = sh.red_off;
   p.red_row = sh.red_row;

@@ -143,7 +143,8 @@ int64_t fmd_cache_attend_workspace(const fmd_cache* c, int32_t n_heads, int32_t 
  * with window == 0, j > p - window or j < sinks: softmax(scale q . k_j) weighted
  * sum of the values. The row's own key is in the cache (append first). Pages
  * outside every row's window and sinks are not looked up. Softmax statistics and
- * sums are f32. What a cached position that no row of the call sees holds, NaN
+ * sums are f32. kv_heads x (2 max_pages_per_slot + 16) is below 2^31 (FMD_ENOTSUP).
+ * What a cached position that no row of the call sees holds, NaN
  * included, has no influence. `workspace` is 16-byte aligned; its first
  * FMD_CACHE_WORKSPACE_ZERO bytes are zero before its first use, and every call
  * leaves them zero, so calls of any shape and cache may take turns with it (after

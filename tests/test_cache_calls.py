@@ -223,3 +223,23 @@ def test_sequences_of_one_row_need_max_rows_of_one():
         r = L.CacheRows(4096, 4096, row0, 1, n_rows, max_rows)
         calls.append(lib.fmd_cache_attend(C.byref(cache), 0, C.byref(r), C.byref(att), 4096, 1 << 40, None, None))
     assert calls == [L.FMD_EINVAL, L.FMD_OK, L.FMD_OK]
+
+
+def test_attention_counts_its_units_in_32_bits():
+    """Units of 32 keys of all kv heads of a sequence are numbered in 32 bits: slots whose
+    positions could pass that are refused, however long the sequences are."""
+    import ctypes as C
+
+    lib = PKG.load_library()
+    r = C.byref(L.CacheRows(4096, 4096, None, 1, 1, 1))
+
+    def attend(kv_heads, pages):
+        cache = L.Cache(4096, 4096, L.CACHE_BF16, 1, 4, kv_heads, 128, 2, pages, 0)
+        att = L.CacheAttendArgs(q=4096, out=1 << 30, q_row=kv_heads * 128, q_head=128, out_row=kv_heads * 128, out_head=128,
+                                scale=0.1, dtype=L.DT_BF16, n_heads=kv_heads)
+        return lib.fmd_cache_attend(C.byref(cache), 0, r, C.byref(att), 4096, 1 << 40, None, None)
+
+    for kv_heads, pages in ((64, 2**24), (1024, 2**20), (32, 2**25 - 1)):
+        assert attend(kv_heads, pages) == L.FMD_ENOTSUP, (kv_heads, pages)
+    for kv_heads, pages in ((64, 2**24 - 9), (1024, 2**20 - 9), (1, 2**25 - 1), (8, 2**25 - 1)):
+        assert attend(kv_heads, pages) == L.FMD_EINVAL, (kv_heads, pages)  # host memory is not a pool
