@@ -16,6 +16,9 @@ A decode loop:
     for layer in range(layers):
         q = cache.append(layer, rows, k, v, q=q, q_norm=..., cos=..., sin=...)
         out = cache.attend(layer, rows, q, window=4096, sinks=4)
+
+A captured step keeps its rows and moves them on itself (`rows.advance()` in the
+graph); `cache.advance(slots)` before each replay keeps the books.
 """
 
 from __future__ import annotations
@@ -393,7 +396,9 @@ class PagedCache:
         `sin[position]` (f32 tables; pairs i and i + half, or neighbours if
         `interleaved`) applied to queries and keys in the same pass. Returns the
         normed and rotated queries (`q_out`, which may be `q`), or None without
-        `q`. f32 arithmetic, one rounding per value."""
+        `q`; rows of padding and behind the last sequence are left as they were in
+        `q_out`, and hold anything without it. f32 arithmetic, one rounding per value.
+        No gradients: operators of the cache are for inference."""
         if not 0 <= layer < self.layers:
             _fail(f"layer {layer} is out of range")
         code, dtype, n = self._dtype(k, "k"), k.dtype, k.shape[0]

@@ -163,7 +163,7 @@ FMD_DEV uint32_t quantise8(float (&x)[8], bool key, __half& scale) {
 // values' heads are passed over one after the other, so that what is done with a
 // head is the same for the whole block. 10,007 rows of 16 + 8 + 8 heads with norms and
 // rotation, 16 bits: 34.7 us, 4.9 TB/s; 16,384 rows of 8 + 8 heads into 4 bits 35.7 us, 2.4
-// TB/s, the quantiser's instructions. One row: 2.6 us, 64 rows 2.9.
+// TB/s, the quantiser's instructions. One row: 2.8 us, 64 rows 3.0 (back to back).
 template <typename T, int D, bool Q4, int HPG>
 __global__ void __launch_bounds__(kRowThreads, kRowBlocks)
     k_cache_append(CacheView c, int layer, CacheRows r, CacheAppend a, int* status) {

@@ -33,10 +33,16 @@
 // Registers go where they are needed: the softmax groups take what the others give.
 // Values of positions that no pair of the item sees are cleared in shared memory
 // before the product, so that what they hold (NaN x 0) has no influence.
-// Measured (16 query heads to 8 kv heads of 128): 2,048 rows behind 8,192 positions
-// 138 us, 870 TFLOP/s; two such chunks over a window of 4,096 168.5 us, 817 TFLOP/s;
-// 2,001 f16 rows behind 9,001 positions in 4 bits 234 us, 560 TFLOP/s of the 4 x head_dim a
-// key (twice the products of P V are issued there). A key tile of A and B takes 2,000
+// Roundings: P enters its product as one 16-bit term, as in the decoder's prefill attention,
+// and from 16 bits that shows: outputs are off by 2.3e-3 of their magnitude (rms; f16 2.9e-4)
+// where their own rounding alone is 1.7e-3 (2.1e-4). With a second term for what the first
+// leaves out, as the decode form has, 1.7e-3 as well, but 220 us instead of 180 for the two
+// chunks below.
+// Measured (16 query heads to 8 kv heads of 128), launches back to back: 2,048 rows behind
+// 8,192 positions 170 us, 909 TFLOP/s; two chunks of 2,048 behind 3,952 and 12,288 positions,
+// window 4,096, 175 us, 786 TFLOP/s; the last 2,001 f16 rows of 9,001 positions in 4 bits 249 us,
+// 527 TFLOP/s of 4 x head_dim a key (twice the products of P V are issued there). With inputs
+// cold in L2 the last two take 180 and 255 us. A key tile of A and B takes 2,000
 // cycles (4 bits: 3,900), an item's queries and outputs 8,000 more. Of the 2,000, a
 // softmax warp spends 900 on its exponentials, the special-function unit half busy with
 // those of A and B; no pipe is full (tensor 44 %, issue 37 %). A quarter of the
@@ -66,8 +72,9 @@ constexpr int kCkConv = 4;  // converter warps (4 bits)
 constexpr int ck_threads(bool q4) { return 384 + (q4 ? kCkConv * 32 : 0); }
 // Registers of a thread at launch, of a softmax thread, of any other; the sums fit.
 //   16 bits: 384 x 168 = 256 x 208 + 128 x 88; 4 bits: 512 x 128 = 256 x 192 + 256 x 64.
-// Eight converter warps leave 152 to a softmax thread, which then spills: 2,048 rows over 2,048
-// to 4,096 keys 62 us instead of 55.5, the f16 chunk above 241 instead of 234.
+// Eight converter warps leave 152 to a softmax thread, which then spills more: 241 us instead of
+// 234 for the f16 chunk above. As it is, the compiler reports 60 bytes of spill stores a thread
+// (16 bits) and 72 to 80 (4 bits).
 template <int N> FMD_DEV void ck_more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
 template <int N> FMD_DEV void ck_fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
 
@@ -331,8 +338,8 @@ __global__ void __launch_bounds__(ck_threads(Q4), 1)
   constexpr int NB = D / 32;
   constexpr int kMore = Q4 ? 192 : 208, kFew = Q4 ? 64 : 88;
   // f16 outputs of a 4-bit cache: P and V go in as two f16 terms each (their roundings,
-  // 2^-11 each as the output's, would be two of the three that f16 operands cost;
-  // error against 64 bits 3.8e-4 without, 2.1e-4 for the output's rounding alone)
+  // 2^-11 each as the output's, would be two of the three that f16 operands cost; error
+  // against 64 bits 2.7e-4 so, 3.8e-4 without, 2.1e-4 for the output's rounding alone)
   constexpr bool kFine = Q4 && !Act<T>::kIsBf16;
   constexpr int CVB = (kFine ? 3 : 2) * TB;  // an operand buffer: K | V (| V's second term)
   constexpr float kPScale = Act<M>::kIsBf16 ? 0.f : 7.f;      // log2 factor of P (f16 subnormals start at 2^-14)

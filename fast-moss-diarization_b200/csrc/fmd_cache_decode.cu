@@ -24,10 +24,10 @@
 //   S^T = K Q^T: A = 16 keys x 16 dims, B = the queries.
 //   O^T += V^T P^T: A = 16 dims x 16 keys, B = P^T, turned with movmatrix.
 //
-// Measured (8 kv heads of 128, 16 query heads): 64 sequences of 8,192 positions
-// 316 us from 16 bits, 6.8 TB/s, and 153 us from 4 bits, 3.9 TB/s; one sequence over
-// 4,096 positions 12.5 us (16 bits), over 16,384 20 us (4 bits), of which launch,
-// lookup and first loads are 6 and the merge of 34 and 74 pieces 4 and 6.
+// Measured (8 kv heads of 128, 16 query heads, launches back to back): 64 sequences of 8,192
+// positions 326 us from 16 bits, 6.6 TB/s, and 166 us from 4 bits, 3.6 TB/s; one sequence over
+// 4,096 positions 11.6 us (16 bits), over 16,384 18 us (4 bits), of which launch, lookup and
+// first loads are 6 and the merge of 34 and 74 pieces 4 and 6.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <float.h>
@@ -429,8 +429,8 @@ FMD_DEV void dc_store(float* red, int tile_rows, int nq, const float (&o)[NT][D 
 // rounding (half a step: 2^-9 for bf16, 2^-12 for f16) does not show: the products are not
 // the bound. Error against 64 bits in f16 2.1e-4 of the output, that of its one rounding;
 // 2.9e-4 with one term, 71.5 us instead of 72 for the 64 streams below.
-// 64 streams of 300 .. 16,384 positions over their newest 2,048 and 64 sinks: 74 us,
-// 408 MB at 5.5 TB/s.
+// 64 streams of 300 .. 16,384 positions over their newest 2,048 and 64 sinks: 72 us,
+// 408 MB at 5.7 TB/s. At head_dim 128 more than 8 pairs spill 36 bytes a thread.
 
 constexpr int kDc16Threads = 160;
 
@@ -634,7 +634,8 @@ __global__ void __launch_bounds__(kDc16Threads, 2)
 // with one, of which the output's rounding is 2.07e-4 (4,096 normal keys).
 // Units of 64 keys, with half the copies and waits, took 142 us instead of 153 for 64
 // sequences of 8,192 positions, but 70 instead of 63 for 256 of 500 and 358 instead of
-// 261 with 16 query heads to a kv head, whose scores then spill.
+// 261 with 16 query heads to a kv head, whose scores then spill. Units of 32 keys spill as
+// well at head_dim 128: 36 to 52 bytes a thread up to 8 pairs, 228 above.
 // 62 % of the issue slots are used (16 warps an SM, 128 registers): what is left are the
 // latencies between an instruction and the next of the same warp.
 

@@ -128,7 +128,8 @@ class Qwen3Decoder:
         """`Qwen3::new_caches` sizing: a paged pool of `max_tokens` positions for
         `max_slots` sequences; up to `max_rows` token rows per forward pass. `kv`:
         "act" (the activation dtype) or "q4" (4 bits); with `window` > 0 a position
-        sees the newest `window` positions and the first `sinks` (`fmd_kv_options`)."""
+        sees the newest `window` positions and the first `sinks` (`fmd_kv_options`);
+        slots keep all their pages all the same."""
         fmt = {"act": _lib.KV_ACT, "q4": _lib.KV_Q4}.get(kv)
         if fmt is None:
             raise _lib.FmdError(_lib.FMD_EINVAL, f"kv must be 'act' or 'q4', not {kv!r}")

@@ -143,7 +143,10 @@ int64_t fmd_cache_attend_workspace(const fmd_cache* c, int32_t n_heads, int32_t 
  * with window == 0, j > p - window or j < sinks: softmax(scale q . k_j) weighted
  * sum of the values. The row's own key is in the cache (append first). Pages
  * outside every row's window and sinks are not looked up. Softmax statistics and
- * sums are f32. kv_heads x (2 max_pages_per_slot + 16) is below 2^31 (FMD_ENOTSUP).
+ * sums are f32. Probabilities meet the values as 16-bit numbers: as two terms each
+ * in calls of up to 16 (row, query head) pairs per kv head and sequence over 16 bits
+ * and for f16 rows over 4 bits, else as one. 4-bit values, and the queries that meet
+ * 4-bit keys, are rounded to f16.
  * What a cached position that no row of the call sees holds, NaN
  * included, has no influence. `workspace` is 16-byte aligned; its first
  * FMD_CACHE_WORKSPACE_ZERO bytes are zero before its first use, and every call

@@ -167,8 +167,9 @@ int fmd_load_weights(fmd_handle* h, const fmd_weights* w);
  * qwen3.rs:33-108). `format`: FMD_KV_ACT (the activation dtype, the default) or
  * FMD_KV_Q4 (4.5 bits a value, fmd_cache.h: 3.6 times the positions in the same
  * memory, plus one layer of 16-bit staging). `window` > 0: a position p sees the
- * positions j > p - window and, of the older ones, the first `sinks`. Positions
- * keep their rotation. Steps with either option run their attention on the
+ * positions j > p - window and, of the older ones, the first `sinks`: they are not
+ * read, but a slot keeps all its pages until it is released. Positions keep their
+ * rotation. Steps with either option run their attention on the
  * operators of fmd_cache.h; the persistent layer tail and split decode steps are
  * off then. */
 #define FMD_KV_ACT 0
@@ -216,9 +217,9 @@ int fmd_slot_release(fmd_handle* h, int32_t slot);
  * layer. No reference counterpart. FMD_ENOMEM when the pool has too few free
  * pages for the rest. */
 int fmd_slot_fork(fmd_handle* h, int32_t src, int32_t dst, int32_t capacity);
-/* Move the pages of the open slots to the front of the pool (the number in use
- * goes to *n_used, which may be NULL): what they hold is then one range of each
- * layer, for a snapshot of the pool. Not while an engine run is under way. */
+/* Move the pages of the open slots to the front of the pool, in one range of each
+ * layer; the number in use goes to *n_used, which may be NULL. Results do not
+ * depend on it. Not while an engine run is under way. */
 int fmd_kv_compact(fmd_handle* h, int32_t* n_used);
 /* Current cached length of a slot (`KvCache::len`, qwen3.rs:57-59). */
 int fmd_slot_len(fmd_handle* h, int32_t slot, int32_t* len);
