@@ -40,6 +40,12 @@ inline bool meet(const HeadRows& a, const HeadRows& b) {
   const int64_t row = a.n_rows > 1 || b.n_rows > 1 ? a.row : 0;
   if ((a.n_rows > 1 || b.n_rows > 1) && a.row != b.row) return true;
   if (a.dim != b.dim) return true;
+  // side by side in every row: of the heads of one fused row, for instance
+  const __int128 ea = (__int128)(a.n_heads - 1) * a.head + a.dim, eb = (__int128)(b.n_heads - 1) * b.head + b.dim;
+  if (row > 0 && ea <= row) {
+    const __int128 d = gap >= 0 ? gap % row : (row - -gap % row) % row;
+    if (d >= ea && d + eb <= row) return false;
+  }
   auto near = [&](__int128 x) {  // whether heads x apart in some two rows overlap
     if (row == 0) return x < a.dim && -x < a.dim;
     const __int128 lo = -(b.n_rows - 1), hi = a.n_rows - 1;  // row of a less row of b
