@@ -933,8 +933,9 @@ int sync_check(fmd_handle* h) {
     e = cudaMemcpy(st, h->d_status, 2 * sizeof(int), cudaMemcpyDeviceToHost);
     if (e != cudaSuccess) return fail(h, FMD_EIO, std::string("status read: ") + cudaGetErrorString(e));
     if (st[0] != 0) {
-      cudaMemset(h->d_status, 0, 2 * sizeof(int));
-      if (h->cache_ws) cudaMemset(h->cache_ws, 0, FMD_CACHE_WORKSPACE_ZERO);
+      // on the steps' stream, which does not wait for the legacy one
+      cudaMemsetAsync(h->d_status, 0, 2 * sizeof(int), h->stream);
+      if (h->cache_ws) cudaMemsetAsync(h->cache_ws, 0, FMD_CACHE_WORKSPACE_ZERO, h->stream);
       return fail(h, st[0], device_status_text(st[0], st[1]));
     }
   }
