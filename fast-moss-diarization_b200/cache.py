@@ -581,7 +581,9 @@ class PagedCache:
 
     def evict(self, slot: int, window: int, sinks: int = 0) -> int:
         """Free the slot's pages that no later row sees with this window and
-        sinks; returns how many. `attend` must not be given more afterwards."""
+        sinks; returns how many. `attend` must not be given more afterwards. Later
+        rows are those behind the slot's length: call it after the launches of the
+        rows that `step` or `advance` gave out."""
         if window < 1 or sinks < 0:
             _fail("window must be >= 1 and sinks >= 0")
         pages, n = self._open(slot), self._length[slot]
